@@ -248,7 +248,7 @@ def _quantise(x):
     """(n, kv heads, dims) fp32 to codes and the groups' fp16 scales and minima."""
     x = x.unflatten(-1, (-1, GROUP))
     low = x.amin(-1).half()
-    scale = ((x.amax(-1) - low.float()) / 15).clamp(min=0).half()
+    scale = ((x.amax(-1) - low.float()) / x.new_full((), 15)).clamp(min=0).half()
     s = scale.double()[..., None]
     t = torch.where(s > 0, (x.double() - low.double()[..., None]) / s, 0.0)
     return t.round().clamp(0, 15).to(torch.int32).flatten(-2), scale, low
