@@ -265,6 +265,35 @@ SIGNATURES["csdr_hsda_build"] = (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _vp, C.c
 SIGNATURES["csdr_free_buffer"] = (None, [_vp])
 
 
+class PagedKV(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_table", C.c_void_p),
+        ("lens", C.c_void_p), ("kv_dtype", C.c_int), ("page_size", C.c_int),
+        ("n_pages", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+        ("n_seqs", C.c_int), ("table_stride", C.c_int),
+    ]
+
+
+class AttnOptions(C.Structure):
+    _fields_ = [("softcap", C.c_float), ("window", C.c_int), ("slopes", C.c_void_p),
+                ("prefix", C.c_void_p)]
+
+
+_i64 = C.c_int64
+SIGNATURES.update({
+    "csdr_paged_page_bytes": (_sz, [C.c_int] * 4),
+    "csdr_paged_append": (C.c_int, [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int,
+                                    _i64, _i64, _i64, C.c_float, _vp, _vp]),
+    "csdr_paged_read": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "csdr_paged_attn_workspace_bytes": (_sz, [_vp, C.c_int, _vp, C.c_int, C.c_int, C.c_int]),
+    "csdr_paged_attn": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, _i64, C.c_int,
+                                  C.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "csdr_token_logprobs_workspace_bytes": (_sz, [C.c_int, C.c_int, C.c_int]),
+    "csdr_token_logprobs": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _i64, C.c_float, _vp, _vp,
+                                      _vp, C.c_int, _vp, _vp, _vp, _sz, _vp]),
+})
+
+
 def _hip_runtimes_mapped() -> set[str]:
     paths = set()
     try:

@@ -1,0 +1,59 @@
+"""Log probabilities of given tokens, entropy and the most likely tokens of rows of logits
+(csdr_token_logprobs): what a scored text (perplexity) or an answer with alternatives needs beside
+the token that select_best_from_logits (api/cortex_sdk.cpp:1005-1030) picks from the same scores.
+"""
+from __future__ import annotations
+
+import typing
+
+from . import _lib
+from .hsdr import _check, _stream_ptr, _torch
+from .paged import _dtype, _on_device
+
+
+class TokenLogprobs(typing.NamedTuple):
+    logprobs: typing.Any      # (rows,) float32, None without tokens
+    entropy: typing.Any       # (rows,) float32, nats
+    top_ids: typing.Any       # (rows, top_n) int32, likeliest first; None without top_n
+    top_logprobs: typing.Any  # (rows, top_n) float32
+
+
+def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0, workspace=None,
+                   stream=None) -> TokenLogprobs:
+    """logits: (rows, n) float32 or float16 on the device, rows any stride apart; tokens: (rows,)
+    int32, negative for none. With `stream` the call runs there, ordered by the caller."""
+    torch = _torch()
+    lib = _lib.load()
+    dt = _dtype(logits)
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be (rows, n) with a row's values side by side")
+    rows, n = logits.shape
+    if rows > 1 and logits.stride(0) < n:  # an expanded tensor, or rows that overlap
+        raise ValueError("the rows of logits overlap")
+    if tokens is not None and (tokens.dtype != torch.int32 or tuple(tokens.shape) != (rows,) or
+                               not tokens.is_contiguous()):
+        raise ValueError("tokens must be a contiguous int32 tensor, one per row")
+    _on_device(torch, "tensors", logits, tokens, workspace)
+    dev = logits.device
+    if workspace is None:
+        need = lib.csdr_token_logprobs_workspace_bytes(rows, n, top_n)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    out = torch.empty((2 + 2 * max(top_n, 0), rows), dtype=torch.float32, device=dev)
+    lp = out[0] if tokens is not None else None
+    ids = top = None
+    if top_n > 0:
+        ids = out[2:2 + top_n].view(torch.int32).view(rows, top_n)
+        top = out[2 + top_n:].view(rows, top_n)
+    _check(lib.csdr_token_logprobs(
+        logits.data_ptr(), dt, rows, n, logits.stride(0) if rows > 1 else 0, temperature,
+        tokens.data_ptr() if tokens is not None else None,
+        lp.data_ptr() if lp is not None else None, out[1].data_ptr(), top_n,
+        ids.data_ptr() if top_n > 0 else None, top.data_ptr() if top_n > 0 else None,
+        workspace.data_ptr() if workspace is not None else None,
+        workspace.numel() * workspace.element_size() if workspace is not None else 0,
+        _stream_ptr(stream)))
+    if stream is not None:
+        out.record_stream(stream)
+        if workspace is not None:
+            workspace.record_stream(stream)
+    return TokenLogprobs(lp, out[1], ids, top)

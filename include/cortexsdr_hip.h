@@ -66,6 +66,8 @@ extern "C" {
 /* ---- element types of activation buffers ---- */
 #define CSDR_F32 0
 #define CSDR_F16 1
+/* 4-bit elements of a paged K/V cache (csdr_paged_kv only) */
+#define CSDR_Q4 2
 
 /* Last error message of the calling thread ("" when none). */
 CSDR_API const char* csdr_last_error(void);
@@ -544,6 +546,119 @@ CSDR_API int csdr_lazy_hsdr_select(const csdr_lazy_hsdr* h, const float* hidden,
                                    int* tokens, int* pos_dev, uint8_t* repeated_update,
                                    float* scores, void* workspace, size_t workspace_bytes,
                                    void* hip_stream);
+
+/* ======================================================================
+ * Paged K/V cache: sequences of different lengths over shared pools of pages
+ *
+ * The cached form flash_attention.cpp:165-247 intends, for serving: in place of one contiguous
+ * cache per sequence (csdr_rope_kv_rows, csdr_attn_decode, csdr_attn_prefill), each sequence has a
+ * row of page ids, and a call takes one token or many of each of its sequences. fp16 pages, or
+ * 4-bit ones of 5/16 the size (a scale and a minimum per position and 32 dims).
+ * ==================================================================== */
+
+/* Sequences over a cache. A page holds page_size positions of every KV head;
+ * csdr_paged_page_bytes gives the bytes of a K page (a V page has as many), and both pools hold
+ * n_pages of them, one behind the other, 16-byte aligned. Sequence b's position p is in page
+ * page_table[b * table_stride + p / page_size]; an entry outside [0, n_pages), or one past the
+ * row's end, is a page that holds nothing: its positions are neither written nor attended to.
+ * Sequences may share pages that no call in flight appends to. lens[b]: positions of sequence b
+ * including the tokens of the call (device memory, as page_table, so a captured step can advance
+ * them). A page's layout, per KV head:
+ *   CSDR_F16  K [position][dim], V [position / 8][dim][position % 8], fp16
+ *   CSDR_Q4   codes, then the scales [dim / 32][position] and the minima [dim / 32][position],
+ *             fp16; a value is minimum + scale * code. Eight codes share a 32-bit word, code e in
+ *             bits 4 (e / 2) + 16 (e % 2) and up: K, per position, words [dim % 32 / 8][dim / 32]
+ *             of 8 dims; V, per 8 positions, words [dim % 16][dim / 16] of those positions. */
+typedef struct csdr_paged_kv {
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table; /* n_seqs x table_stride */
+    const int32_t* lens;       /* n_seqs */
+    int kv_dtype;              /* CSDR_F16 or CSDR_Q4 */
+    int page_size;             /* a power of two from 16 to 4096 */
+    int n_pages, n_kv_heads;
+    int head_dim;              /* 64 or 128 */
+    int n_seqs, table_stride;  /* table_stride * page_size at most 2^30 */
+} csdr_paged_kv;
+
+/* Bytes of one K page (and of one V page); 0 for a shape that is not supported. */
+CSDR_API size_t csdr_paged_page_bytes(int kv_dtype, int page_size, int n_kv_heads, int head_dim);
+
+/* The tokens of a call are n_tokens rows. q_start NULL: n_tokens / n_seqs rows of each sequence,
+ * sequence-major. Else n_seqs + 1 row numbers (device): sequence b has rows q_start[b] up to
+ * q_start[b + 1], none if they are equal, and max_q (host) is the most that one has; rows past
+ * max_q of a sequence and rows behind the last sequence are left as they were. Row i of the n rows
+ * of a sequence is its position lens[b] - n + i; a row whose position is negative is no token.
+ *
+ * csdr_paged_append: q (Hq heads) and k are rotated on adjacent pairs at their positions
+ * (apply_rope_inplace, cortex_sdk.cpp:1395-1423; angles in fp64, theta 0: not at all), k and v
+ * written to the cache, q to q_out (n_tokens x Hq x head_dim, not overlapping an input unless it
+ * is q with its own layout). q and q_out may both be NULL. q, k, v and q_out are of `dtype`
+ * (CSDR_F32 or CSDR_F16); q_stride, k_stride, v_stride: elements from one token to the next, 0 for
+ * packed rows, so that all three may lie in one projection's output. 4 bits: per group of 32 dims
+ * minimum = fp16(min), scale = fp16((max - minimum) / 15), code = the nearest, ties to even; a
+ * group with a value that is not finite, or past fp16, reads as NaN. */
+CSDR_API int csdr_paged_append(const csdr_paged_kv* kv, const void* q, const void* k,
+                               const void* v, int dtype, int n_tokens, const int32_t* q_start,
+                               int max_q, int Hq, int64_t q_stride, int64_t k_stride,
+                               int64_t v_stride, float theta, void* q_out, void* hip_stream);
+/* The tokens' cached rows as values: k and v n_tokens x n_kv_heads x head_dim of `dtype`, zeros
+ * for a position that the cache does not hold. */
+CSDR_API int csdr_paged_read(const csdr_paged_kv* kv, int n_tokens, const int32_t* q_start,
+                             int max_q, void* k, void* v, int dtype, void* hip_stream);
+
+/* How scores are formed and which positions are seen. All zero (or NULL for the struct): causal
+ * softmax(q.K^T * scale). */
+typedef struct csdr_attn_options {
+    float softcap;         /* > 0: score = softcap * tanh(score / softcap) */
+    int window;            /* > 0: of the positions up to its own, a token sees the last `window` */
+    const float* slopes;   /* Hq floats (device), or NULL: score -= slope * |distance| */
+    const int32_t* prefix; /* n_seqs ints (device), or NULL: every token of sequence b sees the
+                            * first prefix[b] positions, those past its own and those left of
+                            * the window too */
+} csdr_attn_options;
+
+/* out (n_tokens x Hq x head_dim, of dtype) = softmax attention of the tokens (rotated queries q,
+ * as csdr_paged_append writes them) to the positions of their sequences that they see, after the
+ * call's tokens were appended; GQA as repeat_kv_heads (cortex_sdk.cpp:1453-1478); scale 0 =
+ * 1/sqrt(head_dim). A row that sees nothing is zero. What a token does not see has no influence on
+ * it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
+ * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
+ * right, with less parallelism).
+ *
+ * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
+ * CSDR_F16: weights rounded to fp16 once, fp32 sums. workspace:
+ * csdr_paged_attn_workspace_bytes (may be 0) device bytes, 16-byte aligned, needed by this call
+ * only: calls that may run at the same time need one each. */
+CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_tokens,
+                                                const int32_t* q_start, int max_q, int Hq,
+                                                int max_len);
+CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
+                             const int32_t* q_start, int max_q, int Hq, int64_t q_stride,
+                             int max_len, float scale, const csdr_attn_options* options, void* out,
+                             void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* ======================================================================
+ * Log probabilities
+ * ==================================================================== */
+
+/* For each of `rows` rows of n logits (dtype CSDR_F32 or CSDR_F16, row_stride elements apart, 0 =
+ * n), y = logits / temperature (temperature <= 0: 1, as select_best_from_logits,
+ * cortex_sdk.cpp:1005-1030): logprobs[r] = y[tokens[r]] - log sum exp y (tokens NULL: not
+ * computed; a negative token: 0; one >= n: NaN), entropy[r] = -sum p log p in nats (may be NULL),
+ * and the top_n (0..64) largest y, largest first and lower ids first among equals:
+ * top_ids[r * top_n + i], top_logprobs likewise; ids -1 and -infinity where fewer tokens have a
+ * logit above -infinity. -infinity is a token that cannot be (probability 0, nothing in the
+ * entropy); a row of nothing else has log probabilities -infinity and entropy 0; a NaN or
+ * +infinity in a row makes its log probabilities and entropy NaN, and NaN is never among the
+ * top. workspace: csdr_token_logprobs_workspace_bytes device bytes, 16-byte aligned, for this
+ * call only. */
+CSDR_API size_t csdr_token_logprobs_workspace_bytes(int rows, int n, int top_n);
+CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
+                                 int64_t row_stride, float temperature, const int32_t* tokens,
+                                 float* logprobs, float* entropy, int top_n, int32_t* top_ids,
+                                 float* top_logprobs, void* workspace, size_t workspace_bytes,
+                                 void* hip_stream);
 
 /* ======================================================================
  * Containers: the .sdr archive, HSDC codes-only streams, the HSDA shared-dictionary archive
