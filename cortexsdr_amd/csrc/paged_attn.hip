@@ -9,7 +9,9 @@
 //   seen: p < len and (p < prefix or (p <= pq and pq - p < window));  out = softmax(s) V
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -110,19 +112,646 @@ __device__ void attend_row(const AttnArgs& a, int b, const SeqRows& r, int t, in
     for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (XT)(l == 0.0f ? 0.0f : o[c] / l);
 }
 
-template <int HD, bool Q4, typename XT>
-__global__ __launch_bounds__(64) void row_kernel(AttnArgs a) {
-    const int b = blockIdx.x / a.pv.max_q, t = blockIdx.x % a.pv.max_q;
-    const SeqRows r = csdr::seq_rows(a.pv, b);
-    if (t >= r.n) return;
-    attend_row<HD, Q4, XT>(a, b, r, t, blockIdx.y);
+// ---------------------------------------------------------------- few tokens: split positions
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 32;       // positions per step of a wave
+constexpr int kCols = 16;       // (token, query head) pairs per wave
+constexpr int kStepWaves = 4;
+constexpr float kLog2e = 1.44269504088896341f;
+// Weights are 2^(s - m + kBias) in the log2 domain, m a maximum that may lag kLag behind: at most
+// 2^15, near the top of fp16: a pair keeps its 22 bits down to 2^-17 of the largest weight (the
+// step of its low half is 2^-24). m moves, and the sums with it, only now and then. (With weights
+// of 2^8 as a rule, rows with a high maximum were 2e-5 to 1.6e-4 off.)
+constexpr float kLag = 1.0f, kBias = 14.0f;
+constexpr float kNoMax = -1e30f;
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 16 + code for the eight codes of a word: the codes shifted into an fp16 mantissa. `magic` is
+// 16.0 twice, in a vector register: with the mask that makes one and-or a pair.
+__device__ __forceinline__ h8 codes16(uint32_t w, uint32_t magic) {
+    u4 r;
+    r.x = ((w << 6) & 0x03C003C0u) | magic;
+    r.y = ((w << 2) & 0x03C003C0u) | magic;
+    r.z = ((w >> 2) & 0x03C003C0u) | magic;
+    r.w = ((w >> 6) & 0x03C003C0u) | magic;
+    return __builtin_bit_cast(h8, r);
+}
+
+// x times y (fp32 values with fp16 factors), rounded to fp16, and what the rounding left: both
+// straight from the exact product (v_fma_mix).
+template <bool PAIR>
+__device__ __forceinline__ void split8(const float* x, h8 y, h8& hi, h8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi[j] = (_Float16)fmaf(x[j], (float)y[j], 0.0f);
+        if constexpr (PAIR) lo[j] = (_Float16)fmaf(x[j], (float)y[j], -(float)hi[j]);
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi[j] = (_Float16)x[j];
+        if constexpr (PAIR) lo[j] = (_Float16)(x[j] - (float)hi[j]);
+    }
+}
+
+__device__ __forceinline__ float lanes16_max(float v) {  // over the four lanes of a column
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float lanes16_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// A tile's operands as they come from memory. Lane (c, g) = (lane % 16, lane / 16) holds, for the
+// scores, the rows of positions 8 (c / 4) + 4 t + c % 4 of tile t, and for the values positions
+// 8 g .. 8 g + 7.
+template <int HD, bool Q4>
+struct Tile;
+template <int HD>
+struct Tile<HD, false> {
+    h8 k[2][HD / 32];  // dims 32 s + 8 g ..
+    h8 v[HD / 16];     // dim 16 d + c
+};
+template <int HD>
+struct Tile<HD, true> {
+    uint32_t k[2][HD / 32], v[HD / 16];
+    h8 par;  // piece `lane` of the tile's 64 pieces of scales and minima (see TileParams)
+};
+
+// A tile's scales and minima, 16-byte pieces of 8 positions: piece 4 r + i holds positions 8 i ..
+// of row r: K's scales of the HD / 32 groups, K's minima, then from piece 32 V's likewise. A lane
+// loads one piece; the wave shares them through LDS, where four lanes' addresses serve all 64
+// (loading what each lane needs took 14 loads and 56 registers a tile: 163 us -> MEASURED us for
+// 64 sequences of about 6000 positions).
+template <int HD>
+struct TileParams {
+    static constexpr int kMin = HD / 32, kV = 8;  // first rows
+    h8 piece[64];
+    __device__ h8 at(int row, int i) const { return piece[4 * row + i]; }
+};
+
+// Where a tile's data lie: a pointer for positions tb .. tb + 15 of the head and one for the rest
+// (the same page unless pages hold 16), and the lane's offsets, which do not change.
+struct Pages {
+    const uint8_t *a, *b;
+};
+template <int HD, bool Q4>
+struct LaneOffsets {
+    int k, v, par;  // bytes
+    bool khigh, high, parhigh, parv;
+    __device__ LaneOffsets(const PagedView& pv, int lane) {
+        const int c = lane & 15, g = lane >> 4, ps = pv.page_size();
+        khigh = c >= 8;
+        high = g >= 2;
+        const int slot = (8 * (c >> 2) + (c & 3)) & (ps - 1), s8 = (8 * g) & (ps - 1);
+        parv = lane >= 32;
+        parhigh = (lane & 3) >= 2;
+        if constexpr (!Q4) {
+            k = 2 * (slot * HD + 8 * g);
+            v = 2 * (s8 * HD + c * 8);
+            par = 0;
+        } else {
+            k = 4 * (slot * (HD / 8) + g * (HD / 32));
+            v = 4 * ((s8 >> 3) * HD + c * (HD / 16));
+            // minima follow the scales; HD 64 has four rows, and lanes that load one twice
+            const int row = (lane >> 2 & 7) % (2 * HD / 32);
+            par = csdr::scale_offset(HD, ps, row, (8 * (lane & 3)) & (ps - 1));
+        }
+    }
+};
+
+template <int HD, bool Q4>
+__device__ __forceinline__ Pages pages_of(const uint8_t* pool, const PagedView& pv, int kvh,
+                                          int page0, int page1) {
+    return Pages{pool + csdr::head_offset<Q4>(pv, HD, max(page0, 0), kvh),
+                 pool + csdr::head_offset<Q4>(pv, HD, max(page1, 0), kvh)};
 }
 
 template <int HD, bool Q4>
-void launch(const AttnArgs& a, int dtype, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)a.pv.n_seqs * a.pv.max_q), a.hq);
-    if (dtype == CSDR_F32) row_kernel<HD, Q4, float><<<grid, 64, 0, st>>>(a);
-    else row_kernel<HD, Q4, _Float16><<<grid, 64, 0, st>>>(a);
+__device__ __forceinline__ void load_k(Tile<HD, Q4>& t, const PagedView& pv, Pages p, int tb,
+                                       const LaneOffsets<HD, Q4>& at) {
+    const int ps = pv.page_size();
+    const int slot = tb & (ps - 1) & ~15;  // uniform; pages of 16: 0
+    if constexpr (!Q4) {
+        const uint8_t* hp = (at.khigh ? p.b : p.a) + slot * (HD * 2) + at.k;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int s = 0; s < HD / 32; ++s)
+                t.k[u][s] = *reinterpret_cast<const h8*>(hp + 2 * (4 * u * HD + 32 * s));
+    } else {
+        const uint8_t* hp = (at.khigh ? p.b : p.a) + slot * (HD / 2) + at.k;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            __builtin_memcpy(t.k[u], __builtin_assume_aligned(hp + 4 * u * (HD / 2), HD / 8), HD / 8);
+    }
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void load_v(Tile<HD, Q4>& t, const PagedView& pv, Pages p, int tb,
+                                       const LaneOffsets<HD, Q4>& at) {
+    const int ps = pv.page_size();
+    const int slot = tb & (ps - 1) & ~15;
+    const uint8_t* hp = at.high ? p.b : p.a;
+    if constexpr (!Q4) {
+        hp += slot * (HD * 2) + at.v;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) t.v[d] = *reinterpret_cast<const h8*>(hp + 256 * d);
+    } else {
+        __builtin_memcpy(t.v, __builtin_assume_aligned(hp + slot * (HD / 2) + at.v, 16), HD / 4);
+    }
+}
+
+template <int HD>
+__device__ __forceinline__ void load_par(Tile<HD, true>& t, const PagedView& pv, Pages k, Pages v,
+                                         int tb, const LaneOffsets<HD, true>& at) {
+    const int slot = tb & (pv.page_size() - 1) & ~15;
+    const uint8_t* a = at.parv ? v.a : k.a;
+    const uint8_t* b = at.parv ? v.b : k.b;
+    t.par = *reinterpret_cast<const h8*>((at.parhigh ? b : a) + 2 * slot + at.par);
+}
+
+// The eight halves of `v` whose bit of `live` is set, zero elsewhere.
+__device__ __forceinline__ h8 only(h8 v, uint32_t live) {
+    u4 w = __builtin_bit_cast(u4, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = (live >> (2 * i) & 1) ? 0x0000FFFFu : 0u;
+        const uint32_t hi = (live >> (2 * i + 1) & 1) ? 0xFFFF0000u : 0u;
+        w[i] &= lo | hi;
+    }
+    return __builtin_bit_cast(h8, w);
+}
+
+// Scores with the options, in the log2 domain; `x` the products q.k in units of 1 / unit.
+template <bool OPTS>
+__device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, float slope,
+                                        int dist) {
+    if constexpr (!OPTS) return x * unit;
+    float s = x * unit;
+    if (a.cap > 0.0f) {
+        const float t = s * a.inv_cap, b = fabsf(t);
+        // tanh: 1 - 2 / (e^2b + 1), absolutely exact to 2^-23, and its series for small b
+        const float e = exp2_fast(2.0f * kLog2e * b);
+        float y = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+        const float t2 = b * b;
+        const float p = b * fmaf(t2, fmaf(t2, fmaf(t2, -17.0f / 315, 2.0f / 15), -1.0f / 3), 1.0f);
+        y = b < 0.2f ? p : y;
+        s = a.cap * copysignf(y, t);
+    }
+    return (s - slope * (float)abs(dist)) * kLog2e;
+}
+
+struct Splits {
+    int len, n;  // positions per split, splits
+    float* stats;  // 2 per (row, head, split): exponent offset and sum
+    float* vecs;   // HD per (row, head, split)
+};
+
+// Split attention of up to 16 (token, head) columns of one KV head. One wave runs a softmax with
+// a running maximum over tiles of 32 positions, all operands straight from memory in the order
+// the matrix cores take them:
+//   S^T = K Q^T, two 16x16 tiles of rows = positions; lane (c, g) ends with column c's scores at
+//     positions 8 g .. 8 g + 7, which is just what it has to give as B operand of
+//   O^T += V^T P^T, whose A operand is a 16-byte piece of V's page.
+// So nothing crosses lanes but the maximum, and that only when it moves by more than kLag.
+// 4 bits: codes enter the products as whole numbers (16 + code for K, the -16 folded into the
+// accumulator's start; code - 8 for V, centred, so that sums do not cancel); K's scale and minimum
+// are applied to the group's 32-dim partial score, V's scale to the weights, its minimum through
+// a sum of its own per group. fp32 calls carry q and the weights as pairs of fp16 (22 bits).
+template <int HD, bool Q4, typename XT, bool OPTS>
+__global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Splits sp) {
+    constexpr bool PAIR = sizeof(XT) == 4;
+    constexpr int NS = HD / 32, ND = HD / 16;
+    const PagedView& pv = a.pv;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = a.hq / pv.hkv;
+    const int b = blockIdx.x / pv.hkv, kvh = blockIdx.x % pv.hkv, split = blockIdx.y;
+    const SeqRows r = csdr::seq_rows(pv, b);
+    const int col0 = blockIdx.z * kCols, ncol = min(r.n * G - col0, kCols);
+    if (ncol <= 0) return;
+    const Seen seen = seen_of(a, b, r);
+    const int col = col0 + min(c, ncol - 1);
+    const int h = kvh * G + col % G, pq = r.p0 + col / G;
+    const long long row = (long long)r.first + col / G;
+    const int pq0 = r.p0 + col0 / G, pq1 = r.p0 + (col0 + ncol - 1) / G;
+    const float slope = OPTS && a.slopes ? a.slopes[h] : 0.0f;
+
+    // positions that some column sees: below `first` only the prefix
+    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);
+    const int end = pq1 < 0 ? 0 : min(seen.keys, max(pq1 + 1, seen.prefix));
+    const int lo = split * sp.len, hi = split == sp.n - 1 ? end : min(end, lo + sp.len);
+    auto next_tile = [&](int tb) {  // the next tile that some column sees, or hi
+        tb += kTile * kStepWaves;
+        if (tb < hi && tb >= seen.prefix && tb + kTile <= first) {
+            const int skip = (first - kTile - tb) / (kTile * kStepWaves) + 1;
+            tb += skip * kTile * kStepWaves;
+            // (prefix tiles lie below tb already: nothing between is seen)
+        }
+        return tb;
+    };
+
+    // q: the B operand, dims 32 s + 8 g .. of column c. fp32: the row scaled by a power of two
+    // that puts its largest magnitude in [2^13, 2^14), then in pairs.
+    h8 qh[NS], ql[PAIR ? NS : 1];
+    float unit = OPTS ? a.scale : a.scale * kLog2e;
+    float qsum[Q4 ? NS : 1];
+    {
+        const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
+        float x[NS][8];
+        float big = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[s][j] = (float)qp[32 * s + 8 * g + j];
+                big = fmaxf(big, fabsf(x[s][j]));
+            }
+        float f = 1.0f;
+        if constexpr (PAIR) {
+            big = lanes16_max(big);
+            const int e = (int)(__float_as_uint(big) >> 23) - 127;
+            const int k = big > 0.0f ? min(max(13 - e, -120), 120) : 0;
+            f = __uint_as_float((uint32_t)(127 + k) << 23);
+            unit *= __uint_as_float((uint32_t)(127 - k) << 23);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            float y[8], t = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j] = x[s][j] * f;
+                t += y[j];
+            }
+            if constexpr (Q4) qsum[s] = lanes16_sum(t);
+            split8<PAIR>(y, qh[s], ql[PAIR ? s : 0]);
+        }
+    }
+
+    __shared__ TileParams<HD> params[Q4 ? kStepWaves : 1];
+    TileParams<HD>& tp = params[Q4 ? wave : 0];
+
+    f4 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 par = {0.f, 0.f, 0.f, 0.f};  // 4 bits: sums of weights times what code 8 stands for
+    float m = kNoMax, l = 0.0f;       // the (lagging) maximum, log2 domain; this lane's sum
+    // exponent above V's largest scale (from fp16's smallest): weights are 2^-ev of the above
+    float ev = Q4 ? -24.0f : 0.0f, vtop = 0x1p-24f;
+    uint32_t magic = 0x4C004C00u;
+    asm("" : "+v"(magic));  // (kept in a register)
+
+    const LaneOffsets<HD, Q4> at(pv, lane);
+    Tile<HD, Q4> t;
+    // One tile at tb (pages pg0, pg1); with MORE, the loads of the next one (nb, ng0, ng1) are
+    // issued as soon as its registers are free. (The last tile is code of its own: a loop whose
+    // loads and exit hang on one condition was compiled with registers of the tile overwritten.)
+    auto tile = [&](auto more, int tb, int pg0, int pg1, int nb, int ng0, int ng1) {
+        constexpr bool MORE = decltype(more)::value;
+        // the lane's positions that its column sees; whole tiles need no mask
+        const int p8 = tb + 8 * g;
+        const bool whole = pg0 >= 0 && pg1 >= 0 && pq0 >= 0 && tb + kTile <= seen.keys &&
+                           (tb + kTile <= seen.prefix || (tb + kTile - 1 <= pq0 && tb >= first &&
+                                                          pq1 - tb < seen.window));
+        uint32_t live = 0xFFu, mine = 0xFFu;  // seen by some column; by this one
+        uint32_t plive = 0u;                  // the same for the positions of the lane's piece
+        if (!whole) {
+            live = mine = 0u;
+            auto some = [&](int p) {
+                return p < seen.keys && (p < seen.prefix || (p >= first && p <= pq1));
+            };
+            if (Q4 && (at.parhigh ? pg1 : pg0) >= 0)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    plive |= (uint32_t)some(tb + 8 * (lane & 3) + j) << j;
+            if ((g >= 2 ? pg1 : pg0) >= 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int p = p8 + j;
+                    mine |= (uint32_t)(pq >= 0 && seen.at(pq, p)) << j;
+                    live |= (uint32_t)some(p) << j;
+                }
+            }
+        }
+
+        float vscale = 0.0f;  // the largest of V's scales that this lane loaded
+        if constexpr (Q4) {
+            if (!whole && at.parv) t.par = only(t.par, plive);
+            if (at.parv && (lane & 31) < 4 * NS)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) vscale = fmaxf(vscale, (float)t.par[j]);
+            tp.piece[lane] = t.par;
+        }
+
+        // scores of positions p8 + j
+        float s8[8];
+        f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if constexpr (!Q4) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[u][s], qh[s], acc[u], 0, 0, 0);
+                    if constexpr (PAIR)
+                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[u][s], ql[s], acc[u], 0, 0, 0);
+                }
+            } else {
+                const float z = -16.0f * qsum[s];
+                const h8 ks = tp.at(s, g), km = tp.at(TileParams<HD>::kMin + s, g);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const h8 kc = codes16(t.k[u][s], magic);
+                    f4 part = {z, z, z, z};
+                    part = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[s], part, 0, 0, 0);
+                    if constexpr (PAIR)
+                        part = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[s], part, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[u][i] = fmaf((float)ks[4 * u + i], part[i], acc[u][i]);
+                        acc[u][i] = fmaf((float)km[4 * u + i], qsum[s], acc[u][i]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s8[4 * u + i] = score2<OPTS>(a, acc[u][i], unit, slope, pq - (p8 + 4 * u + i));
+        if constexpr (MORE) {
+            const Pages kp = pages_of<HD, Q4>(pv.k, pv, kvh, ng0, ng1);
+            load_k<HD, Q4>(t, pv, kp, nb, at);
+            if constexpr (Q4)
+                load_par<HD>(t, pv, kp, pages_of<HD, Q4>(pv.v, pv, kvh, ng0, ng1), nb, at);
+        }
+
+        float top = kNoMax;
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(mine >> j & 1)) s8[j] = -INFINITY;
+            if constexpr (!Q4) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) t.v[d] = only(t.v[d], live);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, s8[j]);
+        bool move = top > m + kLag;
+        if constexpr (Q4) {
+            move = move || vscale > vtop;
+        }
+        if (__any(move)) {
+            const float mn = fmaxf(m, lanes16_max(top));
+            float en = ev;
+            if constexpr (Q4) {
+                const float big = wave_max(vscale);
+                if (big > vtop) {
+                    en = (float)((int)(__float_as_uint(big) >> 23) - 126);
+                    vtop = __uint_as_float((uint32_t)((int)en + 127) << 23);
+                }
+            }
+            const float f = exp2_fast((m + ev) - (mn + en));
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] *= f;
+            if constexpr (Q4) par *= exp2_fast(m - mn);
+            m = mn;
+            ev = en;
+        }
+        const float off = kBias - ev - m;
+        float w8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w8[j] = exp2_fast(s8[j] + off);
+            l += w8[j];
+        }
+        if constexpr (!Q4) {
+            h8 wh, wl;
+            split8<PAIR>(w8, wh, wl);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.v[d], wh, o[d], 0, 0, 0);
+                if constexpr (PAIR)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.v[d], wl, o[d], 0, 0, 0);
+            }
+        } else {
+            // value = scale (code - 8) + (8 scale + minimum): the second, of group c mod NS, as A
+            // operand, in two halves as well; its sum over positions is the same for the group's
+            // dims. (Scales and minima summed apart cancel: 7e-6 off in place of 7e-7.) Weights
+            // without 2^-ev, which would take them past fp16 where scales are small.
+            h8 ch, cl, wh, wl;
+            const h8 rs = tp.at(TileParams<HD>::kV + c % NS, g);
+            const h8 rm = tp.at(TileParams<HD>::kV + TileParams<HD>::kMin + c % NS, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float ctr = fmaf(8.0f, (float)rs[j], (float)rm[j]);
+                ch[j] = (_Float16)ctr;
+                cl[j] = (_Float16)(ctr - (float)ch[j]);
+            }
+            split8<PAIR>(w8, h8{} + (_Float16)vtop, wh, wl);
+            par = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, wh, par, 0, 0, 0);
+            par = __builtin_amdgcn_mfma_f32_16x16x32_f16(cl, wh, par, 0, 0, 0);
+            if constexpr (PAIR)
+                par = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, wl, par, 0, 0, 0);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                split8<PAIR>(w8, tp.at(TileParams<HD>::kV + s, g), wh, wl);
+#pragma unroll
+                for (int d = 2 * s; d < 2 * s + 2; ++d) {
+                    const h8 vc = codes16(t.v[d], magic) - (_Float16)24.0f;
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wh, o[d], 0, 0, 0);
+                    if constexpr (PAIR)
+                        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[d], 0, 0, 0);
+                }
+            }
+        }
+        if constexpr (MORE) load_v<HD, Q4>(t, pv, pages_of<HD, Q4>(pv.v, pv, kvh, ng0, ng1), nb, at);
+    };
+    int tb = next_tile(lo + kTile * (wave - kStepWaves));
+    if (tb < hi) {
+        auto pages_at = [&](int p, int& x, int& y) {
+            x = csdr::page_of(pv, b, p);
+            y = pv.shift == 4 ? csdr::page_of(pv, b, p + 16) : x;
+        };
+        int pg0, pg1, ng0 = -1, ng1 = -1;
+        pages_at(tb, pg0, pg1);
+        const Pages kp = pages_of<HD, Q4>(pv.k, pv, kvh, pg0, pg1);
+        const Pages vp = pages_of<HD, Q4>(pv.v, pv, kvh, pg0, pg1);
+        load_k<HD, Q4>(t, pv, kp, tb, at);
+        if constexpr (Q4) load_par<HD>(t, pv, kp, vp, tb, at);
+        load_v<HD, Q4>(t, pv, vp, tb, at);
+        int nb = next_tile(tb);
+        if (nb < hi) pages_at(nb, ng0, ng1);
+        while (nb < hi) {
+            // the page ids of the tile after the next are on their way during this one
+            const int nn = next_tile(nb);
+            int nng0, nng1;
+            pages_at(nn, nng0, nng1);  // (-1 past the table)
+            tile(std::true_type{}, tb, pg0, pg1, nb, ng0, ng1);
+            tb = nb;
+            pg0 = ng0;
+            pg1 = ng1;
+            nb = nn;
+            ng0 = nng0;
+            ng1 = nng1;
+        }
+        tile(std::false_type{}, tb, pg0, pg1, 0, 0, 0);
+    }
+
+    // join the waves: sums in units of 2^(m + ev)
+    __shared__ float stat[kStepWaves][2][kCols];
+    __shared__ float vec[kStepWaves][kCols][HD + 4];
+    l = lanes16_sum(l);
+    float corr[Q4 ? NS : 1];
+    if constexpr (Q4) {
+        // row 4 g + i of the product is group (4 g + i) mod NS
+        const float f = 1.0f / vtop;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) corr[s] = par[s] * f;
+    }
+    if (g == 0) {
+        stat[wave][0][c] = m + ev;
+        stat[wave][1][c] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if constexpr (Q4) o[d] += corr[d / 2];
+        *reinterpret_cast<f4*>(&vec[wave][c][16 * d + 4 * g]) = o[d];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ncol * HD; i += 64 * kStepWaves) {
+        const int cc = i / HD, d = i % HD;
+        float e = stat[0][0][cc];
+#pragma unroll
+        for (int w = 1; w < kStepWaves; ++w) e = fmaxf(e, stat[w][0][cc]);
+        float sum = 0.0f, den = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kStepWaves; ++w) {
+            const float f = exp2_fast(stat[w][0][cc] - e);
+            den = fmaf(f, stat[w][1][cc], den);
+            sum = fmaf(f, vec[w][cc][d], sum);
+        }
+        const int ci = col0 + cc;
+        const size_t part =
+            (((size_t)r.first + ci / G) * a.hq + kvh * G + ci % G) * sp.n + split;
+        sp.vecs[part * HD + d] = sum;
+        if (d == 0) {
+            sp.stats[2 * part] = e;
+            sp.stats[2 * part + 1] = den;
+        }
+    }
+}
+
+// Joins a row's splits, one workgroup of 1 or 4 waves per (token, head). A row whose sum is not
+// positive or whose result is not finite is done again position by position (attend_row): rows
+// that see nothing, NaN or infinities that a token sees or that lie in a shared tile unseen.
+template <int HD, bool Q4, typename XT>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Splits sp) {
+    constexpr int VPL = HD / 64;
+    const int b = blockIdx.x / a.pv.max_q, tq = blockIdx.x % a.pv.max_q, h = blockIdx.y;
+    const SeqRows r = csdr::seq_rows(a.pv, b);
+    if (tq >= r.n) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const long long row = (long long)r.first + tq;
+    const size_t part = ((size_t)row * a.hq + h) * sp.n;
+    const float* st = sp.stats + 2 * part;
+    const float* vec = sp.vecs + part * HD + VPL * lane;
+    float e = kNoMax;
+    for (int i = lane; i < sp.n; i += 64) e = fmaxf(e, st[2 * i]);
+    e = wave_max(e);
+    float den = 0.0f, num[VPL] = {};
+    for (int i0 = wave; i0 < sp.n; i0 += 8 * nw) {
+        float x[8][VPL], f[8], ls[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(i0 + k * nw, sp.n - 1);
+            f[k] = st[2 * i];
+            ls[k] = st[2 * i + 1];
+#pragma unroll
+            for (int v = 0; v < VPL; ++v) x[k][v] = vec[(size_t)i * HD + v];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float w = i0 + k * nw < sp.n ? exp2_fast(f[k] - e) : 0.0f;
+            den = fmaf(w, ls[k], den);
+#pragma unroll
+            for (int v = 0; v < VPL; ++v)
+                num[v] = i0 + k * nw < sp.n ? fmaf(w, x[k][v], num[v]) : num[v];
+        }
+    }
+    if (nw > 1) {
+        __shared__ float red[4][HD + 1];
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) red[wave][VPL * lane + v] = num[v];
+        if (lane == 0) red[wave][HD] = den;
+        __syncthreads();
+        if (wave > 0) return;
+        den = red[0][HD] + red[1][HD] + red[2][HD] + red[3][HD];
+#pragma unroll
+        for (int v = 0; v < VPL; ++v) {
+            const int i = VPL * lane + v;
+            num[v] = red[0][i] + red[1][i] + red[2][i] + red[3][i];
+        }
+    }
+    bool fine = den > 0.0f && den < INFINITY;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) fine = fine && fabsf(num[v]) < INFINITY;
+    if (!__all(fine)) {
+        attend_row<HD, Q4, XT>(a, b, r, tq, h);
+        return;
+    }
+    XT* out = static_cast<XT*>(a.out) + (row * a.hq + h) * HD + VPL * lane;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) out[v] = (XT)(num[v] / den);
+}
+
+// Positions per split: about 1024 workgroups in all (4 to a CU), 128 (a tile per wave) at least.
+Splits splits_of(const PagedView& pv, int hq, int max_len) {
+    Splits s{};
+    const long long len =
+        std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
+    const long long cols = ((long long)pv.max_q * (hq / pv.hkv) + kCols - 1) / kCols;
+    const long long wgs = (long long)pv.n_seqs * pv.hkv * cols;
+    const long long unit = kTile * kStepWaves;
+    long long each = (len * wgs + 1023) / 1024;
+    each = std::max(unit, (each + unit - 1) / unit * unit);
+    s.len = (int)std::min(each, (long long)csdr::kMaxPositions);
+    s.n = (int)((len + s.len - 1) / s.len);
+    return s;
+}
+
+size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
+    const size_t parts = (size_t)pv.n_tokens * hq * s.n;
+    return csdr::align_up(parts * 8, 16) + parts * hd * 4;
+}
+
+template <int HD, bool Q4, typename XT>
+void launch_step(const AttnArgs& a, const Splits& s, hipStream_t st) {
+    const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
+    const dim3 grid(a.pv.n_seqs * a.pv.hkv, s.n, (cols + kCols - 1) / kCols);
+    if (a.cap > 0.0f || a.slopes)
+        step_kernel<HD, Q4, XT, true><<<grid, 64 * kStepWaves, 0, st>>>(a, s);
+    else
+        step_kernel<HD, Q4, XT, false><<<grid, 64 * kStepWaves, 0, st>>>(a, s);
+    join_kernel<HD, Q4, XT><<<dim3(a.pv.n_seqs * a.pv.max_q, a.hq), s.n > 8 ? 256 : 64, 0, st>>>(a, s);
+}
+
+template <int HD, bool Q4>
+void launch(const AttnArgs& a, int dtype, const Splits& s, hipStream_t st) {
+    if (dtype == CSDR_F32) launch_step<HD, Q4, float>(a, s, st);
+    else launch_step<HD, Q4, _Float16>(a, s, st);
 }
 
 }  // namespace
@@ -132,15 +761,17 @@ extern "C" {
 CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_tokens,
                                                 const int32_t* q_start, int max_q, int Hq,
                                                 int max_len) {
-    (void)kv, (void)n_tokens, (void)q_start, (void)max_q, (void)Hq, (void)max_len;
-    return 0;
+    PagedView pv;
+    if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
+        Hq % kv->n_kv_heads || max_len < 0)
+        return 0;
+    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len));
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
                              const int32_t* q_start, int max_q, int Hq, int64_t q_stride,
                              int max_len, float scale, const csdr_attn_options* options, void* out,
                              void* workspace, size_t workspace_bytes, void* hip_stream) {
-    (void)workspace, (void)workspace_bytes;
     AttnArgs a{};
     if (int rc = csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &a.pv)) return rc;
     if (!q || !out) return set_error(CSDR_E_INVALID, "paged_attn: a pointer is NULL");
@@ -168,16 +799,24 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.q = q;
     a.out = out;
     a.hq = Hq;
-    if ((long long)kv->n_seqs * a.pv.max_q > 0x7fffffffLL)
+    const long long cols = ((long long)a.pv.max_q * (Hq / kv->n_kv_heads) + kCols - 1) / kCols;
+    if ((long long)kv->n_seqs * a.pv.max_q > 0x7fffffffLL || cols > 65535 ||
+        (long long)kv->n_seqs * kv->n_kv_heads > 0x7fffffffLL)
         return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
+    Splits s = splits_of(a.pv, Hq, max_len);
+    if (!workspace || workspace_bytes < workspace_of(a.pv, Hq, hd, s) ||
+        reinterpret_cast<uintptr_t>(workspace) % 16)
+        return set_error(CSDR_E_WORKSPACE, "paged_attn: workspace missing, too small or unaligned");
+    s.stats = static_cast<float*>(workspace);
+    s.vecs = s.stats + csdr::align_up((size_t)n_tokens * Hq * s.n * 2, 4);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const bool q4 = kv->kv_dtype == CSDR_Q4;
     if (hd == 64) {
-        if (q4) launch<64, true>(a, dtype, st);
-        else launch<64, false>(a, dtype, st);
+        if (q4) launch<64, true>(a, dtype, s, st);
+        else launch<64, false>(a, dtype, s, st);
     } else {
-        if (q4) launch<128, true>(a, dtype, st);
-        else launch<128, false>(a, dtype, st);
+        if (q4) launch<128, true>(a, dtype, s, st);
+        else launch<128, false>(a, dtype, s, st);
     }
     CSDR_LAUNCH_CHECK("paged_attn");
     return CSDR_OK;
