@@ -312,6 +312,37 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, 
     return (s - slope * (float)abs(dist)) * kLog2e;
 }
 
+// A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a power
+// of two that puts its largest magnitude in [2^13, 2^14), then in pairs of fp16. Returns the factor
+// from products to scores (in the log2 domain, if there are no options).
+template <int HD, typename XT, bool OPTS>
+__device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int g, h8* qh, h8* ql) {
+    constexpr bool PAIR = sizeof(XT) == 4;
+    float unit = OPTS ? a.scale : a.scale * kLog2e;
+    float x[HD / 32][8], big = 0.0f, f = 1.0f;
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[s][j] = (float)qp[32 * s + 8 * g + j];
+            big = fmaxf(big, fabsf(x[s][j]));
+        }
+    if constexpr (PAIR) {
+        big = lanes16_max(big);
+        const int e = (int)(__float_as_uint(big) >> 23) - 127;
+        const int k = big > 0.0f ? min(max(13 - e, -120), 120) : 0;
+        f = __uint_as_float((uint32_t)(127 + k) << 23);
+        unit *= __uint_as_float((uint32_t)(127 - k) << 23);
+    }
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] *= f;
+        split8<PAIR>(x[s], qh[s], ql[PAIR ? s : 0]);
+    }
+    return unit;
+}
+
 struct Splits {
     int len, n;  // positions per split, splits
     float* stats;  // 2 per (row, head, split): exponent offset and sum
@@ -362,43 +393,18 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
         return tb;
     };
 
-    // q: the B operand, dims 32 s + 8 g .. of column c. fp32: the row scaled by a power of two
-    // that puts its largest magnitude in [2^13, 2^14), then in pairs.
-    h8 qh[NS], ql[PAIR ? NS : 1];
-    float unit = OPTS ? a.scale : a.scale * kLog2e;
-    float qsum[Q4 ? NS : 1];
-    {
-        const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
-        float x[NS][8];
-        float big = 0.0f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[s][j] = (float)qp[32 * s + 8 * g + j];
-                big = fmaxf(big, fabsf(x[s][j]));
-            }
-        float f = 1.0f;
-        if constexpr (PAIR) {
-            big = lanes16_max(big);
-            const int e = (int)(__float_as_uint(big) >> 23) - 127;
-            const int k = big > 0.0f ? min(max(13 - e, -120), 120) : 0;
-            f = __uint_as_float((uint32_t)(127 + k) << 23);
-            unit *= __uint_as_float((uint32_t)(127 - k) << 23);
-        }
+    h8 qh[NS], ql[NS];
+    const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
+    const float unit = load_query<HD, XT, OPTS>(a, qp, g, qh, ql);
+    float qsum[Q4 ? NS : 1];  // sums of the groups of 32 dims
+    if constexpr (Q4)
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            float y[8], t = 0.0f;
+            float t = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                y[j] = x[s][j] * f;
-                t += y[j];
-            }
-            if constexpr (Q4) qsum[s] = lanes16_sum(t);
-            split8<PAIR>(y, qh[s], ql[PAIR ? s : 0]);
+            for (int j = 0; j < 8; ++j) t += PAIR ? (float)qh[s][j] + (float)ql[s][j] : (float)qh[s][j];
+            qsum[s] = lanes16_sum(t);
         }
-    }
-
     __shared__ TileParams<HD> params[Q4 ? kStepWaves : 1];
     TileParams<HD>& tp = params[Q4 ? wave : 0];
 
@@ -717,35 +723,479 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, Splits sp) {
     for (int v = 0; v < VPL; ++v) out[v] = (XT)(num[v] / den);
 }
 
-// Positions per split: about 1024 workgroups in all (4 to a CU), 128 (a tile per wave) at least.
+// ---------------------------------------------------------------- prompts: tiles shared in LDS
+
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// Attention of many columns, the (token, query head) pairs of one sequence and KV head: a workgroup
+// takes 64 NQ of them, a wave NQ tiles of 16 (column tiles are dealt to the waves in turn, so that
+// under a causal mask all four see about as many positions). Tiles of TP positions of K and V lie
+// in LDS twice, the next one being brought in while the current one is worked on; a wave reads each
+// operand once for its NQ column tiles. The products, the running maximum and what a lane holds
+// are step_kernel's, all NQ column tiles beside each other.
+//
+// fp16 pages go straight to LDS (16 bytes a lane); K's 16-byte chunks of a row are permuted within
+// the row on the way (chunk j of row r at j ^ key(r)), so that the 16 rows of an operand read fall
+// on distinct banks; V's pieces lie in operand order already. 4-bit pages are turned into fp16
+// values by the threads, one plane for fp16 calls (values rounded to 11 bits, which is what such a
+// call's inputs have), two for fp32 calls: value = hi + lo to 22 bits, and three products
+// hi hi, hi lo, lo hi.
+template <int HD, bool Q4, typename XT, int NQ>
+struct PromptShape {
+    static constexpr bool kPair = sizeof(XT) == 4;
+    static constexpr int kPlanes = Q4 && kPair ? 2 : 1;
+    static constexpr int TP = kPlanes == 2 && HD == 128 ? 32 : 64;  // positions per tile
+    static constexpr int kPlane = TP * HD;                          // halves
+    static constexpr int kLds = 2 * 2 * kPlanes * kPlane * 2;       // bytes
+    static constexpr int kColumns = 4 * 16 * NQ;
+};
+
+// Where the LDS row of position r of a tile keeps chunk j.
+template <int HD>
+__device__ __forceinline__ int chunk_key(int r) {
+    return HD == 128 ? 4 * ((r >> 3) & 3) + (r & 3) : 2 * ((r >> 3) & 3) + ((r >> 1) & 1);
+}
+
+template <int HD, bool Q4, typename XT, bool OPTS, int NQ>
+__global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
+    using Shape = PromptShape<HD, Q4, XT, NQ>;
+    constexpr bool PAIR = Shape::kPair;
+    constexpr int NS = HD / 32, ND = HD / 16, TP = Shape::TP, PLANES = Shape::kPlanes;
+    constexpr int PLANE = Shape::kPlane, GR = TP / 16;
+    extern __shared__ __attribute__((aligned(16))) _Float16 lds[];  // [2][K, V][planes][TP * HD]
+    const PagedView& pv = a.pv;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int G = a.hq / pv.hkv;
+    // (sequence, KV head) fastest: on a chip of 8 dies that take workgroups in turn, the blocks of
+    // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns first.
+    const int pairs = pv.n_seqs * pv.hkv;
+    const int bh = blockIdx.x % pairs, block = (int)(gridDim.x / pairs) - 1 - blockIdx.x / pairs;
+    const int b = bh / pv.hkv, kvh = bh % pv.hkv, split = blockIdx.y;
+    const SeqRows r = csdr::seq_rows(pv, b);
+    const int ncols = r.n * G, col0 = block * Shape::kColumns;
+    if (col0 >= ncols) return;
+    const Seen seen = seen_of(a, b, r);
+    const int ps = pv.page_size();
+    auto pos_of = [&](int col) { return r.p0 + col / G; };
+    const int last_col = min(ncols, col0 + Shape::kColumns) - 1;
+    const int pq0 = pos_of(col0), pq1 = pos_of(last_col);  // of the workgroup
+
+    // positions that some column sees: below `first` only the prefix
+    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);
+    const int end = pq1 < 0 ? 0 : min(seen.keys, max(pq1 + 1, seen.prefix));
+    const int lo = split * sp.len, hi = split == sp.n - 1 ? end : min(end, lo + sp.len);
+    auto next_tile = [&](int tb) {
+        tb += TP;
+        if (tb < hi && tb >= seen.prefix && tb + TP <= first) tb += (first - TP - tb) / TP * TP + TP;
+        return tb;
+    };
+
+    // the columns of this lane: tile q holds columns col0 + 16 (4 q + wave) + c
+    h8 qh[NQ][NS], ql[PAIR ? NQ : 1][NS];
+    float unit[NQ], slope[NQ];
+    int pq[NQ];
+    int wp0 = 0x7fffffff, wp1 = -0x7fffffff;  // first and last position of the wave's columns
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int t0 = col0 + 16 * (4 * q + wave);
+        const int col = min(t0 + c, ncols - 1);
+        if (t0 < ncols) {
+            wp0 = min(wp0, pos_of(t0));
+            wp1 = max(wp1, pos_of(min(t0 + 15, ncols - 1)));
+        }
+        const int h = kvh * G + col % G;
+        pq[q] = pos_of(col);
+        slope[q] = OPTS && a.slopes ? a.slopes[h] : 0.0f;
+        const XT* qp = static_cast<const XT*>(a.q) + ((long long)r.first + col / G) * a.q_stride +
+                       (long long)h * HD;
+        unit[q] = load_query<HD, XT, OPTS>(a, qp, g, qh[q], ql[PAIR ? q : 0]);
+    }
+
+    f4 o[NQ][ND];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        m[q] = kNoMax;
+        l[q] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[q][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto buffer = [&](int buf, int v, int plane) {
+        return lds + ((buf * 2 + v) * PLANES + plane) * PLANE;
+    };
+    // page ids of a tile's granules of 16 positions (uniform)
+    auto pages_at = [&](int tb, int* pg) {
+#pragma unroll
+        for (int i = 0; i < GR; ++i)
+            pg[i] = i > 0 && ps >= TP ? pg[0] : csdr::page_of(pv, b, tb + 16 * i);
+    };
+
+    // 4 bits: the words this thread turns into values, and their groups' scales and minima
+    constexpr int W = TP * HD / 8 / 256;  // words per thread: 2 or 4
+    struct Codes {
+        uint32_t k[W], v[W];
+        _Float16 ks[W], km[W];
+        h8 vs[W / 2], vm[W / 2];
+    };
+    Codes cd;
+
+    // brings the tile at tb into buffer `buf` (fp16 pages) or its codes into registers
+    auto fetch = [&](int tb, int buf, const int* pg) {
+        if constexpr (!Q4) {
+            constexpr int N = PLANE * 2 / 1024 / 4;  // 1 KB pieces per wave, for K and for V
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int piece = 4 * i + wave;
+                const int row = piece * (512 / HD);  // K: 4 or 8 rows a piece
+                const int page = max(pg[row / 16], 0);
+                const size_t head = csdr::head_offset<Q4>(pv, HD, page, kvh);
+                const int slot = (tb + row) & (ps - 1);
+                const int in = lane / (HD / 8), ch = lane % (HD / 8);
+                const uint8_t* src = pv.k + head + (slot + in) * (HD * 2) +
+                                     (ch ^ chunk_key<HD>(row + in)) * 16;
+                __builtin_amdgcn_global_load_lds((GlobalPtr)src,
+                                                 (LdsPtr)(buffer(buf, 0, 0) + piece * 512), 16, 0, 0);
+                // V: [8 positions][dim][8], a piece is half a block of 8 positions or a whole one
+                const int vrow = piece * 512 / (8 * HD) * 8;
+                const int vpage = max(pg[vrow / 16], 0);
+                const int vslot = (tb + vrow) & (ps - 1);
+                const uint8_t* vsrc = pv.v + csdr::head_offset<Q4>(pv, HD, vpage, kvh) +
+                                      vslot * (HD * 2) + piece * 1024 % (HD * 16) + lane * 16;
+                __builtin_amdgcn_global_load_lds((GlobalPtr)vsrc,
+                                                 (LdsPtr)(buffer(buf, 1, 0) + piece * 512), 16, 0, 0);
+            }
+        } else {
+            // K: words [slot][dim % 32 / 8][dim / 32]; V: words [slot / 8][dim % 16][dim / 16]
+            const int w0 = tid * W;
+            const int kr = w0 / (HD / 8), vr = w0 / HD * 8;
+            const int kp = max(pg[0], 0), vp = kp;
+            int kpage = kp, vpage = vp;
+#pragma unroll
+            for (int i = 1; i < GR; ++i) {
+                kpage = kr / 16 == i ? max(pg[i], 0) : kpage;
+                vpage = vr / 16 == i ? max(pg[i], 0) : vpage;
+            }
+            const uint8_t* kb = pv.k + csdr::head_offset<Q4>(pv, HD, kpage, kvh);
+            const uint8_t* vb = pv.v + csdr::head_offset<Q4>(pv, HD, vpage, kvh);
+            const int ks = (tb + kr) & (ps - 1), vs = (tb + vr) & (ps - 1);
+            __builtin_memcpy(cd.k, __builtin_assume_aligned(
+                                       kb + 4 * (ks * (HD / 8) + w0 % (HD / 8)), 4 * W), 4 * W);
+            __builtin_memcpy(cd.v, __builtin_assume_aligned(
+                                       vb + 4 * ((vs >> 3) * HD + w0 % HD), 4 * W), 4 * W);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int grp = (w0 + i) % NS;
+                cd.ks[i] = *reinterpret_cast<const _Float16*>(kb + csdr::scale_offset(HD, ps, grp, ks));
+                cd.km[i] = *reinterpret_cast<const _Float16*>(kb + csdr::min_offset(HD, ps, grp, ks));
+            }
+#pragma unroll
+            for (int i = 0; i < W / 2; ++i) {
+                const int grp = (w0 % ND) / 2 + i;
+                cd.vs[i] = *reinterpret_cast<const h8*>(vb + csdr::scale_offset(HD, ps, grp, vs));
+                cd.vm[i] = *reinterpret_cast<const h8*>(vb + csdr::min_offset(HD, ps, grp, vs));
+            }
+        }
+    };
+    // 4 bits: this thread's words as values into buffer `buf`
+    auto unpack = [&](int buf) {
+        const int w0 = tid * W;
+        const int kr = w0 / (HD / 8);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int kw = w0 % (HD / 8) + i, ch = kw % NS * 4 + kw / NS;  // dims 8 ch ..
+            h8 hi8, lo8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = fmaf((float)cd.ks[i],
+                                     (float)((cd.k[i] >> csdr::code_shift(e)) & 15u), (float)cd.km[i]);
+                hi8[e] = (_Float16)x;
+                if constexpr (PLANES == 2) lo8[e] = (_Float16)(x - (float)hi8[e]);
+            }
+            const int at = kr * HD + (ch ^ chunk_key<HD>(kr)) * 8;
+            *reinterpret_cast<h8*>(buffer(buf, 0, 0) + at) = hi8;
+            if constexpr (PLANES == 2) *reinterpret_cast<h8*>(buffer(buf, 0, PLANES - 1) + at) = lo8;
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int vw = w0 % HD + i, d = vw % ND * 16 + vw / ND;
+            h8 hi8, lo8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float x = fmaf((float)cd.vs[i / 2][e],
+                                     (float)((cd.v[i] >> csdr::code_shift(e)) & 15u),
+                                     (float)cd.vm[i / 2][e]);
+                hi8[e] = (_Float16)x;
+                if constexpr (PLANES == 2) lo8[e] = (_Float16)(x - (float)hi8[e]);
+            }
+            const int at = (w0 / HD * HD + d) * 8;
+            *reinterpret_cast<h8*>(buffer(buf, 1, 0) + at) = hi8;
+            if constexpr (PLANES == 2) *reinterpret_cast<h8*>(buffer(buf, 1, PLANES - 1) + at) = lo8;
+        }
+    };
+    // zeros for V at positions of the tile that hold nothing (their weights are zero)
+    auto clear = [&](int tb, int buf, const int* pg) {
+        for (int i = tid; i < TP * HD; i += 256) {
+            const int pos = i / (8 * HD) * 8 + i % 8;
+            int page = pg[0];
+#pragma unroll
+            for (int k = 1; k < GR; ++k) page = pos / 16 == k ? pg[k] : page;
+            if (page >= 0 && tb + pos < seen.keys) continue;
+#pragma unroll
+            for (int k = 0; k < PLANES; ++k) buffer(buf, 1, k)[i] = (_Float16)0.0f;
+        }
+    };
+
+    int tb = next_tile(lo - TP), buf = 0;
+    int pg[GR] = {};
+    if (tb < hi) {
+        pages_at(tb, pg);
+        fetch(tb, 0, pg);
+        if constexpr (Q4) unpack(0);
+    }
+    while (tb < hi) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's pieces are in LDS)
+        __syncthreads();  // the tile is whole, and everyone is done with the other buffer
+        bool held = tb + TP <= seen.keys;
+        uint32_t have = 0u;  // granules with a page
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            held = held && pg[i] >= 0;
+            have |= (uint32_t)(pg[i] >= 0) << i;
+        }
+        if (!held) {
+            clear(tb, buf, pg);
+            __syncthreads();
+        }
+        const int nb = next_tile(tb);
+        if (Q4 || nb < hi) {  // (4 bits: the last tile again, so that the registers are always set)
+            pages_at(min(nb, hi - 1) / TP * TP, pg);
+            fetch(min(nb, hi - 1) / TP * TP, buf ^ 1, pg);
+        }
+        const bool any = wp0 <= wp1 && ((tb <= wp1 && tb + TP > first) || tb < seen.prefix);
+        const bool whole = held && wp0 >= 0 &&
+                           (tb + TP <= seen.prefix ||
+                            (tb + TP - 1 <= wp0 && tb >= 0 && wp1 - tb < seen.window));
+        if (any) {
+#pragma unroll
+            for (int hb = 0; hb < TP / 32; ++hb) {
+                const _Float16* kt = buffer(buf, 0, 0) + (32 * hb + 8 * (c >> 2) + (c & 3)) * HD;
+                const _Float16* vt = buffer(buf, 1, 0) + (4 * hb + g) * (8 * HD) + c * 8;
+                const int key = chunk_key<HD>(8 * (c >> 2) + (c & 3));
+                f4 acc[NQ][2];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) acc[q][0] = acc[q][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const _Float16* kp = kt + 4 * u * HD + ((4 * s + g) ^ key) * 8;
+                        const h8 k0 = *reinterpret_cast<const h8*>(kp);
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) {
+                            acc[q][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[q][s],
+                                                                               acc[q][u], 0, 0, 0);
+                            if constexpr (PAIR)
+                                acc[q][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    k0, ql[q][s], acc[q][u], 0, 0, 0);
+                        }
+                        if constexpr (PLANES == 2) {
+                            const h8 k1 = *reinterpret_cast<const h8*>(kp + PLANE);
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q)
+                                acc[q][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    k1, qh[q][s], acc[q][u], 0, 0, 0);
+                        }
+                    }
+                float x[NQ][8];
+                bool move = false;
+                float top[NQ];
+                const int p8 = tb + 32 * hb + 8 * g;
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        x[q][j] = score2<OPTS>(a, acc[q][j >> 2][j & 3], unit[q], slope[q],
+                                               pq[q] - (p8 + j));
+                    if (!whole) {
+                        const bool page = have >> ((32 * hb + 8 * g) / 16) & 1;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (!(page && pq[q] >= 0 && seen.at(pq[q], p8 + j)))
+                                x[q][j] = -INFINITY;
+                    }
+                    top[q] = kNoMax;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top[q] = fmaxf(top[q], x[q][j]);
+                    move = move || top[q] > m[q] + kLag;
+                }
+                if (__any(move)) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        const float mn = fmaxf(m[q], lanes16_max(top[q]));
+                        const float f = exp2_fast(m[q] - mn);
+                        l[q] *= f;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) o[q][d] *= f;
+                        m[q] = mn;
+                    }
+                }
+                h8 wh[NQ], wl[PAIR ? NQ : 1];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    float w8[8], sum = 0.0f;
+                    const float off = kBias - m[q];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        w8[j] = exp2_fast(x[q][j] + off);
+                        sum += w8[j];
+                    }
+                    l[q] += sum;
+                    split8<PAIR>(w8, wh[q], wl[PAIR ? q : 0]);
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const h8 v0 = *reinterpret_cast<const h8*>(vt + d * 128);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        o[q][d] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wh[q], o[q][d], 0, 0, 0);
+                        if constexpr (PAIR)
+                            o[q][d] =
+                                __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wl[q], o[q][d], 0, 0, 0);
+                    }
+                    if constexpr (PLANES == 2) {
+                        const h8 v1 = *reinterpret_cast<const h8*>(vt + d * 128 + PLANE);
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+                            o[q][d] =
+                                __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wh[q], o[q][d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if constexpr (Q4) unpack(buf ^ 1);
+        tb = nb;
+        buf ^= 1;
+    }
+
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int t0 = col0 + 16 * (4 * q + wave), col = t0 + c;
+        l[q] = lanes16_sum(l[q]);
+        const long long row = (long long)r.first + col / G;
+        const int h = kvh * G + col % G;
+        if (sp.n > 1) {
+            if (col < ncols) {
+                const size_t part = ((size_t)row * a.hq + h) * sp.n + split;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    *reinterpret_cast<f4*>(sp.vecs + part * HD + 16 * d + 4 * g) = o[q][d];
+                if (g == 0) {
+                    sp.stats[2 * part] = m[q];
+                    sp.stats[2 * part + 1] = l[q];
+                }
+            }
+            continue;
+        }
+        bool fine = l[q] > 0.0f && l[q] < INFINITY;
+        const float inv = 1.0f / l[q];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            o[q][d] *= inv;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fine = fine && fabsf(o[q][d][i]) < INFINITY;
+        }
+        XT* out = static_cast<XT*>(a.out) + (row * a.hq + h) * HD + 4 * g;
+        if (col < ncols)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[16 * d + i] = (XT)o[q][d][i];
+        // rows that see nothing, or something that is not finite (perhaps unseen): once more
+        uint64_t redo = __ballot(!fine && col < ncols);
+        redo |= redo >> 32;
+        redo = (redo | redo >> 16) & 0xFFFFu;
+        while (redo) {
+            const int k = __builtin_ctzll(redo);
+            redo &= redo - 1;
+            const int col1 = t0 + k;
+            attend_row<HD, Q4, XT>(a, b, r, col1 / G, kvh * G + col1 % G);
+        }
+    }
+}
+
+// Up to this many columns of a KV head go to step_kernel (16 at a time), more to prompt_kernel.
+constexpr int kStepColumns = 64;
+constexpr int kPromptColumns = 128;  // of the smallest workgroup of prompt_kernel
+
+// Positions per split. step_kernel: about 1024 workgroups in all (4 to a CU), 128 positions (a tile
+// per wave) at least. prompt_kernel: one split if there are 512 workgroups (two to a CU), else
+// enough for that, 512 positions at least.
 Splits splits_of(const PagedView& pv, int hq, int max_len) {
     Splits s{};
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
-    const long long cols = ((long long)pv.max_q * (hq / pv.hkv) + kCols - 1) / kCols;
-    const long long wgs = (long long)pv.n_seqs * pv.hkv * cols;
-    const long long unit = kTile * kStepWaves;
-    long long each = (len * wgs + 1023) / 1024;
+    const long long cols = (long long)pv.max_q * (hq / pv.hkv);
+    const bool step = cols <= kStepColumns;
+    const long long per = step ? kCols : kPromptColumns, unit = step ? kTile * kStepWaves : 512;
+    const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
+    const long long target = step ? 1024 : 512;
+    long long each = step || wgs < target ? (len * wgs + target - 1) / target : len;
     each = std::max(unit, (each + unit - 1) / unit * unit);
     s.len = (int)std::min(each, (long long)csdr::kMaxPositions);
     s.n = (int)((len + s.len - 1) / s.len);
     return s;
 }
 
+// A call of prompt_kernel without splits needs none.
+bool one_launch(const PagedView& pv, int hq, const Splits& s) {
+    return (long long)pv.max_q * (hq / pv.hkv) > kStepColumns && s.n == 1;
+}
+
 size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
+    if (one_launch(pv, hq, s)) return 0;
     const size_t parts = (size_t)pv.n_tokens * hq * s.n;
     return csdr::align_up(parts * 8, 16) + parts * hd * 4;
 }
 
+// Column tiles per wave of prompt_kernel: as many as 256 registers hold (sums, queries, weights).
+template <int HD, bool Q4, typename XT>
+constexpr int prompt_tiles() {
+    return HD == 128 ? (sizeof(XT) == 4 || Q4 ? 2 : 3) : (sizeof(XT) == 4 || Q4 ? 3 : 4);
+}
+
+template <int HD, bool Q4, typename XT, bool OPTS>
+void launch_kernel(const AttnArgs& a, const Splits& s, hipStream_t st) {
+    const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
+    if (cols > kStepColumns) {
+        constexpr int NQ = prompt_tiles<HD, Q4, XT>();
+        using Shape = PromptShape<HD, Q4, XT, NQ>;
+        static const bool raised = [] {
+            (void)hipFuncSetAttribute(
+                reinterpret_cast<const void*>(&prompt_kernel<HD, Q4, XT, OPTS, NQ>),
+                hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
+            return true;
+        }();
+        (void)raised;
+        const int blocks = (cols + Shape::kColumns - 1) / Shape::kColumns;
+        prompt_kernel<HD, Q4, XT, OPTS, NQ>
+            <<<dim3((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n), 256, Shape::kLds, st>>>(a, s);
+        if (s.n == 1) return;
+    } else {
+        const dim3 grid(a.pv.n_seqs * a.pv.hkv, s.n, (cols + kCols - 1) / kCols);
+        step_kernel<HD, Q4, XT, OPTS><<<grid, 64 * kStepWaves, 0, st>>>(a, s);
+    }
+    join_kernel<HD, Q4, XT>
+        <<<dim3(a.pv.n_seqs * a.pv.max_q, a.hq), s.n > 8 ? 256 : 64, 0, st>>>(a, s);
+}
+
 template <int HD, bool Q4, typename XT>
 void launch_step(const AttnArgs& a, const Splits& s, hipStream_t st) {
-    const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
-    const dim3 grid(a.pv.n_seqs * a.pv.hkv, s.n, (cols + kCols - 1) / kCols);
-    if (a.cap > 0.0f || a.slopes)
-        step_kernel<HD, Q4, XT, true><<<grid, 64 * kStepWaves, 0, st>>>(a, s);
-    else
-        step_kernel<HD, Q4, XT, false><<<grid, 64 * kStepWaves, 0, st>>>(a, s);
-    join_kernel<HD, Q4, XT><<<dim3(a.pv.n_seqs * a.pv.max_q, a.hq), s.n > 8 ? 256 : 64, 0, st>>>(a, s);
+    if (a.cap > 0.0f || a.slopes) launch_kernel<HD, Q4, XT, true>(a, s, st);
+    else launch_kernel<HD, Q4, XT, false>(a, s, st);
 }
 
 template <int HD, bool Q4>
@@ -800,12 +1250,13 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.out = out;
     a.hq = Hq;
     const long long cols = ((long long)a.pv.max_q * (Hq / kv->n_kv_heads) + kCols - 1) / kCols;
-    if ((long long)kv->n_seqs * a.pv.max_q > 0x7fffffffLL || cols > 65535 ||
-        (long long)kv->n_seqs * kv->n_kv_heads > 0x7fffffffLL)
+    if ((long long)kv->n_seqs * std::max((long long)a.pv.max_q, kv->n_kv_heads * cols) >
+        0x7fffffffLL)
         return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
     Splits s = splits_of(a.pv, Hq, max_len);
-    if (!workspace || workspace_bytes < workspace_of(a.pv, Hq, hd, s) ||
-        reinterpret_cast<uintptr_t>(workspace) % 16)
+    const size_t need = workspace_of(a.pv, Hq, hd, s);
+    if (need && (!workspace || workspace_bytes < need ||
+                 reinterpret_cast<uintptr_t>(workspace) % 16))
         return set_error(CSDR_E_WORKSPACE, "paged_attn: workspace missing, too small or unaligned");
     s.stats = static_cast<float*>(workspace);
     s.vecs = s.stats + csdr::align_up((size_t)n_tokens * Hq * s.n * 2, 4);

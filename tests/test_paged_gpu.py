@@ -93,6 +93,7 @@ class Setup:
 
 
 HEADS = {"qwen": (14, 2, 64), "llama": (4, 4, 128), "gqa": (8, 2, 128), "many": (20, 1, 64),
+         "one": (2, 2, 64),
          "three": (6, 2, 64)}
 
 
@@ -286,6 +287,11 @@ def test_attend_step_options(gpu, kv, x, o):
     ("many", [31], [2], 16),
     ("three", [5, 0, 64], [1, 40, 0], 16),
     ("gqa", [30, 1, 0], [2, 1, 2], 16),
+    ("llama", [0, 333], [150, 70], 16),
+    ("llama", [2000], [66], 64),           # few columns, many positions: split
+    ("three", [1500, 0], [30, 25], 128),
+    ("many", [700], [9], 32),
+    ("one", [90, 0], [70, 200], 32),
 ])
 def test_attend_tokens(gpu, kv, x, heads, old, new, ps):
     s = Setup(gpu, [a + b for a, b in zip(old, new)], HEADS[heads], kv, x, ps=ps, seed=8,
@@ -308,6 +314,19 @@ def test_attend_tokens_options(gpu, kv, x, o):
     a, e = options(s, o)
     got = s.batch.attend(qd, q_start=s.starts(new), max_q=70, **a).cpu().numpy()
     assert rel_l2(got, s.expect(qd.cpu().numpy(), new, **e)) <= tol(x, kv, 2)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("o", OPTIONS)
+def test_attend_tokens_options_long(gpu, kv, x, o):
+    """The same where positions are split and most lie left of the window."""
+    s = Setup(gpu, [1700], HEADS["gqa"], kv, x, ps=32, seed=21)
+    s.append([1660], with_q=False)
+    qd, _ = s.append([40])
+    a, e = options(s, o)
+    got = s.batch.attend(qd, max_len=1700, **a).cpu().numpy()
+    assert rel_l2(got, s.expect(qd.cpu().numpy(), [40], **e)) <= tol(x, kv, 2)
 
 
 def test_attend_uniform_tokens_and_stride(gpu):
