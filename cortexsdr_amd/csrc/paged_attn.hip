@@ -44,7 +44,8 @@ __device__ __forceinline__ float wave_max(float v) {
 struct Seen {
     int keys, window, prefix;
     __device__ bool at(int pq, int p) const {
-        return p < keys && (p < prefix || (p <= pq && pq - p < window));
+        // (no short cuts: they compile to branches)
+        return (p < keys) & ((p < prefix) | ((p <= pq) & (pq - p < window)));
     }
 };
 
@@ -124,11 +125,15 @@ constexpr int kTile = 32;       // positions per step of a wave
 constexpr int kCols = 16;       // (token, query head) pairs per wave
 constexpr int kStepWaves = 4;
 constexpr float kLog2e = 1.44269504088896341f;
-// Weights are 2^(s - m + kBias) in the log2 domain, m a maximum that may lag kLag behind: at most
-// 2^15, near the top of fp16: a pair keeps its 22 bits down to 2^-17 of the largest weight (the
-// step of its low half is 2^-24). m moves, and the sums with it, only now and then. (With weights
-// of 2^8 as a rule, rows with a high maximum were 2e-5 to 1.6e-4 off.)
-constexpr float kLag = 1.0f, kBias = 14.0f;
+// Weights are 2^(s - m + bias) in the log2 domain, m a maximum that may lag `lag` behind, so that m
+// moves, and the sums with it, only now and then: at most 2^15, near the top of fp16. fp32 calls: a
+// pair keeps its 22 bits down to 2^(bias - 30) of the largest weight (the step of its low half is
+// 2^-24); with a bias of 8, rows with a high maximum were 2e-5 to 1.6e-4 off. fp16 calls: one
+// rounding to 11 bits down to 2^-21 of it, which leaves more room to lag.
+template <typename XT>
+constexpr float kLag = sizeof(XT) == 4 ? 2.0f : 8.0f;
+template <typename XT>
+constexpr float kBias = 15.0f - kLag<XT>;
 constexpr float kNoMax = -1e30f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -313,12 +318,13 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, 
 }
 
 // A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a power
-// of two that puts its largest magnitude in [2^13, 2^14), then in pairs of fp16. Returns the factor
-// from products to scores (in the log2 domain, if there are no options).
+// of two that puts its largest magnitude in [2^13, 2^14), then in pairs of fp16. A negative scale
+// turns the query round. Returns the (positive) factor from products to scores, in the log2 domain
+// if there are no options.
 template <int HD, typename XT, bool OPTS>
 __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int g, h8* qh, h8* ql) {
     constexpr bool PAIR = sizeof(XT) == 4;
-    float unit = OPTS ? a.scale : a.scale * kLog2e;
+    float unit = fabsf(OPTS ? a.scale : a.scale * kLog2e);
     float x[HD / 32][8], big = 0.0f, f = 1.0f;
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s)
@@ -334,6 +340,7 @@ __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int
         f = __uint_as_float((uint32_t)(127 + k) << 23);
         unit *= __uint_as_float((uint32_t)(127 - k) << 23);
     }
+    f = copysignf(f, a.scale);
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s) {
 #pragma unroll
@@ -435,7 +442,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
         if (!whole) {
             live = mine = 0u;
             auto some = [&](int p) {
-                return p < seen.keys && (p < seen.prefix || (p >= first && p <= pq1));
+                return (p < seen.keys) & ((p < seen.prefix) | ((p >= first) & (p <= pq1)));
             };
             if (Q4 && (at.parhigh ? pg1 : pg0) >= 0)
 #pragma unroll
@@ -445,7 +452,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int p = p8 + j;
-                    mine |= (uint32_t)(pq >= 0 && seen.at(pq, p)) << j;
+                    mine |= (uint32_t)((pq >= 0) & seen.at(pq, p)) << j;
                     live |= (uint32_t)some(p) << j;
                 }
             }
@@ -514,7 +521,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) top = fmaxf(top, s8[j]);
-        bool move = top > m + kLag;
+        bool move = top > m + kLag<XT>;
         if constexpr (Q4) {
             move = move || vscale > vtop;
         }
@@ -536,7 +543,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
             m = mn;
             ev = en;
         }
-        const float off = kBias - ev - m;
+        const float off = kBias<XT> - ev - m;
         float w8[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -729,8 +736,8 @@ typedef const __attribute__((address_space(1))) void* GlobalPtr;
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
 // Attention of many columns, the (token, query head) pairs of one sequence and KV head: a workgroup
-// takes 64 NQ of them, a wave NQ tiles of 16 (column tiles are dealt to the waves in turn, so that
-// under a causal mask all four see about as many positions). Tiles of TP positions of K and V lie
+// of NW waves takes 16 NQ NW of them, a wave NQ tiles of 16 (column tiles are dealt to the waves in
+// turn, so that under a causal mask all see about as many positions). Tiles of TP positions of K and V lie
 // in LDS twice, the next one being brought in while the current one is worked on; a wave reads each
 // operand once for its NQ column tiles. The products, the running maximum and what a lane holds
 // are step_kernel's, all NQ column tiles beside each other.
@@ -741,14 +748,15 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // values by the threads, one plane for fp16 calls (values rounded to 11 bits, which is what such a
 // call's inputs have), two for fp32 calls: value = hi + lo to 22 bits, and three products
 // hi hi, hi lo, lo hi.
-template <int HD, bool Q4, typename XT, int NQ>
+template <int HD, bool Q4, typename XT, int NQ, int NW>
 struct PromptShape {
     static constexpr bool kPair = sizeof(XT) == 4;
     static constexpr int kPlanes = Q4 && kPair ? 2 : 1;
-    static constexpr int TP = kPlanes == 2 && HD == 128 ? 32 : 64;  // positions per tile
+    // positions per tile: LDS for two workgroups of four waves or one of eight on a CU
+    static constexpr int TP = kPlanes == 2 && HD == 128 && NW == 4 ? 32 : 64;
     static constexpr int kPlane = TP * HD;                          // halves
     static constexpr int kLds = 2 * 2 * kPlanes * kPlane * 2;       // bytes
-    static constexpr int kColumns = 4 * 16 * NQ;
+    static constexpr int kColumns = NW * 16 * NQ;
 };
 
 // Where the LDS row of position r of a tile keeps chunk j.
@@ -757,9 +765,9 @@ __device__ __forceinline__ int chunk_key(int r) {
     return HD == 128 ? 4 * ((r >> 3) & 3) + (r & 3) : 2 * ((r >> 3) & 3) + ((r >> 1) & 1);
 }
 
-template <int HD, bool Q4, typename XT, bool OPTS, int NQ>
-__global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
-    using Shape = PromptShape<HD, Q4, XT, NQ>;
+template <int HD, bool Q4, typename XT, bool OPTS, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Splits sp) {
+    using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
     constexpr bool PAIR = Shape::kPair;
     constexpr int NS = HD / 32, ND = HD / 16, TP = Shape::TP, PLANES = Shape::kPlanes;
     constexpr int PLANE = Shape::kPlane, GR = TP / 16;
@@ -792,14 +800,14 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
         return tb;
     };
 
-    // the columns of this lane: tile q holds columns col0 + 16 (4 q + wave) + c
+    // the columns of this lane: tile q holds columns col0 + 16 (NW q + wave) + c
     h8 qh[NQ][NS], ql[PAIR ? NQ : 1][NS];
     float unit[NQ], slope[NQ];
     int pq[NQ];
     int wp0 = 0x7fffffff, wp1 = -0x7fffffff;  // first and last position of the wave's columns
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-        const int t0 = col0 + 16 * (4 * q + wave);
+        const int t0 = col0 + 16 * (NW * q + wave);
         const int col = min(t0 + c, ncols - 1);
         if (t0 < ncols) {
             wp0 = min(wp0, pos_of(t0));
@@ -813,12 +821,13 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
         unit[q] = load_query<HD, XT, OPTS>(a, qp, g, qh[q], ql[PAIR ? q : 0]);
     }
 
-    f4 o[NQ][ND];
-    float m[NQ], l[NQ];
+    f4 o[NQ][ND], l[NQ];  // l: the sum of the weights, in all four rows (a product with ones)
+    float m[NQ];
+    const h8 ones = h8{} + (_Float16)1.0f;
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         m[q] = kNoMax;
-        l[q] = 0.0f;
+        l[q] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[q][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -834,7 +843,7 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
     };
 
     // 4 bits: the words this thread turns into values, and their groups' scales and minima
-    constexpr int W = TP * HD / 8 / 256;  // words per thread: 2 or 4
+    constexpr int W = TP * HD / 8 / (64 * NW);  // words per thread: 2 or 4
     struct Codes {
         uint32_t k[W], v[W];
         _Float16 ks[W], km[W];
@@ -845,34 +854,29 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
     // brings the tile at tb into buffer `buf` (fp16 pages) or its codes into registers
     auto fetch = [&](int tb, int buf, const int* pg) {
         if constexpr (!Q4) {
-            constexpr int N = PLANE * 2 / 1024 / 4;  // 1 KB pieces per wave, for K and for V
+            constexpr int N = PLANE * 2 / 1024 / NW;  // 1 KB pieces per wave, for K and for V
+            constexpr int R = 512 / HD;               // K: rows a piece
+            // the lane's chunk of a piece of K (a key depends on the piece only by R = 4)
+            const int in = lane / (HD / 8), ch = lane % (HD / 8);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int piece = 4 * i + wave;
-                const int row = piece * (512 / HD);  // K: 4 or 8 rows a piece
+                const int piece = NW * i + wave, row = piece * R;
                 const int page = max(pg[row / 16], 0);
                 const size_t head = csdr::head_offset<Q4>(pv, HD, page, kvh);
                 const int slot = (tb + row) & (ps - 1);
-                const int in = lane / (HD / 8), ch = lane % (HD / 8);
-                const uint8_t* src = pv.k + head + (slot + in) * (HD * 2) +
-                                     (ch ^ chunk_key<HD>(row + in)) * 16;
-                __builtin_amdgcn_global_load_lds((GlobalPtr)src,
-                                                 (LdsPtr)(buffer(buf, 0, 0) + piece * 512), 16, 0, 0);
-                // V: [8 positions][dim][8], a piece is half a block of 8 positions or a whole one
-                const int vrow = piece * 512 / (8 * HD) * 8;
-                const int vpage = max(pg[vrow / 16], 0);
-                const int vslot = (tb + vrow) & (ps - 1);
-                const uint8_t* vsrc = pv.v + csdr::head_offset<Q4>(pv, HD, vpage, kvh) +
-                                      vslot * (HD * 2) + piece * 1024 % (HD * 16) + lane * 16;
-                __builtin_amdgcn_global_load_lds((GlobalPtr)vsrc,
+                __builtin_amdgcn_global_load_lds(
+                    (GlobalPtr)(pv.k + head + slot * (HD * 2) +
+                                (in * (HD * 2) + (ch ^ chunk_key<HD>(row + in)) * 16)),
+                    (LdsPtr)(buffer(buf, 0, 0) + piece * 512), 16, 0, 0);
+                // V: [8 positions][dim][8]: the same piece of memory, R of 8 rows of a block
+                __builtin_amdgcn_global_load_lds((GlobalPtr)(pv.v + head + slot * (HD * 2) + lane * 16),
                                                  (LdsPtr)(buffer(buf, 1, 0) + piece * 512), 16, 0, 0);
             }
         } else {
             // K: words [slot][dim % 32 / 8][dim / 32]; V: words [slot / 8][dim % 16][dim / 16]
             const int w0 = tid * W;
             const int kr = w0 / (HD / 8), vr = w0 / HD * 8;
-            const int kp = max(pg[0], 0), vp = kp;
-            int kpage = kp, vpage = vp;
+            int kpage = max(pg[0], 0), vpage = kpage;
 #pragma unroll
             for (int i = 1; i < GR; ++i) {
                 kpage = kr / 16 == i ? max(pg[i], 0) : kpage;
@@ -900,44 +904,35 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
         }
     };
     // 4 bits: this thread's words as values into buffer `buf`
+    uint32_t magic = 0x4C004C00u;
+    asm("" : "+v"(magic));
+    auto put = [&](_Float16* at, uint32_t w, auto scale, auto low) {
+        const h8 code = codes16(w, magic) - (_Float16)16.0f;
+        h8 hi8, lo8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = fmaf((float)scale(e), (float)code[e], (float)low(e));
+            hi8[e] = (_Float16)x;
+            if constexpr (PLANES == 2) lo8[e] = (_Float16)(x - (float)hi8[e]);
+        }
+        *reinterpret_cast<h8*>(at) = hi8;
+        if constexpr (PLANES == 2) *reinterpret_cast<h8*>(at + PLANE) = lo8;
+    };
     auto unpack = [&](int buf) {
-        const int w0 = tid * W;
-        const int kr = w0 / (HD / 8);
+        const int w0 = tid * W, kr = w0 / (HD / 8);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             const int kw = w0 % (HD / 8) + i, ch = kw % NS * 4 + kw / NS;  // dims 8 ch ..
-            h8 hi8, lo8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = fmaf((float)cd.ks[i],
-                                     (float)((cd.k[i] >> csdr::code_shift(e)) & 15u), (float)cd.km[i]);
-                hi8[e] = (_Float16)x;
-                if constexpr (PLANES == 2) lo8[e] = (_Float16)(x - (float)hi8[e]);
-            }
-            const int at = kr * HD + (ch ^ chunk_key<HD>(kr)) * 8;
-            *reinterpret_cast<h8*>(buffer(buf, 0, 0) + at) = hi8;
-            if constexpr (PLANES == 2) *reinterpret_cast<h8*>(buffer(buf, 0, PLANES - 1) + at) = lo8;
-        }
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
+            put(buffer(buf, 0, 0) + kr * HD + (ch ^ chunk_key<HD>(kr)) * 8, cd.k[i],
+                [&](int) { return cd.ks[i]; }, [&](int) { return cd.km[i]; });
             const int vw = w0 % HD + i, d = vw % ND * 16 + vw / ND;
-            h8 hi8, lo8;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float x = fmaf((float)cd.vs[i / 2][e],
-                                     (float)((cd.v[i] >> csdr::code_shift(e)) & 15u),
-                                     (float)cd.vm[i / 2][e]);
-                hi8[e] = (_Float16)x;
-                if constexpr (PLANES == 2) lo8[e] = (_Float16)(x - (float)hi8[e]);
-            }
-            const int at = (w0 / HD * HD + d) * 8;
-            *reinterpret_cast<h8*>(buffer(buf, 1, 0) + at) = hi8;
-            if constexpr (PLANES == 2) *reinterpret_cast<h8*>(buffer(buf, 1, PLANES - 1) + at) = lo8;
+            put(buffer(buf, 1, 0) + (w0 / HD * HD + d) * 8, cd.v[i],
+                [&](int e) { return cd.vs[i / 2][e]; }, [&](int e) { return cd.vm[i / 2][e]; });
         }
     };
     // zeros for V at positions of the tile that hold nothing (their weights are zero)
     auto clear = [&](int tb, int buf, const int* pg) {
-        for (int i = tid; i < TP * HD; i += 256) {
+        for (int i = tid; i < TP * HD; i += 64 * NW) {
             const int pos = i / (8 * HD) * 8 + i % 8;
             int page = pg[0];
 #pragma unroll
@@ -1009,51 +1004,44 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
                                     k1, qh[q][s], acc[q][u], 0, 0, 0);
                         }
                     }
-                float x[NQ][8];
-                bool move = false;
-                float top[NQ];
                 const int p8 = tb + 32 * hb + 8 * g;
+                h8 wh[NQ], wl[PAIR ? NQ : 1];
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
+                    // scores, without options still in the products' units
+                    float x[8], top = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        x[q][j] = score2<OPTS>(a, acc[q][j >> 2][j & 3], unit[q], slope[q],
-                                               pq[q] - (p8 + j));
+                    for (int j = 0; j < 8; ++j) {
+                        x[j] = acc[q][j >> 2][j & 3];
+                        if constexpr (OPTS)
+                            x[j] = score2<OPTS>(a, x[j], unit[q], slope[q], pq[q] - (p8 + j));
+                    }
                     if (!whole) {
-                        const bool page = have >> ((32 * hb + 8 * g) / 16) & 1;
+                        const bool row = (have >> ((32 * hb + 8 * g) / 16) & 1) & (pq[q] >= 0);
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            if (!(page && pq[q] >= 0 && seen.at(pq[q], p8 + j)))
-                                x[q][j] = -INFINITY;
+                            if (!(row & seen.at(pq[q], p8 + j))) x[j] = -INFINITY;
                     }
-                    top[q] = kNoMax;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) top[q] = fmaxf(top[q], x[q][j]);
-                    move = move || top[q] > m[q] + kLag;
-                }
-                if (__any(move)) {
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-                        const float mn = fmaxf(m[q], lanes16_max(top[q]));
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
+                    if constexpr (!OPTS) top *= unit[q];
+                    if (__any(top > m[q] + kLag<XT>)) {
+                        const float mn = fmaxf(m[q], lanes16_max(top));
                         const float f = exp2_fast(m[q] - mn);
                         l[q] *= f;
 #pragma unroll
                         for (int d = 0; d < ND; ++d) o[q][d] *= f;
                         m[q] = mn;
                     }
-                }
-                h8 wh[NQ], wl[PAIR ? NQ : 1];
+                    const float off = kBias<XT> - m[q];
+                    float w8[8];
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    float w8[8], sum = 0.0f;
-                    const float off = kBias - m[q];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        w8[j] = exp2_fast(x[q][j] + off);
-                        sum += w8[j];
-                    }
-                    l[q] += sum;
+                    for (int j = 0; j < 8; ++j)
+                        w8[j] = exp2_fast(OPTS ? x[j] + off : fmaf(x[j], unit[q], off));
                     split8<PAIR>(w8, wh[q], wl[PAIR ? q : 0]);
+                    l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wh[q], l[q], 0, 0, 0);
+                    if constexpr (PAIR)
+                        l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wl[q], l[q], 0, 0, 0);
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
@@ -1083,8 +1071,8 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
 
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-        const int t0 = col0 + 16 * (4 * q + wave), col = t0 + c;
-        l[q] = lanes16_sum(l[q]);
+        const int t0 = col0 + 16 * (NW * q + wave), col = t0 + c;
+        const float sum = l[q][0];
         const long long row = (long long)r.first + col / G;
         const int h = kvh * G + col % G;
         if (sp.n > 1) {
@@ -1095,13 +1083,13 @@ __global__ __launch_bounds__(256, 2) void prompt_kernel(AttnArgs a, Splits sp) {
                     *reinterpret_cast<f4*>(sp.vecs + part * HD + 16 * d + 4 * g) = o[q][d];
                 if (g == 0) {
                     sp.stats[2 * part] = m[q];
-                    sp.stats[2 * part + 1] = l[q];
+                    sp.stats[2 * part + 1] = sum;
                 }
             }
             continue;
         }
-        bool fine = l[q] > 0.0f && l[q] < INFINITY;
-        const float inv = 1.0f / l[q];
+        bool fine = sum > 0.0f && sum < INFINITY;
+        const float inv = 1.0f / sum;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             o[q][d] *= inv;
@@ -1171,18 +1159,18 @@ template <int HD, bool Q4, typename XT, bool OPTS>
 void launch_kernel(const AttnArgs& a, const Splits& s, hipStream_t st) {
     const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
     if (cols > kStepColumns) {
-        constexpr int NQ = prompt_tiles<HD, Q4, XT>();
-        using Shape = PromptShape<HD, Q4, XT, NQ>;
+        constexpr int NQ = prompt_tiles<HD, Q4, XT>(), NW = 4;
+        using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
+        constexpr auto kernel = &prompt_kernel<HD, Q4, XT, OPTS, NQ, NW>;
         static const bool raised = [] {
-            (void)hipFuncSetAttribute(
-                reinterpret_cast<const void*>(&prompt_kernel<HD, Q4, XT, OPTS, NQ>),
-                hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
+            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
             return true;
         }();
         (void)raised;
         const int blocks = (cols + Shape::kColumns - 1) / Shape::kColumns;
-        prompt_kernel<HD, Q4, XT, OPTS, NQ>
-            <<<dim3((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n), 256, Shape::kLds, st>>>(a, s);
+        kernel<<<dim3((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n), 64 * NW, Shape::kLds, st>>>(
+            a, s);
         if (s.n == 1) return;
     } else {
         const dim3 grid(a.pv.n_seqs * a.pv.hkv, s.n, (cols + kCols - 1) / kCols);
