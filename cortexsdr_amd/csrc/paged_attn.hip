@@ -57,6 +57,22 @@ __device__ __forceinline__ Seen seen_of(const AttnArgs& a, int b, const SeqRows&
     return s;
 }
 
+// The tiles of T positions that columns at positions pq0 .. pq1 see: `low` tiles from 0 on (prefix),
+// then those from w0 on (window and causal part), n in all.
+template <int T>
+struct Tiles {
+    int low, w0, n;
+    __device__ Tiles(const Seen& s, int pq0, int pq1) {
+        const int first = max(0, pq0 - min(pq0 + 1, s.window) + 1) / T * T;
+        const int end = pq1 < 0 ? 0 : min(s.keys, max(pq1 + 1, s.prefix));
+        const int prefix = min(max(s.prefix, 0), s.keys);
+        w0 = first;
+        low = pq1 < 0 ? 0 : min((prefix + T - 1) / T, first / T);
+        n = low + max(0, (end - first + T - 1) / T);
+    }
+    __device__ int at(int i) const { return i < low ? i * T : w0 + (i - low) * T; }
+};
+
 __device__ __forceinline__ float shaped(const AttnArgs& a, float s, float slope, int dist) {
     if (a.cap > 0.0f) s = a.cap * tanhf(s * a.inv_cap);
     return s - slope * (float)abs(dist);
@@ -386,19 +402,10 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
     const int pq0 = r.p0 + col0 / G, pq1 = r.p0 + (col0 + ncol - 1) / G;
     const float slope = OPTS && a.slopes ? a.slopes[h] : 0.0f;
 
-    // positions that some column sees: below `first` only the prefix
-    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);
-    const int end = pq1 < 0 ? 0 : min(seen.keys, max(pq1 + 1, seen.prefix));
-    const int lo = split * sp.len, hi = split == sp.n - 1 ? end : min(end, lo + sp.len);
-    auto next_tile = [&](int tb) {  // the next tile that some column sees, or hi
-        tb += kTile * kStepWaves;
-        if (tb < hi && tb >= seen.prefix && tb + kTile <= first) {
-            const int skip = (first - kTile - tb) / (kTile * kStepWaves) + 1;
-            tb += skip * kTile * kStepWaves;
-            // (prefix tiles lie below tb already: nothing between is seen)
-        }
-        return tb;
-    };
+    const Tiles<kTile> tiles(seen, pq0, pq1);
+    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);  // below: only the prefix
+    const int lo = split * (sp.len / kTile);
+    const int hi = split == sp.n - 1 ? tiles.n : min(tiles.n, lo + sp.len / kTile);
 
     h8 qh[NS], ql[NS];
     const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
@@ -592,26 +599,26 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
         }
         if constexpr (MORE) load_v<HD, Q4>(t, pv, pages_of<HD, Q4>(pv.v, pv, kvh, ng0, ng1), nb, at);
     };
-    int tb = next_tile(lo + kTile * (wave - kStepWaves));
-    if (tb < hi) {
+    int i = lo + wave;
+    if (i < hi) {
         auto pages_at = [&](int p, int& x, int& y) {
             x = csdr::page_of(pv, b, p);
             y = pv.shift == 4 ? csdr::page_of(pv, b, p + 16) : x;
         };
-        int pg0, pg1, ng0 = -1, ng1 = -1;
+        int tb = tiles.at(i), nb = tiles.at(i + kStepWaves);
+        int pg0, pg1, ng0, ng1;
         pages_at(tb, pg0, pg1);
         const Pages kp = pages_of<HD, Q4>(pv.k, pv, kvh, pg0, pg1);
         const Pages vp = pages_of<HD, Q4>(pv.v, pv, kvh, pg0, pg1);
         load_k<HD, Q4>(t, pv, kp, tb, at);
         if constexpr (Q4) load_par<HD>(t, pv, kp, vp, tb, at);
         load_v<HD, Q4>(t, pv, vp, tb, at);
-        int nb = next_tile(tb);
-        if (nb < hi) pages_at(nb, ng0, ng1);
-        while (nb < hi) {
+        pages_at(nb, ng0, ng1);  // (-1 past the table)
+        for (i += kStepWaves; i < hi; i += kStepWaves) {
             // the page ids of the tile after the next are on their way during this one
-            const int nn = next_tile(nb);
+            const int nn = tiles.at(i + kStepWaves);
             int nng0, nng1;
-            pages_at(nn, nng0, nng1);  // (-1 past the table)
+            pages_at(nn, nng0, nng1);
             tile(std::true_type{}, tb, pg0, pg1, nb, ng0, ng1);
             tb = nb;
             pg0 = ng0;
@@ -766,7 +773,7 @@ __device__ __forceinline__ int chunk_key(int r) {
 }
 
 template <int HD, bool Q4, typename XT, bool OPTS, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Splits sp) {
+__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnArgs a, Splits sp) {
     using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
     constexpr bool PAIR = Shape::kPair;
     constexpr int NS = HD / 32, ND = HD / 16, TP = Shape::TP, PLANES = Shape::kPlanes;
@@ -790,15 +797,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Spl
     const int last_col = min(ncols, col0 + Shape::kColumns) - 1;
     const int pq0 = pos_of(col0), pq1 = pos_of(last_col);  // of the workgroup
 
-    // positions that some column sees: below `first` only the prefix
-    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);
-    const int end = pq1 < 0 ? 0 : min(seen.keys, max(pq1 + 1, seen.prefix));
-    const int lo = split * sp.len, hi = split == sp.n - 1 ? end : min(end, lo + sp.len);
-    auto next_tile = [&](int tb) {
-        tb += TP;
-        if (tb < hi && tb >= seen.prefix && tb + TP <= first) tb += (first - TP - tb) / TP * TP + TP;
-        return tb;
-    };
+    const Tiles<TP> tiles(seen, pq0, pq1);
+    const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);  // below: only the prefix
+    const int lo = split * (sp.len / TP);
+    const int hi = split == sp.n - 1 ? tiles.n : min(tiles.n, lo + sp.len / TP);
 
     // the columns of this lane: tile q holds columns col0 + 16 (NW q + wave) + c
     h8 qh[NQ][NS], ql[PAIR ? NQ : 1][NS];
@@ -943,14 +945,15 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Spl
         }
     };
 
-    int tb = next_tile(lo - TP), buf = 0;
+    int buf = 0;
     int pg[GR] = {};
-    if (tb < hi) {
-        pages_at(tb, pg);
-        fetch(tb, 0, pg);
+    if (lo < hi) {
+        pages_at(tiles.at(lo), pg);
+        fetch(tiles.at(lo), 0, pg);
         if constexpr (Q4) unpack(0);
     }
-    while (tb < hi) {
+    for (int i = lo; i < hi; ++i) {
+        const int tb = tiles.at(i);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wave's pieces are in LDS)
         __syncthreads();  // the tile is whole, and everyone is done with the other buffer
         bool held = tb + TP <= seen.keys;
@@ -964,10 +967,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Spl
             clear(tb, buf, pg);
             __syncthreads();
         }
-        const int nb = next_tile(tb);
-        if (Q4 || nb < hi) {  // (4 bits: the last tile again, so that the registers are always set)
-            pages_at(min(nb, hi - 1) / TP * TP, pg);
-            fetch(min(nb, hi - 1) / TP * TP, buf ^ 1, pg);
+        if (Q4 || i + 1 < hi) {  // (4 bits: the last tile again, so that the registers are set)
+            const int nb = tiles.at(min(i + 1, hi - 1));
+            pages_at(nb, pg);
+            fetch(nb, buf ^ 1, pg);
         }
         const bool any = wp0 <= wp1 && ((tb <= wp1 && tb + TP > first) || tb < seen.prefix);
         const bool whole = held && wp0 >= 0 &&
@@ -1065,7 +1068,6 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Spl
             }
         }
         if constexpr (Q4) unpack(buf ^ 1);
-        tb = nb;
         buf ^= 1;
     }
 
@@ -1117,24 +1119,35 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void prompt_kernel(AttnArgs a, Spl
 
 // Up to this many columns of a KV head go to step_kernel (16 at a time), more to prompt_kernel.
 constexpr int kStepColumns = 64;
-constexpr int kPromptColumns = 128;  // of the smallest workgroup of prompt_kernel
+constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
+constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
-// Positions per split. step_kernel: about 1024 workgroups in all (4 to a CU), 128 positions (a tile
-// per wave) at least. prompt_kernel: one split if there are 512 workgroups (two to a CU), else
-// enough for that, 512 positions at least.
-Splits splits_of(const PagedView& pv, int hq, int max_len) {
+// Positions per split, counted over the tiles that a workgroup sees (all, or a window's): for
+// step_kernel about 1024 workgroups in all (4 to a CU), 128 positions (a tile per wave) at least;
+// for prompt_kernel one split if there are 512 workgroups, else enough for that, 512 positions at
+// least. A window only ever makes the splits shorter, not more.
+Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
     Splits s{};
+    const int G = hq / pv.hkv;
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
-    const long long cols = (long long)pv.max_q * (hq / pv.hkv);
+    const long long cols = (long long)pv.max_q * G;
     const bool step = cols <= kStepColumns;
-    const long long per = step ? kCols : kPromptColumns, unit = step ? kTile * kStepWaves : 512;
+    const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
-    const long long target = step ? 1024 : 512;
-    long long each = step || wgs < target ? (len * wgs + target - 1) / target : len;
-    each = std::max(unit, (each + unit - 1) / unit * unit);
-    s.len = (int)std::min(each, (long long)csdr::kMaxPositions);
+    const long long target = step ? 1024 : kPromptBlocks;
+    auto each = [&](long long n) {
+        const long long e = step || wgs < target ? (n * wgs + target - 1) / target : n;
+        return std::max(unit, (e + unit - 1) / unit * unit);
+    };
+    s.len = (int)std::min(each(len), (long long)csdr::kMaxPositions);
     s.n = (int)((len + s.len - 1) / s.len);
+    // (a block's columns see a window each, and two tiles more where these do not fall on tiles)
+    const long long seen = (long long)window + std::min(cols, per) / G + 2 * 64;
+    if (window > 0 && seen < len) {
+        s.len = (int)each(seen);
+        s.n = (int)std::min((long long)s.n, (seen + s.len - 1) / s.len);
+    }
     return s;
 }
 
@@ -1149,28 +1162,43 @@ size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
     return csdr::align_up(parts * 8, 16) + parts * hd * 4;
 }
 
-// Column tiles per wave of prompt_kernel: as many as 256 registers hold (sums, queries, weights).
-template <int HD, bool Q4, typename XT>
-constexpr int prompt_tiles() {
-    return HD == 128 ? (sizeof(XT) == 4 || Q4 ? 2 : 3) : (sizeof(XT) == 4 || Q4 ? 3 : 4);
+// Column tiles per wave of prompt_kernel: as many as 256 registers hold (sums, queries, weights), or
+// one where that would leave the chip without two workgroups a CU (SMALL). Waves per workgroup:
+// eight where 4-bit rows of 128 are unpacked, which then serves twice the columns.
+template <int HD, bool Q4, typename XT, bool SMALL>
+struct PromptConfig {
+    static constexpr int NQ =
+        SMALL ? 1 : HD == 128 ? (sizeof(XT) == 4 || Q4 ? 2 : 3) : (sizeof(XT) == 4 || Q4 ? 3 : 4);
+    static constexpr int NW = !SMALL && Q4 && HD == 128 ? 8 : 4;
+    using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
+};
+
+template <int HD, bool Q4, typename XT, bool OPTS, bool SMALL>
+void launch_prompt(const AttnArgs& a, const Splits& s, hipStream_t st) {
+    using Config = PromptConfig<HD, Q4, XT, SMALL>;
+    using Shape = typename Config::Shape;
+    constexpr auto kernel = &prompt_kernel<HD, Q4, XT, OPTS, Config::NQ, Config::NW>;
+    static const bool raised = [] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
+        return true;
+    }();
+    (void)raised;
+    const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
+    const int blocks = (cols + Shape::kColumns - 1) / Shape::kColumns;
+    const dim3 grid((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n);
+    kernel<<<grid, 64 * Config::NW, Shape::kLds, st>>>(a, s);
 }
 
 template <int HD, bool Q4, typename XT, bool OPTS>
 void launch_kernel(const AttnArgs& a, const Splits& s, hipStream_t st) {
     const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
     if (cols > kStepColumns) {
-        constexpr int NQ = prompt_tiles<HD, Q4, XT>(), NW = 4;
-        using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
-        constexpr auto kernel = &prompt_kernel<HD, Q4, XT, OPTS, NQ, NW>;
-        static const bool raised = [] {
-            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
-            return true;
-        }();
-        (void)raised;
-        const int blocks = (cols + Shape::kColumns - 1) / Shape::kColumns;
-        kernel<<<dim3((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n), 64 * NW, Shape::kLds, st>>>(
-            a, s);
+        const long long columns = PromptConfig<HD, Q4, XT, false>::Shape::kColumns;
+        if ((long long)a.pv.n_seqs * a.pv.hkv * cols < kPromptBlocks * columns)
+            launch_prompt<HD, Q4, XT, OPTS, true>(a, s, st);
+        else
+            launch_prompt<HD, Q4, XT, OPTS, false>(a, s, st);
         if (s.n == 1) return;
     } else {
         const dim3 grid(a.pv.n_seqs * a.pv.hkv, s.n, (cols + kCols - 1) / kCols);
@@ -1203,7 +1231,7 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
         Hq % kv->n_kv_heads || max_len < 0)
         return 0;
-    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len));
+    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len, 0));
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
@@ -1241,7 +1269,7 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     if ((long long)kv->n_seqs * std::max((long long)a.pv.max_q, kv->n_kv_heads * cols) >
         0x7fffffffLL)
         return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
-    Splits s = splits_of(a.pv, Hq, max_len);
+    Splits s = splits_of(a.pv, Hq, max_len, a.window);
     const size_t need = workspace_of(a.pv, Hq, hd, s);
     if (need && (!workspace || workspace_bytes < need ||
                  reinterpret_cast<uintptr_t>(workspace) % 16))
