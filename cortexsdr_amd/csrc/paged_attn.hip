@@ -759,8 +759,12 @@ template <int HD, bool Q4, typename XT, int NQ, int NW>
 struct PromptShape {
     static constexpr bool kPair = sizeof(XT) == 4;
     static constexpr int kPlanes = Q4 && kPair ? 2 : 1;
-    // positions per tile: LDS for two workgroups of four waves or one of eight on a CU
-    static constexpr int TP = kPlanes == 2 && HD == 128 && NW == 4 ? 32 : 64;
+    // positions per tile, and waves per SIMD: LDS for two workgroups of four waves or one of eight
+    // on a CU; three of four where 168 registers do (4096 tokens of fp16, HD 128: tiles of 64 and
+    // two waves 171 us, of 32 and three 164)
+    static constexpr bool kLean = !Q4 && !kPair && HD == 128;
+    static constexpr int kSimdWaves = kLean ? 3 : 2;
+    static constexpr int TP = (kPlanes == 2 && HD == 128 && NW == 4) || kLean ? 32 : 64;
     static constexpr int kPlane = TP * HD;                          // halves
     static constexpr int kLds = 2 * 2 * kPlanes * kPlane * 2;       // bytes
     static constexpr int kColumns = NW * 16 * NQ;
@@ -773,7 +777,8 @@ __device__ __forceinline__ int chunk_key(int r) {
 }
 
 template <int HD, bool Q4, typename XT, bool OPTS, int NQ, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnArgs a, Splits sp) {
+__global__ __launch_bounds__(64 * NW, (PromptShape<HD, Q4, XT, NQ, NW>::kSimdWaves)) void
+prompt_kernel(AttnArgs a, Splits sp) {
     using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
     constexpr bool PAIR = Shape::kPair;
     constexpr int NS = HD / 32, ND = HD / 16, TP = Shape::TP, PLANES = Shape::kPlanes;
@@ -784,9 +789,15 @@ __global__ __launch_bounds__(64 * NW, 2) void prompt_kernel(AttnArgs a, Splits s
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.hq / pv.hkv;
     // (sequence, KV head) fastest: on a chip of 8 dies that take workgroups in turn, the blocks of
-    // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns first.
-    const int pairs = pv.n_seqs * pv.hkv;
-    const int bh = blockIdx.x % pairs, block = (int)(gridDim.x / pairs) - 1 - blockIdx.x / pairs;
+    // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns, which see
+    // most, first; where a CU takes two workgroups, the second 256 in the opposite order, so that a CU
+    // with the longest of the first has the shortest of the second (4096 tokens: 182 -> 175 us).
+    const int pairs = pv.n_seqs * pv.hkv, blocks = gridDim.x / pairs;
+    const int bh = blockIdx.x % pairs, around = max(1, 256 / pairs);
+    int rank = blockIdx.x / pairs;
+    if (NW == 4 && rank >= around && rank < min(2 * around, blocks))
+        rank = around + min(2 * around, blocks) - 1 - rank;
+    const int block = blocks - 1 - rank;
     const int b = bh / pv.hkv, kvh = bh % pv.hkv, split = blockIdx.y;
     const SeqRows r = csdr::seq_rows(pv, b);
     const int ncols = r.n * G, col0 = block * Shape::kColumns;
@@ -1168,7 +1179,7 @@ size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
 template <int HD, bool Q4, typename XT, bool SMALL>
 struct PromptConfig {
     static constexpr int NQ =
-        SMALL ? 1 : HD == 128 ? (sizeof(XT) == 4 || Q4 ? 2 : 3) : (sizeof(XT) == 4 || Q4 ? 3 : 4);
+        SMALL ? 1 : HD == 128 ? 2 : sizeof(XT) == 4 || Q4 ? 3 : 4;
     static constexpr int NW = !SMALL && Q4 && HD == 128 ? 8 : 4;
     using Shape = PromptShape<HD, Q4, XT, NQ, NW>;
 };
