@@ -71,6 +71,12 @@ struct Tiles {
         n = low + max(0, (end - first + T - 1) / T);
     }
     __device__ int at(int i) const { return i < low ? i * T : w0 + (i - low) * T; }
+    // Tiles [lo, hi) of a split: equal shares of what there is, in whole units of tiles.
+    __device__ void share(int split, int splits, int unit, int& lo, int& hi) const {
+        const int each = ((n + splits - 1) / splits + unit - 1) / unit * unit;
+        lo = min(n, split * each);
+        hi = min(n, lo + each);
+    }
 };
 
 __device__ __forceinline__ float shaped(const AttnArgs& a, float s, float slope, int dist) {
@@ -367,7 +373,7 @@ __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int
 }
 
 struct Splits {
-    int len, n;  // positions per split, splits
+    int n;         // of the tiles that a workgroup's columns see
     float* stats;  // 2 per (row, head, split): exponent offset and sum
     float* vecs;   // HD per (row, head, split)
 };
@@ -404,8 +410,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
 
     const Tiles<kTile> tiles(seen, pq0, pq1);
     const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);  // below: only the prefix
-    const int lo = split * (sp.len / kTile);
-    const int hi = split == sp.n - 1 ? tiles.n : min(tiles.n, lo + sp.len / kTile);
+    int lo, hi;
+    tiles.share(split, sp.n, kStepWaves, lo, hi);
 
     h8 qh[NS], ql[NS];
     const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
@@ -810,8 +816,8 @@ prompt_kernel(AttnArgs a, Splits sp) {
 
     const Tiles<TP> tiles(seen, pq0, pq1);
     const int first = max(0, pq0 - min(pq0 + 1, seen.window) + 1);  // below: only the prefix
-    const int lo = split * (sp.len / TP);
-    const int hi = split == sp.n - 1 ? tiles.n : min(tiles.n, lo + sp.len / TP);
+    int lo, hi;
+    tiles.share(split, sp.n, 256 / TP, lo, hi);
 
     // the columns of this lane: tile q holds columns col0 + 16 (NW q + wave) + c
     h8 qh[NQ][NS], ql[PAIR ? NQ : 1][NS];
@@ -1133,12 +1139,12 @@ constexpr int kStepColumns = 64;
 constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
 constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
-// Positions per split, counted over the tiles that a workgroup sees (all, or a window's): for
-// step_kernel about 1024 workgroups in all (4 to a CU), 128 positions (a tile per wave) at least;
-// for prompt_kernel one split if there are 512 workgroups, else enough for that, 512 positions at
-// least. A window only ever makes the splits shorter, not more.
+// Splits of the positions: for step_kernel about 1024 workgroups in all (4 to a CU), 128 positions (a
+// tile per wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for
+// that, 512 positions at least. A sequence's positions are shared out equally, so a call with
+// sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
+// ever makes fewer splits.
 Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
-    Splits s{};
     const int G = hq / pv.hkv;
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
@@ -1147,18 +1153,12 @@ Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
     const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
     const long long target = step ? 1024 : kPromptBlocks;
-    auto each = [&](long long n) {
-        const long long e = step || wgs < target ? (n * wgs + target - 1) / target : n;
-        return std::max(unit, (e + unit - 1) / unit * unit);
-    };
-    s.len = (int)std::min(each(len), (long long)csdr::kMaxPositions);
-    s.n = (int)((len + s.len - 1) / s.len);
     // (a block's columns see a window each, and two tiles more where these do not fall on tiles)
-    const long long seen = (long long)window + std::min(cols, per) / G + 2 * 64;
-    if (window > 0 && seen < len) {
-        s.len = (int)each(seen);
-        s.n = (int)std::min((long long)s.n, (seen + s.len - 1) / s.len);
-    }
+    const long long seen =
+        window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
+    Splits s{};
+    s.n = (int)std::max(1LL, std::min((seen + unit - 1) / unit,
+                                      step ? (target + wgs - 1) / wgs : target / wgs));
     return s;
 }
 
