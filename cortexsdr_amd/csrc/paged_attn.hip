@@ -171,6 +171,17 @@ __device__ __forceinline__ h8 codes16(uint32_t w, uint32_t magic) {
     return __builtin_bit_cast(h8, r);
 }
 
+// code - 8: the codes at the foot of a mantissa of 1024 or, four bits up, of 64, where pairs need
+// no shift of their own (`m0`, `m1`: 1024.0 and 64.0 twice, in vector registers).
+__device__ __forceinline__ h8 codes8(uint32_t w, uint32_t m0, uint32_t m1) {
+    const uint32_t v = w >> 8;
+    const h2 a = __builtin_bit_cast(h2, (w & 0x000F000Fu) | m0) - (_Float16)1032.0f;
+    const h2 b = __builtin_bit_cast(h2, (w & 0x00F000F0u) | m1) - (_Float16)72.0f;
+    const h2 c = __builtin_bit_cast(h2, (v & 0x000F000Fu) | m0) - (_Float16)1032.0f;
+    const h2 d = __builtin_bit_cast(h2, (v & 0x00F000F0u) | m1) - (_Float16)72.0f;
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // x times y (fp32 values with fp16 factors), rounded to fp16, and what the rounding left: both
 // straight from the exact product (v_fma_mix).
 template <bool PAIR>
@@ -218,12 +229,13 @@ struct Tile<HD, true> {
 // A tile's scales and minima, 16-byte pieces of 8 positions: piece 4 r + i holds positions 8 i ..
 // of row r: K's scales of the HD / 32 groups, K's minima, then from piece 32 V's likewise. A lane
 // loads one piece; the wave shares them through LDS, where four lanes' addresses serve all 64
-// (loading what each lane needs took 14 loads and 56 registers a tile: 163 us -> MEASURED us for
-// 64 sequences of about 6000 positions).
+// (what each lane needs, loaded by itself, takes 14 loads and 56 registers a tile). `k` holds K's
+// once more, the rows of each position side by side.
 template <int HD>
 struct TileParams {
     static constexpr int kMin = HD / 32, kV = 8;  // first rows
     h8 piece[64];
+    h8 k[32];
     __device__ h8 at(int row, int i) const { return piece[4 * row + i]; }
 };
 
@@ -340,10 +352,10 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, 
 }
 
 // A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a power
-// of two that puts its largest magnitude in [2^13, 2^14), then in pairs of fp16. A negative scale
-// turns the query round. Returns the (positive) factor from products to scores, in the log2 domain
+// of two that puts its largest magnitude in [2^TOP, 2^(TOP + 1)), then in pairs of fp16 (fp16: as it
+// is unless TOP is given). A negative scale turns the query round. Returns the (positive) factor from products to scores, in the log2 domain
 // if there are no options.
-template <int HD, typename XT, bool OPTS>
+template <int HD, typename XT, bool OPTS, int TOP = sizeof(XT) == 4 ? 13 : 0>
 __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int g, h8* qh, h8* ql) {
     constexpr bool PAIR = sizeof(XT) == 4;
     float unit = fabsf(OPTS ? a.scale : a.scale * kLog2e);
@@ -355,10 +367,10 @@ __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int
             x[s][j] = (float)qp[32 * s + 8 * g + j];
             big = fmaxf(big, fabsf(x[s][j]));
         }
-    if constexpr (PAIR) {
+    if constexpr (TOP != 0) {
         big = lanes16_max(big);
         const int e = (int)(__float_as_uint(big) >> 23) - 127;
-        const int k = big > 0.0f ? min(max(13 - e, -120), 120) : 0;
+        const int k = big > 0.0f ? min(max(TOP - e, -120), 120) : 0;
         f = __uint_as_float((uint32_t)(127 + k) << 23);
         unit *= __uint_as_float((uint32_t)(127 - k) << 23);
     }
@@ -385,12 +397,11 @@ struct Splits {
 //     positions 8 g .. 8 g + 7, which is just what it has to give as B operand of
 //   O^T += V^T P^T, whose A operand is a 16-byte piece of V's page.
 // So nothing crosses lanes but the maximum, and that only when it moves by more than kLag.
-// 4 bits: codes enter the products as whole numbers (16 + code for K, the -16 folded into the
-// accumulator's start; code - 8 for V, centred, so that sums do not cancel); K's scale and minimum
-// are applied to the group's 32-dim partial score, V's scale to the weights, its minimum through
-// a sum of its own per group. fp32 calls carry q and the weights as pairs of fp16 (22 bits).
+// 4 bits: codes enter the products as whole numbers (16 + code for K; code - 8 for V, centred, so
+// that sums do not cancel); K's scale is applied to the group's 32-dim partial score, V's to the
+// weights, and what the minima (and the 16) add comes from small products of their own. fp32 calls carry q and the weights as pairs of fp16 (22 bits).
 template <int HD, bool Q4, typename XT, bool OPTS>
-__global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Splits sp) {
+__global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Splits sp) {
     constexpr bool PAIR = sizeof(XT) == 4;
     constexpr int NS = HD / 32, ND = HD / 16;
     const PagedView& pv = a.pv;
@@ -415,18 +426,27 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
 
     h8 qh[NS], ql[NS];
     const XT* qp = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
-    const float unit = load_query<HD, XT, OPTS>(a, qp, g, qh, ql);
-    float qsum[Q4 ? NS : 1];  // sums of the groups of 32 dims
-    if constexpr (Q4)
+    const float unit = load_query<HD, XT, OPTS, Q4 ? 5 : PAIR ? 13 : 0>(a, qp, g, qh, ql);
+    // 4 bits: what the groups' minima and the 16 too many in the codes add to a score, the sum over
+    // groups of minimum * qsum - scale * 16 qsum, is a product of its own: row 0 .. of a position's
+    // parameters against these (in two halves; |q| below 2^6 keeps 16 qsum in fp16)
+    h8 sh, sl;
+    if constexpr (Q4) {
+        float x[8] = {};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             float t = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) t += PAIR ? (float)qh[s][j] + (float)ql[s][j] : (float)qh[s][j];
-            qsum[s] = lanes16_sum(t);
+            t = lanes16_sum(t);
+            x[s] = g == 0 ? -16.0f * t : 0.0f;
+            x[NS + s] = g == 0 ? t : 0.0f;
         }
+        split8<true>(x, sh, sl);
+    }
     __shared__ TileParams<HD> params[Q4 ? kStepWaves : 1];
     TileParams<HD>& tp = params[Q4 ? wave : 0];
+    if (Q4 && NS < 4) tp.k[lane & 31] = h8{};  // (its unused half meets zeros)
 
     f4 o[ND];
 #pragma unroll
@@ -436,7 +456,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
     // exponent above V's largest scale (from fp16's smallest): weights are 2^-ev of the above
     float ev = Q4 ? -24.0f : 0.0f, vtop = 0x1p-24f;
     uint32_t magic = 0x4C004C00u;
-    asm("" : "+v"(magic));  // (kept in a register)
+    uint32_t m0 = 0x64006400u, m1 = 0x54005400u;
+    asm("" : "+v"(magic), "+v"(m0), "+v"(m1));  // (kept in registers)
 
     const LaneOffsets<HD, Q4> at(pv, lane);
     Tile<HD, Q4> t;
@@ -478,11 +499,23 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
 #pragma unroll
                 for (int j = 0; j < 8; ++j) vscale = fmaxf(vscale, (float)t.par[j]);
             tp.piece[lane] = t.par;
+            if (lane < 8 * NS)  // K's row lane / 4 of positions 8 (lane % 4) ..
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    reinterpret_cast<_Float16*>(&tp.k[8 * (lane & 3) + j])[lane >> 2] = t.par[j];
         }
 
         // scores of positions p8 + j
         float s8[8];
         f4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        if constexpr (Q4) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const h8 kp = tp.k[8 * (c >> 2) + 4 * u + (c & 3)];
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kp, sh, acc[u], 0, 0, 0);
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kp, sl, acc[u], 0, 0, 0);
+            }
+        }
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             if constexpr (!Q4) {
@@ -493,20 +526,17 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
                         acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[u][s], ql[s], acc[u], 0, 0, 0);
                 }
             } else {
-                const float z = -16.0f * qsum[s];
-                const h8 ks = tp.at(s, g), km = tp.at(TileParams<HD>::kMin + s, g);
+                const h8 ks = tp.at(s, g);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const h8 kc = codes16(t.k[u][s], magic);
-                    f4 part = {z, z, z, z};
+                    f4 part = {0.f, 0.f, 0.f, 0.f};
                     part = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, qh[s], part, 0, 0, 0);
                     if constexpr (PAIR)
                         part = __builtin_amdgcn_mfma_f32_16x16x32_f16(kc, ql[s], part, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 4; ++i)
                         acc[u][i] = fmaf((float)ks[4 * u + i], part[i], acc[u][i]);
-                        acc[u][i] = fmaf((float)km[4 * u + i], qsum[s], acc[u][i]);
-                    }
                 }
             }
         }
@@ -596,7 +626,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(AttnArgs a, Sp
                 split8<PAIR>(w8, tp.at(TileParams<HD>::kV + s, g), wh, wl);
 #pragma unroll
                 for (int d = 2 * s; d < 2 * s + 2; ++d) {
-                    const h8 vc = codes16(t.v[d], magic) - (_Float16)24.0f;
+                    const h8 vc = codes8(t.v[d], m0, m1);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wh, o[d], 0, 0, 0);
                     if constexpr (PAIR)
                         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[d], 0, 0, 0);
@@ -1139,8 +1169,10 @@ constexpr int kStepColumns = 64;
 constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
 constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
-// Splits of the positions: for step_kernel about 1024 workgroups in all (4 to a CU), 128 positions (a
-// tile per wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for
+// Splits of the positions: for step_kernel 768 workgroups in all (the three that a CU holds at once),
+// or twice as many where sequences may differ in length (one sequence of 131071 on 4-bit pages: 768
+// 50 us, 1536 57; 64 sequences of 4096 to 8192: 148 and 139), 128 positions (a tile per wave) each
+// at least; for prompt_kernel one if there are 512 workgroups, else enough for
 // that, 512 positions at least. A sequence's positions are shared out equally, so a call with
 // sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
 // ever makes fewer splits.
@@ -1152,7 +1184,7 @@ Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
     const bool step = cols <= kStepColumns;
     const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
-    const long long target = step ? 1024 : kPromptBlocks;
+    const long long target = !step ? kPromptBlocks : pv.n_seqs == 1 ? 768 : 1536;
     // (a block's columns see a window each, and two tiles more where these do not fall on tiles)
     const long long seen =
         window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
