@@ -38,22 +38,23 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
     if workspace is None:
         need = lib.csdr_token_logprobs_workspace_bytes(rows, n, top_n)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    out = torch.empty((2 + 2 * max(top_n, 0), rows), dtype=torch.float32, device=dev)
-    lp = out[0] if tokens is not None else None
+    lp, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
     ids = top = None
     if top_n > 0:
-        ids = out[2:2 + top_n].view(torch.int32).view(rows, top_n)
-        top = out[2 + top_n:].view(rows, top_n)
+        ids = torch.empty((rows, top_n), dtype=torch.int32, device=dev)
+        top = torch.empty((rows, top_n), dtype=torch.float32, device=dev)
+    if tokens is None:
+        lp = None
     _check(lib.csdr_token_logprobs(
         logits.data_ptr(), dt, rows, n, logits.stride(0) if rows > 1 else 0, temperature,
         tokens.data_ptr() if tokens is not None else None,
-        lp.data_ptr() if lp is not None else None, out[1].data_ptr(), top_n,
+        lp.data_ptr() if lp is not None else None, entropy.data_ptr(), top_n,
         ids.data_ptr() if top_n > 0 else None, top.data_ptr() if top_n > 0 else None,
         workspace.data_ptr() if workspace is not None else None,
         workspace.numel() * workspace.element_size() if workspace is not None else 0,
         _stream_ptr(stream)))
     if stream is not None:
-        out.record_stream(stream)
-        if workspace is not None:
-            workspace.record_stream(stream)
-    return TokenLogprobs(lp, out[1], ids, top)
+        for t in (entropy, ids, top, workspace):
+            if t is not None:
+                t.record_stream(stream)
+    return TokenLogprobs(lp, entropy, ids, top)

@@ -101,6 +101,7 @@ class PagedBatch:
                                 int(table.shape[1]))
         self._ref = C.byref(self._kv)
         self._lib = _lib.load()
+        self._need = {}  # workspace bytes by the call's sizes
 
     def _starts(self, torch, q_start, max_q):
         if q_start is None:
@@ -112,21 +113,21 @@ class PagedBatch:
 
     def _heads(self, what: str, t, n_heads=None):
         """The token stride of (tokens, heads, head_dim) or (tokens, heads * head_dim)."""
-        hd = self.cache.head_dim
-        if t.dim() == 3:
-            ok = t.shape[2] == hd and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == hd)
-            n = t.shape[1]
+        hd, shape, stride = self.cache.head_dim, t.shape, t.stride()
+        if len(shape) == 3:
+            n = shape[1]
+            ok = shape[2] == hd and stride[2] == 1 and (n == 1 or stride[1] == hd)
         else:
-            ok = t.dim() == 2 and t.shape[1] % hd == 0 and t.stride(1) == 1
-            n = t.shape[-1] // hd
+            ok = len(shape) == 2 and shape[1] % hd == 0 and stride[1] == 1
+            n = shape[-1] // hd if ok else 0
         if not ok or n < 1 or (n_heads is not None and n != n_heads):
             raise ValueError(f"{what} must be (tokens, {n_heads or 'heads'}, {hd}) with a token's "
                              "values side by side")
-        if t.shape[0] < 2:
+        if shape[0] < 2:
             return n, 0
-        if t.stride(0) < n * hd:  # an expanded tensor, or rows that overlap
+        if stride[0] < n * hd:  # an expanded tensor, or rows that overlap
             raise ValueError(f"{what}: its tokens overlap")
-        return n, t.stride(0)
+        return n, stride[0]
 
     def append(self, q, k, v, theta: float = 0.0, q_start=None, max_q=None, q_out=None,
                stream=None):
@@ -191,7 +192,13 @@ class PagedBatch:
         starts, mq = self._starts(torch, q_start, max_q)
         _on_device(torch, "tensors", q, out, q_start, slopes, prefix, workspace)
         if workspace is None:
-            need = self._lib.csdr_paged_attn_workspace_bytes(self._ref, n, starts, mq, nq, max_len)
+            key = (n, starts is None, mq, nq, max_len)
+            need = self._need.get(key)
+            if need is None:
+                if len(self._need) >= 256:
+                    self._need.clear()
+                need = self._need[key] = self._lib.csdr_paged_attn_workspace_bytes(
+                    self._ref, n, starts, mq, nq, max_len)
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
                 if stream is not None:
