@@ -788,13 +788,13 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // fp16 pages go straight to LDS (16 bytes a lane); K's 16-byte chunks of a row are permuted within
 // the row on the way (chunk j of row r at j ^ key(r)), so that the 16 rows of an operand read fall
 // on distinct banks; V's pieces lie in operand order already. 4-bit pages are turned into fp16
-// values by the threads, one plane for fp16 calls (values rounded to 11 bits, which is what such a
-// call's inputs have), two for fp32 calls: value = hi + lo to 22 bits, and three products
-// hi hi, hi lo, lo hi.
+// values by the threads, in two planes: value = hi + lo to 22 bits, and products hi hi, lo hi and
+// for fp32 calls hi lo. (One plane, values rounded to 11 bits, would do with half the products for
+// fp16 calls, but left them 2.2 times as far off as the rounding of their outputs alone.)
 template <int HD, bool Q4, typename XT, int NQ, int NW>
 struct PromptShape {
     static constexpr bool kPair = sizeof(XT) == 4;
-    static constexpr int kPlanes = Q4 && kPair ? 2 : 1;
+    static constexpr int kPlanes = Q4 ? 2 : 1;
     // positions per tile, and waves per SIMD: LDS for two workgroups of four waves or one of eight
     // on a CU; three of four where 168 registers do (4096 tokens of fp16, HD 128: tiles of 64 and
     // two waves 171 us, of 32 and three 164)
