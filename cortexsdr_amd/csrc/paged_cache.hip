@@ -281,6 +281,48 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
     const uint8_t* hp =
         (is_v ? pv.v : pv.k) + csdr::head_offset<Q4>(pv, HD, max(page, 0), head);
     XT* dst = static_cast<XT*>(is_v ? a.v : a.k) + (long long)head * HD + 2 * li;
+    // the block's data first, all of it (page 0 stands in for none)
+    float x[8][2];
+    if constexpr (!Q4) {
+        const _Float16* h = reinterpret_cast<const _Float16*>(hp);
+        if (!is_v) {
+            h2 w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                w[i] = *reinterpret_cast<const h2*>(h + (slot0 + i) * HD + 2 * li);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i][0] = (float)w[i][0];
+                x[i][1] = (float)w[i][1];
+            }
+        } else {
+            const h8* d = reinterpret_cast<const h8*>(h + ((slot0 >> 3) * HD + 2 * li) * 8);
+            const h8 v0 = d[0], v1 = d[1];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i][0] = (float)v0[i];
+                x[i][1] = (float)v1[i];
+            }
+        }
+    } else {
+        const int g = 2 * li / kGroup;
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(hp);
+        const h8 sc = *reinterpret_cast<const h8*>(hp + csdr::scale_offset(HD, ps, g, slot0));
+        const h8 mn = *reinterpret_cast<const h8*>(hp + csdr::min_offset(HD, ps, g, slot0));
+        uint32_t w[8];  // K: the word of each position; V: the words of the lane's two dims
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = words[is_v ? csdr::v_word<HD>(slot0, 2 * li + (i & 1))
+                              : csdr::k_word<HD>(slot0 + i, 2 * li)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t code = is_v ? w[u] >> csdr::code_shift(i)
+                                           : w[i] >> (4 * (li & 3) + 16 * u);
+                x[i][u] = fmaf((float)sc[i], (float)(code & 15u), (float)mn[i]);
+            }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int p = base + i;
@@ -288,8 +330,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
         const long long row = (long long)r.first + (p - r.p0);
         Pair<XT> w{};
         if (page >= 0) {
-            w.a = (XT)csdr::cache_value<HD, Q4>(hp, is_v, ps, slot0 + i, 2 * li);
-            w.b = (XT)csdr::cache_value<HD, Q4>(hp, is_v, ps, slot0 + i, 2 * li + 1);
+            w.a = (XT)x[i][0];
+            w.b = (XT)x[i][1];
         }
         *reinterpret_cast<Pair<XT>*>(dst + row * ((long long)pv.hkv * HD)) = w;
     }
