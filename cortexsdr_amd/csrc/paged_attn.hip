@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -1221,12 +1222,17 @@ void launch_prompt(const AttnArgs& a, const Splits& s, hipStream_t st) {
     using Config = PromptConfig<HD, Q4, XT, SMALL>;
     using Shape = typename Config::Shape;
     constexpr auto kernel = &prompt_kernel<HD, Q4, XT, OPTS, Config::NQ, Config::NW>;
-    static const bool raised = [] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
-        return true;
-    }();
-    (void)raised;
+    if constexpr (Shape::kLds > 65536) {  // beyond the default: allowed once per device
+        static std::atomic<uint64_t> allowed{0};
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, Shape::kLds);
+            allowed.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
     const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
     const int blocks = (cols + Shape::kColumns - 1) / Shape::kColumns;
     const dim3 grid((unsigned)(a.pv.n_seqs * a.pv.hkv * blocks), s.n);

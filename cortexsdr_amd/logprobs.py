@@ -8,7 +8,7 @@ import typing
 
 from . import _lib
 from .hsdr import _check, _stream_ptr, _torch
-from .paged import _dtype, _on_device
+from .paged import _dtype, _empty, _on_device
 
 
 class TokenLogprobs(typing.NamedTuple):
@@ -21,7 +21,8 @@ class TokenLogprobs(typing.NamedTuple):
 def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0, workspace=None,
                    stream=None) -> TokenLogprobs:
     """logits: (rows, n) float32 or float16 on the device, rows any stride apart; tokens: (rows,)
-    int32, negative for none. With `stream` the call runs there, ordered by the caller."""
+    int32, negative for none. With `stream` the call runs and allocates there, ordered by the
+    caller."""
     torch = _torch()
     lib = _lib.load()
     dt = _dtype(logits)
@@ -37,12 +38,12 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
     dev = logits.device
     if workspace is None:
         need = lib.csdr_token_logprobs_workspace_bytes(rows, n, top_n)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    lp, entropy = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+        workspace = _empty(torch, need, torch.uint8, dev, stream) if need else None
+    lp, entropy = _empty(torch, (2, rows), torch.float32, dev, stream).unbind(0)
     ids = top = None
     if top_n > 0:
-        ids = torch.empty((rows, top_n), dtype=torch.int32, device=dev)
-        top = torch.empty((rows, top_n), dtype=torch.float32, device=dev)
+        ids = _empty(torch, (rows, top_n), torch.int32, dev, stream)
+        top = _empty(torch, (rows, top_n), torch.float32, dev, stream)
     if tokens is None:
         lp = None
     _check(lib.csdr_token_logprobs(
@@ -53,8 +54,4 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         workspace.data_ptr() if workspace is not None else None,
         workspace.numel() * workspace.element_size() if workspace is not None else 0,
         _stream_ptr(stream)))
-    if stream is not None:
-        for t in (entropy, ids, top, workspace):
-            if t is not None:
-                t.record_stream(stream)
     return TokenLogprobs(lp, entropy, ids, top)

@@ -11,10 +11,10 @@ the caller's scheduler fills and may change between calls):
     q = batch.append(q, k, v, theta=1e6)      # rotated queries; keys and values into the pages
     out = batch.attend(q)
 
-Outputs are allocated by torch on the current device; with `stream`, a call runs on that stream
-and the caller orders it against the streams its tensors come from. Workspaces are allocated per
-call (inside a graph capture, from that graph's pool), so calls on different streams and captured
-graphs share none unless the caller passes one to both.
+With `stream`, a call runs on that stream, its outputs and workspace are allocated there, and the
+caller orders it against the streams its tensors come from. Workspaces are allocated per call
+(inside a graph capture, from that graph's pool), so calls on different streams and captured graphs
+share none unless the caller passes one to both.
 """
 from __future__ import annotations
 
@@ -42,6 +42,14 @@ def _on_device(torch, what: str, *ts) -> None:
     for t in ts:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what} must be on the current device")
+
+
+def _empty(torch, shape, dtype, device, stream):
+    """A tensor of the stream that will write it (the current one if None)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _ints(torch, what: str, t, shape) -> None:
@@ -147,7 +155,7 @@ class PagedBatch:
             if q.shape[0] != n or q.dtype != k.dtype:
                 raise ValueError("q and k must have the same tokens and type")
             if q_out is None:
-                q_out = torch.empty((n, nq, hd), dtype=q.dtype, device=q.device)
+                q_out = _empty(torch, (n, nq, hd), q.dtype, q.device, stream)
             elif q_out.dtype != q.dtype or q_out.numel() != n * nq * hd or \
                     not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous (tokens, heads, head_dim) of q's type")
@@ -159,8 +167,6 @@ class PagedBatch:
             self._ref, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), dt, n,
             starts, mq, nq, qs, ks, vs, theta, q_out.data_ptr() if q_out is not None else None,
             _stream_ptr(stream)))
-        if stream is not None and q_out is not None:
-            q_out.record_stream(stream)
         return q_out
 
     def attend(self, q, q_start=None, max_q=None, max_len: int = 0, scale: float = 0.0,
@@ -175,7 +181,7 @@ class PagedBatch:
         n = q.shape[0]
         nq, qs = self._heads("q", q)
         if out is None:
-            out = torch.empty((n, nq, self.cache.head_dim), dtype=q.dtype, device=q.device)
+            out = _empty(torch, (n, nq, self.cache.head_dim), q.dtype, q.device, stream)
         elif out.dtype != q.dtype or out.numel() != n * nq * self.cache.head_dim or \
                 not out.is_contiguous():
             raise ValueError("out must be contiguous (tokens, heads, head_dim) of q's type")
@@ -200,16 +206,12 @@ class PagedBatch:
                 need = self._need[key] = self._lib.csdr_paged_attn_workspace_bytes(
                     self._ref, n, starts, mq, nq, max_len)
             if need:
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-                if stream is not None:
-                    workspace.record_stream(stream)
+                workspace = _empty(torch, need, torch.uint8, q.device, stream)
         _check(self._lib.csdr_paged_attn(
             self._ref, q.data_ptr(), dt, n, starts, mq, nq, qs, max_len, scale, opt,
             out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
             workspace.numel() * workspace.element_size() if workspace is not None else 0,
             _stream_ptr(stream)))
-        if stream is not None:
-            out.record_stream(stream)
         return out
 
     def workspace_bytes(self, n_tokens: int, n_heads: int, q_start=None, max_q=None,
@@ -226,14 +228,11 @@ class PagedBatch:
         if dtype not in ("f32", "f16"):
             raise ValueError("dtype must be 'f32' or 'f16'")
         c = self.cache
-        k, v = (torch.empty((n_tokens, c.n_kv_heads, c.head_dim), device=c.k.device,
-                            dtype=torch.float16 if dtype == "f16" else torch.float32)
+        k, v = (_empty(torch, (n_tokens, c.n_kv_heads, c.head_dim),
+                       torch.float16 if dtype == "f16" else torch.float32, c.k.device, stream)
                 for _ in range(2))
         starts, mq = self._starts(torch, q_start, max_q)
         _on_device(torch, "tensors", k, q_start)
         _check(self._lib.csdr_paged_read(self._ref, n_tokens, starts, mq, k.data_ptr(),
                                          v.data_ptr(), int(dtype == "f16"), _stream_ptr(stream)))
-        if stream is not None:
-            k.record_stream(stream)
-            v.record_stream(stream)
         return k, v

@@ -624,7 +624,9 @@ typedef struct csdr_attn_options {
  * 1/sqrt(head_dim). A row that sees nothing is zero. What a token does not see has no influence on
  * it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
  * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
- * right, with less parallelism).
+ * right, with less parallelism). One kernel serves a whole call, chosen by the most (token, query
+ * head) pairs of a sequence and KV head: up to 64 take the form for single tokens, so sequences
+ * with a token each are better off in a call of their own than beside a prompt.
  *
  * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
  * CSDR_F16: weights rounded to fp16 once, fp32 sums. workspace:

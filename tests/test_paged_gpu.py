@@ -324,15 +324,65 @@ def test_attend_tokens_options_long(gpu, kv, x, o):
     assert rel_l2(got, s.expect(qd.cpu().numpy(), [40], **e)) <= tol(x)
 
 
-def test_attend_uniform_tokens_and_stride(gpu):
-    """As many tokens of each sequence, without q_start; queries as slices of wider rows."""
-    s = Setup(gpu, [50, 50], HEADS["three"], "f16", seed=10)
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("tokens", [1, 11, 40])
+def test_attend_uniform_tokens_and_stride(gpu, kv, x, tokens):
+    """As many tokens of each sequence, without q_start; queries as slices of wider rows, at odd
+    offsets, and the output at one too."""
+    s = Setup(gpu, [80, 80], HEADS["three"], kv, x, seed=10)
     s.append([20, 9], with_q=False)
-    qd, _ = s.append([11, 11])
-    wide = s.gpu.zeros((22, 6 * 64 + 5), device="cuda")
-    wide[:, 5:] = qd.reshape(22, -1)
-    got = s.batch.attend(wide[:, 5:]).cpu().numpy()
-    assert rel_l2(got, s.expect(qd.cpu().numpy(), [11, 11])) <= TOL32
+    qd, _ = s.append([tokens, tokens])
+    n = 2 * tokens
+    wide = s.gpu.zeros((n, 6 * 64 + 5), device="cuda", dtype=qd.dtype)
+    wide[:, 5:] = qd.reshape(n, -1)
+    room = s.gpu.full((n * 6 * 64 + 2,), 7.0, device="cuda", dtype=qd.dtype)
+    out = room[1:-1].view(n, 6, 64)
+    s.batch.attend(wide[:, 5:], out=out)
+    assert room[0] == 7.0 and room[-1] == 7.0
+    assert rel_l2(out.cpu().numpy(), s.expect(qd.cpu().numpy(), [tokens] * 2)) <= tol(x)
+
+
+def test_python_refusals(gpu):
+    """What the Python entry points refuse before a launch."""
+    from cortexsdr_amd import _lib
+    from cortexsdr_amd.logprobs import token_logprobs
+    from cortexsdr_amd.paged import PagedCache
+
+    s = Setup(gpu, [16], HEADS["three"], "f16", seed=22)
+    s.append([4], with_q=False)
+    b, q = s.batch, gpu.zeros(1, 6, 64, device="cuda")
+    k = gpu.zeros(1, 2, 64, device="cuda")
+    two = gpu.zeros(2, dtype=gpu.int32, device="cuda")
+    for call in (
+        lambda: b.attend(q.double()), lambda: b.attend(q.cpu()), lambda: b.attend(q[:, :, ::2]),
+        lambda: b.attend(gpu.zeros(1, 6 * 64 + 1, device="cuda")),
+        lambda: b.attend(q.expand(3, 6, 64), q_start=two, max_q=3),  # rows that overlap
+        lambda: b.attend(q, q_start=two), lambda: b.attend(q, q_start=two.long(), max_q=1),
+        lambda: b.attend(q, slopes=gpu.zeros(5, device="cuda")),
+        lambda: b.attend(q, prefix=two), lambda: b.attend(q, out=q.half()),
+        lambda: b.append(q, k, k.half()), lambda: b.append(q, k[:, :1], k),
+        lambda: b.append(None, k, k, q_out=q), lambda: b.append(q, k, k, q_out=q[:, :3]),
+        lambda: b.read(1, dtype="bf16"),
+        lambda: PagedCache(4, 24, 2, 64), lambda: PagedCache(0, 16, 2, 64),
+        lambda: PagedCache(4, 16, 2, 64, "f32"), lambda: PagedCache(4, 16, 2, 64, k=q, v=q),
+        lambda: s.cache.batch(two, two), lambda: s.cache.batch(two.view(1, 2).long(), two[:1]),
+        lambda: s.cache.batch(two.view(2, 1), two[:1]),
+        lambda: token_logprobs(q), lambda: token_logprobs(gpu.zeros(4, 8, device="cuda")[:, ::2]),
+        lambda: token_logprobs(gpu.zeros(1, 8, device="cuda").expand(4, 8)),
+        lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), two),
+    ):
+        with pytest.raises(ValueError):
+            call()
+    for call in (
+        lambda: b.attend(gpu.zeros(1, 5, 64, device="cuda")),  # 5 heads over 2
+        lambda: b.attend(q, window=-1), lambda: b.attend(q, softcap=float("nan")),
+        lambda: b.attend(q, workspace=gpu.zeros(4, device="cuda")),
+        lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), top_n=65),
+        lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), workspace=q[0, 0, :4]),
+    ):
+        with pytest.raises(_lib.CsdrError):
+            call()
 
 
 # ---------------------------------------------------------------- what is not seen
