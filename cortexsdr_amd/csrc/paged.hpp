@@ -61,12 +61,20 @@ __host__ __device__ __forceinline__ SeqRows seq_rows(const PagedView& pv, int b)
     return r;
 }
 
-// The page of position p of sequence b, or -1 where the table has none (positions past its end,
+// The page of position p of sequence b (SCALAR: the same in the whole wave, looked up through the
+// scalar cache also behind barriers, which a constant table allows), or -1 where the table has none (positions past its end,
 // ids outside [0, n_pages)).
+template <bool SCALAR = false>
 __host__ __device__ __forceinline__ int page_of(const PagedView& pv, int b, int p) {
     const int i = p >> pv.shift;
     if (p < 0 || i >= pv.stride) return -1;
-    const int pg = pv.table[(size_t)b * pv.stride + i];
+    const size_t at = (size_t)b * pv.stride + i;
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int pg = SCALAR ? ((const __attribute__((address_space(4))) int32_t*)pv.table)[at]
+                          : pv.table[at];
+#else
+    const int pg = pv.table[at];
+#endif
     return (unsigned)pg < (unsigned)pv.n_pages ? pg : -1;
 }
 

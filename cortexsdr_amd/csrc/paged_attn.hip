@@ -885,11 +885,12 @@ prompt_kernel(AttnArgs a, Splits sp) {
     auto buffer = [&](int buf, int v, int plane) {
         return lds + ((buf * 2 + v) * PLANES + plane) * PLANE;
     };
-    // page ids of a tile's granules of 16 positions (uniform)
+    // page ids of a tile's granules of 16 positions (uniform; through the scalar cache 172 -> 168 us
+    // for 4096 tokens on fp16 pages, but 600 -> 644 where 4-bit pages are unpacked between)
     auto pages_at = [&](int tb, int* pg) {
 #pragma unroll
         for (int i = 0; i < GR; ++i)
-            pg[i] = i > 0 && ps >= TP ? pg[0] : csdr::page_of(pv, b, tb + 16 * i);
+            pg[i] = i > 0 && ps >= TP ? pg[0] : csdr::page_of<!Q4>(pv, b, tb + 16 * i);
     };
 
     // 4 bits: the words this thread turns into values, and their groups' scales and minima
