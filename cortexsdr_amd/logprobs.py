@@ -7,8 +7,8 @@ from __future__ import annotations
 import typing
 
 from . import _lib
-from .hsdr import _check, _stream_ptr, _torch
-from .paged import _dtype, _empty, _on_device
+from .hsdr import _check, _torch
+from .paged import _dtype, _empty, _on_device, _stream_of
 
 
 class TokenLogprobs(typing.NamedTuple):
@@ -34,7 +34,7 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
     if tokens is not None and (tokens.dtype != torch.int32 or tuple(tokens.shape) != (rows,) or
                                not tokens.is_contiguous()):
         raise ValueError("tokens must be a contiguous int32 tensor, one per row")
-    _on_device(torch, "tensors", logits, tokens, workspace)
+    index = _on_device(torch, "tensors", logits, tokens, workspace)
     dev = logits.device
     if workspace is None:
         need = lib.csdr_token_logprobs_workspace_bytes(rows, n, top_n)
@@ -52,6 +52,5 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         lp.data_ptr() if lp is not None else None, entropy.data_ptr(), top_n,
         ids.data_ptr() if top_n > 0 else None, top.data_ptr() if top_n > 0 else None,
         workspace.data_ptr() if workspace is not None else None,
-        workspace.numel() * workspace.element_size() if workspace is not None else 0,
-        _stream_ptr(stream)))
+        workspace.nbytes if workspace is not None else 0, _stream_of(torch, index, stream)))
     return TokenLogprobs(lp, entropy, ids, top)

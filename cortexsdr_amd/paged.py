@@ -21,7 +21,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from .hsdr import _check, _stream_ptr, _torch
+from .hsdr import _check, _torch
 
 KV_DTYPES = {"f16": 1, "q4": 2}
 _DTYPES = {}
@@ -37,11 +37,27 @@ def _dtype(t) -> int:
     return dt
 
 
-def _on_device(torch, what: str, *ts) -> None:
+_raw = None  # torch's raw accessor of a device's current stream, where it has one
+
+
+def _on_device(torch, what: str, *ts) -> int:
+    """Checks that the tensors are on the current device; its index."""
     dev = torch.cuda.current_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"{what} must be on the current device")
+    return dev
+
+
+def _stream_of(torch, dev: int, stream) -> int:
+    """The hipStream_t of `stream`, or of the device's current stream."""
+    global _raw
+    if stream is None:
+        if _raw is None:
+            _raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+                (lambda d: int(torch.cuda.current_stream(d).cuda_stream))
+        return _raw(dev)
+    return int(stream.cuda_stream)
 
 
 def _empty(torch, shape, dtype, device, stream):
@@ -109,6 +125,7 @@ class PagedBatch:
                                 int(table.shape[1]))
         self._ref = C.byref(self._kv)
         self._lib = _lib.load()
+        self._append, self._attn = self._lib.csdr_paged_append, self._lib.csdr_paged_attn
         self._need = {}  # workspace bytes by the call's sizes
 
     def _starts(self, torch, q_start, max_q):
@@ -162,11 +179,13 @@ class PagedBatch:
         elif q_out is not None:
             raise ValueError("q_out without q")
         starts, mq = self._starts(torch, q_start, max_q)
-        _on_device(torch, "tensors", q, k, v, q_out, q_start)
-        _check(self._lib.csdr_paged_append(
+        dev = _on_device(torch, "tensors", q, k, v, q_out, q_start)
+        rc = self._append(
             self._ref, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), dt, n,
             starts, mq, nq, qs, ks, vs, theta, q_out.data_ptr() if q_out is not None else None,
-            _stream_ptr(stream)))
+            _stream_of(torch, dev, stream))
+        if rc:
+            _check(rc)
         return q_out
 
     def attend(self, q, q_start=None, max_q=None, max_len: int = 0, scale: float = 0.0,
@@ -196,7 +215,7 @@ class PagedBatch:
                                            slopes.data_ptr() if slopes is not None else None,
                                            prefix.data_ptr() if prefix is not None else None))
         starts, mq = self._starts(torch, q_start, max_q)
-        _on_device(torch, "tensors", q, out, q_start, slopes, prefix, workspace)
+        dev = _on_device(torch, "tensors", q, out, q_start, slopes, prefix, workspace)
         if workspace is None:
             key = (n, starts is None, mq, nq, max_len)
             need = self._need.get(key)
@@ -207,11 +226,12 @@ class PagedBatch:
                     self._ref, n, starts, mq, nq, max_len)
             if need:
                 workspace = _empty(torch, need, torch.uint8, q.device, stream)
-        _check(self._lib.csdr_paged_attn(
+        rc = self._attn(
             self._ref, q.data_ptr(), dt, n, starts, mq, nq, qs, max_len, scale, opt,
             out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
-            workspace.numel() * workspace.element_size() if workspace is not None else 0,
-            _stream_ptr(stream)))
+            workspace.nbytes if workspace is not None else 0, _stream_of(torch, dev, stream))
+        if rc:
+            _check(rc)
         return out
 
     def workspace_bytes(self, n_tokens: int, n_heads: int, q_start=None, max_q=None,
@@ -228,11 +248,12 @@ class PagedBatch:
         if dtype not in ("f32", "f16"):
             raise ValueError("dtype must be 'f32' or 'f16'")
         c = self.cache
-        k, v = (_empty(torch, (n_tokens, c.n_kv_heads, c.head_dim),
-                       torch.float16 if dtype == "f16" else torch.float32, c.k.device, stream)
-                for _ in range(2))
+        k, v = _empty(torch, (2, n_tokens, c.n_kv_heads, c.head_dim),
+                      torch.float16 if dtype == "f16" else torch.float32, c.k.device,
+                      stream).unbind(0)
         starts, mq = self._starts(torch, q_start, max_q)
-        _on_device(torch, "tensors", k, q_start)
+        dev = _on_device(torch, "tensors", k, q_start)
         _check(self._lib.csdr_paged_read(self._ref, n_tokens, starts, mq, k.data_ptr(),
-                                         v.data_ptr(), int(dtype == "f16"), _stream_ptr(stream)))
+                                         v.data_ptr(), int(dtype == "f16"),
+                                         _stream_of(torch, dev, stream)))
         return k, v
