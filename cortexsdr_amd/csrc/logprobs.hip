@@ -35,6 +35,7 @@ constexpr int kPer = 32;               // values per lane and round
 constexpr int kRound = 64 * kPer;
 constexpr int kList = 192;             // entries of a wave's list: room for 64 more at 128
 constexpr int kMaxSegments = 128;
+constexpr int kListEntries = 7168;     // of a row's segments' lists in all: 56 KB
 constexpr float kLog2e = 1.44269504088896341f;
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -429,10 +430,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
     }
 }
 
-// Segments of a row: whole rounds, about 8192 waves in all.
+// Segments of a row: whole rounds, about 8192 waves in all, as many as leave join_kernel's lists
+// and its few KB beside them in the 64 KB of LDS that every launch may have.
 void set_segments(Args& a) {
     const int all = (int)(((long long)a.n + kRound - 1) / kRound);
-    const int want = std::min(std::max(8192 / a.rows, 1), kMaxSegments);
+    const int most = std::min(kMaxSegments, kListEntries / std::max(a.top_n, 1));
+    const int want = std::min(std::max(8192 / a.rows, 1), most);
     a.rounds = (all + want - 1) / want;
     a.segments = (all + a.rounds - 1) / a.rounds;
 }

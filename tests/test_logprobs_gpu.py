@@ -181,3 +181,11 @@ def test_two_streams(gpu):
     for w, os_ in zip(want, outs):
         for o in os_:
             assert gpu.equal(o.top_ids, w.top_ids) and gpu.equal(o.entropy, w.entropy)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("top_n", [56, 57, 64])
+def test_most_segments_and_places(gpu, dtype, top_n):
+    """The longest rows with the most places: the lists of a row's segments at their largest."""
+    x = np.random.default_rng(top_n).normal(size=(2, 300000)).astype(dtype)
+    check(gpu, x, [0, 299999], top_n)
