@@ -20,6 +20,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "common.hpp"
@@ -484,6 +485,10 @@ CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
         return set_error(CSDR_E_INVALID, "token_logprobs: the row stride is below n");
     if (!(temperature < INFINITY) || temperature == -INFINITY)
         return set_error(CSDR_E_INVALID, "token_logprobs: the temperature is not finite");
+    if (temperature > 0.0f && temperature < FLT_MIN)  // (its reciprocal may be infinite)
+        return set_error(CSDR_E_INVALID, "token_logprobs: the temperature is a denormal number");
+    if (rows > (1 << 24) - 1)  // (workgroups of a launch: 2^32 threads)
+        return set_error(CSDR_E_INVALID, "token_logprobs: more than 2^24 - 1 rows");
     Args a{};
     a.x = logits;
     a.rows = rows;

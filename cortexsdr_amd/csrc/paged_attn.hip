@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -1291,6 +1292,8 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     AttnArgs a{};
     if (int rc = csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &a.pv)) return rc;
     if (!q || !out) return set_error(CSDR_E_INVALID, "paged_attn: a pointer is NULL");
+    if (q == out)  // (rows with values that are not finite are read again)
+        return set_error(CSDR_E_INVALID, "paged_attn: out must not be q");
     if (dtype != CSDR_F32 && dtype != CSDR_F16)
         return set_error(CSDR_E_INVALID, "paged_attn: dtype must be CSDR_F32 or CSDR_F16");
     if (Hq <= 0 || Hq > 65535 || Hq % kv->n_kv_heads)
@@ -1304,7 +1307,10 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
         return set_error(CSDR_E_INVALID, "paged_attn: the scale is not finite");
     a.scale = scale == 0.0f ? 1.0f / std::sqrt((float)hd) : scale;
     if (options) {
-        if (!(options->softcap >= 0.0f && options->softcap < INFINITY) || options->window < 0)
+        // (a denormal cap has no finite reciprocal)
+        if (!(options->softcap == 0.0f ||
+              (options->softcap >= FLT_MIN && options->softcap < INFINITY)) ||
+            options->window < 0)
             return set_error(CSDR_E_INVALID, "paged_attn: bad options");
         a.cap = options->softcap;
         a.inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
@@ -1315,11 +1321,13 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.q = q;
     a.out = out;
     a.hq = Hq;
-    const long long cols = ((long long)a.pv.max_q * (Hq / kv->n_kv_heads) + kCols - 1) / kCols;
-    if ((long long)kv->n_seqs * std::max((long long)a.pv.max_q, kv->n_kv_heads * cols) >
-        0x7fffffffLL)
-        return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
     Splits s = splits_of(a.pv, Hq, max_len, a.window);
+    // fewer than 2^32 threads a launch: workgroups of at most 256 (prompt_kernel: two threads a
+    // column, except where it has few), join_kernel's only where there is one
+    const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);
+    if ((long long)kv->n_seqs * kv->n_kv_heads * ((cols + 127) / 128) >= 1LL << 24 ||
+        (!one_launch(a.pv, Hq, s) && (long long)kv->n_seqs * a.pv.max_q >= 1LL << 24))
+        return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
     const size_t need = workspace_of(a.pv, Hq, hd, s);
     if (need && (!workspace || workspace_bytes < need ||
                  reinterpret_cast<uintptr_t>(workspace) % 16))

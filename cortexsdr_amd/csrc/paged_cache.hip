@@ -31,6 +31,7 @@ using csdr::set_error;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr long long kMaxBlocks = (1LL << 32) / kThreads - 1;  // a launch has fewer than 2^32 threads
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -418,6 +419,8 @@ CSDR_API int csdr_paged_append(const csdr_paged_kv* kv, const void* q, const voi
         return set_error(CSDR_E_INVALID, "paged_append: dtype must be CSDR_F32 or CSDR_F16");
     if (q && (Hq <= 0 || Hq > 65535 || Hq % kv->n_kv_heads))
         return set_error(CSDR_E_INVALID, "paged_append: bad number of heads");
+    if (q && q_out == q && q_stride != 0 && q_stride != (int64_t)Hq * kv->head_dim)
+        return set_error(CSDR_E_INVALID, "paged_append: q in place must be packed");
     if (!(theta >= 0.0f) || theta == INFINITY)
         return set_error(CSDR_E_INVALID, "paged_append: theta must be positive, or 0 for none");
     const int hd = kv->head_dim;
@@ -437,7 +440,7 @@ CSDR_API int csdr_paged_append(const csdr_paged_kv* kv, const void* q, const voi
     a.log2_theta = a.rotate ? std::log2((double)theta) : 0.0;
     const int upw = kWaves * (128 / hd), units = a.hq + 2 * kv->n_kv_heads;
     const long long gx = (long long)kv->n_seqs * a.nblk;
-    if (gx > 0x7fffffffLL) return set_error(CSDR_E_INVALID, "paged_append: too many tokens");
+    if (gx > kMaxBlocks) return set_error(CSDR_E_INVALID, "paged_append: too many tokens");
     const dim3 grid((unsigned)gx, (units + upw - 1) / upw);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const bool q4 = kv->kv_dtype == CSDR_Q4;
@@ -464,7 +467,7 @@ CSDR_API int csdr_paged_read(const csdr_paged_kv* kv, int n_tokens, const int32_
     a.nblk = blocks_of(a.pv.max_q);
     const int hd = kv->head_dim, upw = kWaves * (128 / hd);
     const long long gx = (long long)kv->n_seqs * a.nblk;
-    if (gx > 0x7fffffffLL) return set_error(CSDR_E_INVALID, "paged_read: too many tokens");
+    if (gx > kMaxBlocks) return set_error(CSDR_E_INVALID, "paged_read: too many tokens");
     const dim3 grid((unsigned)gx, (2 * kv->n_kv_heads + upw - 1) / upw);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const bool q4 = kv->kv_dtype == CSDR_Q4;

@@ -8,7 +8,7 @@ import typing
 
 from . import _lib
 from .hsdr import _check, _torch
-from .paged import _dtype, _empty, _on_device, _stream_of
+from .paged import _bytes, _dtype, _empty, _on_device, _stream_of
 
 
 class TokenLogprobs(typing.NamedTuple):
@@ -52,5 +52,5 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         lp.data_ptr() if lp is not None else None, entropy.data_ptr(), top_n,
         ids.data_ptr() if top_n > 0 else None, top.data_ptr() if top_n > 0 else None,
         workspace.data_ptr() if workspace is not None else None,
-        workspace.nbytes if workspace is not None else 0, _stream_of(torch, index, stream)))
+        _bytes(workspace) if workspace is not None else 0, _stream_of(torch, index, stream)))
     return TokenLogprobs(lp, entropy, ids, top)

@@ -68,6 +68,16 @@ def _empty(torch, shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _bytes(workspace) -> int:
+    """What a caller's workspace holds: all of it has to be there (an expanded tensor's is not)."""
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.nbytes
+
+
 def _ints(torch, what: str, t, shape) -> None:
     if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape}")
@@ -134,7 +144,7 @@ class PagedBatch:
         _ints(torch, "q_start", q_start, (self.n_seqs + 1,))
         if max_q is None:
             raise ValueError("q_start needs max_q, the most tokens of one sequence")
-        return q_start.data_ptr(), int(max_q)
+        return q_start.data_ptr(), min(int(max_q), _INT_MAX)
 
     def _heads(self, what: str, t, n_heads=None):
         """The token stride of (tokens, heads, head_dim) or (tokens, heads * head_dim)."""
@@ -211,10 +221,11 @@ class PagedBatch:
                 raise ValueError("slopes must be a contiguous float32 tensor, one per head")
             if prefix is not None:
                 _ints(torch, "prefix", prefix, (self.n_seqs,))
-            opt = C.byref(_lib.AttnOptions(softcap, window,
+            opt = C.byref(_lib.AttnOptions(softcap, min(window, _INT_MAX),
                                            slopes.data_ptr() if slopes is not None else None,
                                            prefix.data_ptr() if prefix is not None else None))
         starts, mq = self._starts(torch, q_start, max_q)
+        max_len = min(max_len, _INT_MAX)
         dev = _on_device(torch, "tensors", q, out, q_start, slopes, prefix, workspace)
         if workspace is None:
             key = (n, starts is None, mq, nq, max_len)
@@ -229,7 +240,7 @@ class PagedBatch:
         rc = self._attn(
             self._ref, q.data_ptr(), dt, n, starts, mq, nq, qs, max_len, scale, opt,
             out.data_ptr(), workspace.data_ptr() if workspace is not None else None,
-            workspace.nbytes if workspace is not None else 0, _stream_of(torch, dev, stream))
+            _bytes(workspace) if workspace is not None else 0, _stream_of(torch, dev, stream))
         if rc:
             _check(rc)
         return out
@@ -239,7 +250,7 @@ class PagedBatch:
         """Bytes of attend's workspace, for callers that keep one."""
         starts, mq = self._starts(_torch(), q_start, max_q)
         return int(self._lib.csdr_paged_attn_workspace_bytes(self._ref, n_tokens, starts, mq,
-                                                            n_heads, max_len))
+                                                            n_heads, min(max_len, _INT_MAX)))
 
     def read(self, n_tokens: int, q_start=None, max_q=None, dtype: str = "f32", stream=None):
         """The cached keys and values of the sequences' last n_tokens rows (laid out as append's

@@ -610,7 +610,7 @@ CSDR_API int csdr_paged_read(const csdr_paged_kv* kv, int n_tokens, const int32_
 /* How scores are formed and which positions are seen. All zero (or NULL for the struct): causal
  * softmax(q.K^T * scale). */
 typedef struct csdr_attn_options {
-    float softcap;         /* > 0: score = softcap * tanh(score / softcap) */
+    float softcap;         /* > 0, not denormal: score = softcap * tanh(score / softcap) */
     int window;            /* > 0: of the positions up to its own, a token sees the last `window` */
     const float* slopes;   /* Hq floats (device), or NULL: score -= slope * |distance| */
     const int32_t* prefix; /* n_seqs ints (device), or NULL: every token of sequence b sees the
@@ -621,7 +621,7 @@ typedef struct csdr_attn_options {
 /* out (n_tokens x Hq x head_dim, of dtype) = softmax attention of the tokens (rotated queries q,
  * as csdr_paged_append writes them) to the positions of their sequences that they see, after the
  * call's tokens were appended; GQA as repeat_kv_heads (cortex_sdk.cpp:1453-1478); scale 0 =
- * 1/sqrt(head_dim). A row that sees nothing is zero. What a token does not see has no influence on
+ * 1/sqrt(head_dim); out must not overlap q. A row that sees nothing is zero. What a token does not see has no influence on
  * it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
  * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
  * right, with less parallelism). One kernel serves a whole call, chosen by the most (token, query
@@ -645,7 +645,7 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
  * ==================================================================== */
 
 /* For each of `rows` rows of n logits (dtype CSDR_F32 or CSDR_F16, row_stride elements apart, 0 =
- * n), y = logits / temperature (temperature <= 0: 1, as select_best_from_logits,
+ * n), y = logits / temperature (temperature <= 0: 1, a denormal one is refused, as select_best_from_logits,
  * cortex_sdk.cpp:1005-1030): logprobs[r] = y[tokens[r]] - log sum exp y (tokens NULL: not
  * computed; a negative token: 0; one >= n: NaN), entropy[r] = -sum p log p in nats (may be NULL),
  * and the top_n (0..64) largest y, largest first and lower ids first among equals:

@@ -371,18 +371,31 @@ def test_python_refusals(gpu):
         lambda: token_logprobs(q), lambda: token_logprobs(gpu.zeros(4, 8, device="cuda")[:, ::2]),
         lambda: token_logprobs(gpu.zeros(1, 8, device="cuda").expand(4, 8)),
         lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), two),
+        lambda: b.attend(q, workspace=two[:1].expand(1 << 20)),
+        lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), workspace=two[:1].expand(1 << 20)),
     ):
         with pytest.raises(ValueError):
             call()
     for call in (
         lambda: b.attend(gpu.zeros(1, 5, 64, device="cuda")),  # 5 heads over 2
         lambda: b.attend(q, window=-1), lambda: b.attend(q, softcap=float("nan")),
-        lambda: b.attend(q, workspace=gpu.zeros(4, device="cuda")),
+        lambda: b.attend(q, workspace=gpu.zeros(4, device="cuda")), lambda: b.attend(q, out=q),
         lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), top_n=65),
         lambda: token_logprobs(gpu.zeros(4, 8, device="cuda"), workspace=q[0, 0, :4]),
     ):
         with pytest.raises(_lib.CsdrError):
             call()
+
+
+def test_bounds_past_an_int(gpu):
+    """A window, a length bound and a most of tokens past 2^31 bound nothing."""
+    s = Setup(gpu, [300], HEADS["three"], "f16", seed=23)
+    qd, _ = s.append([300])
+    want = s.batch.attend(qd)
+    for far in (2 ** 31, 2 ** 32 + 3):
+        assert gpu.equal(s.batch.attend(qd, window=far), want)
+        assert gpu.equal(s.batch.attend(qd, max_len=far), want)
+        assert gpu.equal(s.batch.attend(qd, q_start=s.starts([300]), max_q=far), want)
 
 
 # ---------------------------------------------------------------- what is not seen

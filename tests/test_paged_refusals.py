@@ -13,6 +13,7 @@ from cortexsdr_amd import _lib
 
 INVALID, WORKSPACE, UNSUPPORTED = -1, -5, -6
 P = 4096  # an aligned address that no refused call reads
+OUT = 2 * P
 
 
 def kv(**over):
@@ -46,7 +47,7 @@ def test_bad_cache(over, status):
     refused(lib.csdr_paged_append(kv(**over), P, P, P, 0, 2, None, 0, 4, 0, 0, 0, 1e4, P, None),
             status)
     refused(lib.csdr_paged_read(kv(**over), 2, None, 0, P, P, 0, None), status)
-    refused(lib.csdr_paged_attn(kv(**over), P, 0, 2, None, 0, 4, 0, 0, 0.0, None, P, P, 1 << 40,
+    refused(lib.csdr_paged_attn(kv(**over), P, 0, 2, None, 0, 4, 0, 0, 0.0, None, OUT, P, 1 << 40,
                                 None), status)
     assert lib.csdr_paged_attn_workspace_bytes(kv(**over), 2, None, 0, 4, 0) == 0
 
@@ -63,17 +64,17 @@ def test_bad_tokens(n, starts, mq):
     refused(lib.csdr_paged_append(kv(), P, P, P, 0, n, starts, mq, 4, 0, 0, 0, 1e4, P, None),
             INVALID)
     refused(lib.csdr_paged_read(kv(), n, starts, mq, P, P, 0, None), INVALID)
-    refused(lib.csdr_paged_attn(kv(), P, 0, n, starts, mq, 4, 0, 0, 0.0, None, P, P, 1 << 40,
+    refused(lib.csdr_paged_attn(kv(), P, 0, n, starts, mq, 4, 0, 0, 0.0, None, OUT, P, 1 << 40,
                                 None), INVALID)
 
 
 @pytest.mark.parametrize("over", [
     dict(k=None), dict(v=None), dict(q=None), dict(q_out=None), dict(dtype=2), dict(Hq=3),
     dict(Hq=0), dict(theta=-1.0), dict(theta=float("nan")), dict(theta=float("inf")),
-    dict(qs=255), dict(ks=127), dict(vs=-128),
+    dict(qs=255), dict(ks=127), dict(vs=-128), dict(q_out=P, qs=512),
 ])
 def test_bad_append(over):
-    a = dict(q=P, k=P, v=P, dtype=0, Hq=4, qs=0, ks=0, vs=0, theta=1e4, q_out=P)
+    a = dict(q=P, k=P, v=P, dtype=0, Hq=4, qs=0, ks=0, vs=0, theta=1e4, q_out=OUT)
     a.update(over)
     refused(_lib.load().csdr_paged_append(kv(), a["q"], a["k"], a["v"], a["dtype"], 2, None, 0,
                                           a["Hq"], a["qs"], a["ks"], a["vs"], a["theta"],
@@ -85,14 +86,28 @@ def test_bad_append(over):
     dict(max_len=-1), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(opt=_lib.AttnOptions(softcap=-1.0)), dict(opt=_lib.AttnOptions(softcap=float("inf"))),
     dict(opt=_lib.AttnOptions(softcap=float("nan"))), dict(opt=_lib.AttnOptions(window=-1)),
+    dict(opt=_lib.AttnOptions(softcap=1e-40)), dict(out=P),
 ])
 def test_bad_attn(over):
-    a = dict(q=P, out=P, dtype=0, Hq=4, qs=0, max_len=0, scale=0.0, opt=None)
+    a = dict(q=P, out=OUT, dtype=0, Hq=4, qs=0, max_len=0, scale=0.0, opt=None)
     a.update(over)
     opt = C.byref(a["opt"]) if a["opt"] is not None else None
     refused(_lib.load().csdr_paged_attn(kv(), a["q"], a["dtype"], 2, None, 0, a["Hq"], a["qs"],
                                         a["max_len"], a["scale"], opt, a["out"], P, 1 << 40,
                                         None), INVALID)
+
+
+def test_too_many_tokens():
+    """More workgroups than one launch may have."""
+    lib = _lib.load()
+    n, big = 1 << 27, kv(n_seqs=1 << 20)
+    refused(lib.csdr_paged_append(big, P, P, P, 0, n, P, n, 4, 0, 0, 0, 1e4, OUT, None), INVALID)
+    refused(lib.csdr_paged_read(big, n, P, n, P, OUT, 0, None), INVALID)
+    # prompts; steps, joined by one workgroup per token and head
+    refused(lib.csdr_paged_attn(big, P, 0, n, P, n, 4, 0, 0, 0.0, None, OUT, P, 1 << 60, None),
+            INVALID)
+    refused(lib.csdr_paged_attn(big, P, 0, n, P, 32, 4, 0, 0, 0.0, None, OUT, P, 1 << 60, None),
+            INVALID)
 
 
 def test_bad_read():
@@ -114,7 +129,7 @@ def test_page_bytes():
     (dict(dtype=2), INVALID), (dict(top=-1), UNSUPPORTED), (dict(top=65), UNSUPPORTED),
     (dict(tokens=None), INVALID), (dict(lp=None), INVALID), (dict(ids=None), INVALID),
     (dict(tl=None), INVALID), (dict(stride=99), INVALID), (dict(t=float("nan")), INVALID),
-    (dict(t=float("inf")), INVALID),
+    (dict(t=float("inf")), INVALID), (dict(t=1e-40), INVALID), (dict(rows=1 << 24), INVALID),
 ])
 def test_bad_logprobs(over, status):
     a = dict(x=P, dtype=0, rows=2, n=100, stride=0, t=1.0, tokens=P, lp=P, h=P, top=3, ids=P, tl=P)
