@@ -6,17 +6,17 @@
 // The order of the top: larger y first, among equals the lower id.
 //
 // Bound by the read of the logits: 2048 rows of 151936 fp32 with the top 5 take 232 us, 5.4 TB/s.
-// segment_kernel reads them once: a wave takes a segment of a row
-// in rounds of 2048 values that stay in registers, the next round's loads issued before the
-// current one is worked on. Per round: the maximum, then the two sums about the running maximum;
-// for the top, values that beat the wave's n-th best so far go to a list in LDS, which is cut to
-// the best n when it fills. The first round's bound is the n-th largest of 128 group maxima (there
-// are n values no smaller), found bit by bit with ballots, so that about n values pass it and not
-// all. join_kernel joins a row's segments: sums rescaled to one maximum; of the segments' lists the
-// entries no smaller than the n-th largest of their heads, which are few, are ranked. Where they are
-// many (equals; fewer segments than places), the n-th best is found bit by bit over all entries
-// first, then, if there are more equals of it than places, the last id among them (8 rows of
-// 151936, top 20: always bit by bit 13.2 us, heads first 9.4).
+// segment_kernel reads them once: a wave takes a segment of a row in rounds of 2048 values that
+// stay in registers, the next round's loads issued before the current one is worked on. Per round:
+// the maximum, then the two sums about the running maximum; for the top, values that beat the
+// wave's n-th best so far go to a list in LDS, which is cut to the best n when it fills. The first
+// round's bound is the n-th largest of 128 group maxima (there are n values no smaller), found bit
+// by bit with ballots, so that about n values pass it and not all. join_kernel joins a row's
+// segments: sums rescaled to one maximum; of the segments' lists the entries no smaller than the
+// n-th largest of their heads, which are few, are ranked. Where they are many (equals; fewer
+// segments than places), the n-th best is found bit by bit over all entries first, then, if there
+// are more equals of it than places, the last id among them (8 rows of 151936, top 20: always bit
+// by bit 13.2 us, heads first 9.4).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -143,7 +143,8 @@ __global__ __launch_bounds__(kThreads) void segment_kernel(Args a) {
     float m = -INFINITY, z = 0.0f, w = 0.0f;
     bool bad = false;
 
-    // round r's values of this lane: element e of piece p is id from + r kRound + (64 p + lane) VEC + e
+    // round r's values of this lane: element e of piece p is id
+    // from + r kRound + (64 p + lane) VEC + e
     u4 next[NP];
     auto load = [&](int r) {
         const long long base = from + (long long)r * kRound;
@@ -502,7 +503,8 @@ CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
     a.top_logprobs = top_logprobs;
     a.top_n = top_n;
     set_segments(a);
-    if (!workspace || workspace_bytes < workspace_of(a) || reinterpret_cast<uintptr_t>(workspace) % 16)
+    if (!workspace || workspace_bytes < workspace_of(a) ||
+        reinterpret_cast<uintptr_t>(workspace) % 16)
         return set_error(CSDR_E_WORKSPACE,
                          "token_logprobs: workspace missing, too small or unaligned");
     const size_t parts = (size_t)rows * a.segments;

@@ -62,8 +62,8 @@ __host__ __device__ __forceinline__ SeqRows seq_rows(const PagedView& pv, int b)
 }
 
 // The page of position p of sequence b (SCALAR: the same in the whole wave, looked up through the
-// scalar cache also behind barriers, which a constant table allows), or -1 where the table has none (positions past its end,
-// ids outside [0, n_pages)).
+// scalar cache also behind barriers, which a constant table allows), or -1 where the table has none
+// (positions past its end, ids outside [0, n_pages)).
 template <bool SCALAR = false>
 __host__ __device__ __forceinline__ int page_of(const PagedView& pv, int b, int p) {
     const int i = p >> pv.shift;
@@ -113,8 +113,9 @@ __device__ __forceinline__ float cache_value(const uint8_t* p, bool is_v, int ps
     const uint32_t w =
         reinterpret_cast<const uint32_t*>(p)[is_v ? v_word<HD>(slot, d) : k_word<HD>(slot, d)];
     const float c = (float)((w >> code_shift(is_v ? slot & 7 : d & 7)) & 15u);
-    const float s = (float)*reinterpret_cast<const _Float16*>(p + scale_offset(HD, ps, d / kGroup, slot));
-    const float m = (float)*reinterpret_cast<const _Float16*>(p + min_offset(HD, ps, d / kGroup, slot));
+    const int g = d / kGroup;
+    const float s = (float)*reinterpret_cast<const _Float16*>(p + scale_offset(HD, ps, g, slot));
+    const float m = (float)*reinterpret_cast<const _Float16*>(p + min_offset(HD, ps, g, slot));
     return fmaf(s, c, m);
 }
 

@@ -59,8 +59,8 @@ __device__ __forceinline__ Seen seen_of(const AttnArgs& a, int b, const SeqRows&
     return s;
 }
 
-// The tiles of T positions that columns at positions pq0 .. pq1 see: `low` tiles from 0 on (prefix),
-// then those from w0 on (window and causal part), n in all.
+// The tiles of T positions that columns at positions pq0 .. pq1 see: `low` tiles from 0 on
+// (prefix), then those from w0 on (window and causal part), n in all.
 template <int T>
 struct Tiles {
     int low, w0, n;
@@ -241,6 +241,12 @@ struct TileParams {
     __device__ h8 at(int row, int i) const { return piece[4 * row + i]; }
 };
 
+// Orders a wave's LDS accesses on both sides: lanes read what others have written. (LDS serves a
+// wave in order, so this costs no wait.)
+__device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+}
+
 // Where a tile's data lie: a pointer for positions tb .. tb + 15 of the head and one for the rest
 // (the same page unless pages hold 16), and the lane's offsets, which do not change.
 struct Pages {
@@ -353,12 +359,13 @@ __device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, 
     return (s - slope * (float)abs(dist)) * kLog2e;
 }
 
-// A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a power
-// of two that puts its largest magnitude in [2^TOP, 2^(TOP + 1)), then in pairs of fp16 (fp16: as it
-// is unless TOP is given). A negative scale turns the query round. Returns the (positive) factor from products to scores, in the log2 domain
-// if there are no options.
+// A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a
+// power of two that puts its largest magnitude in [2^TOP, 2^(TOP + 1)), then in pairs of fp16
+// (fp16: as it is unless TOP is given). A negative scale turns the query round. Returns the
+// (positive) factor from products to scores, in the log2 domain if there are no options.
 template <int HD, typename XT, bool OPTS, int TOP = sizeof(XT) == 4 ? 13 : 0>
-__device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int g, h8* qh, h8* ql) {
+__device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int g, h8* qh,
+                                            h8* ql) {
     constexpr bool PAIR = sizeof(XT) == 4;
     float unit = fabsf(OPTS ? a.scale : a.scale * kLog2e);
     float x[HD / 32][8], big = 0.0f, f = 1.0f;
@@ -401,7 +408,8 @@ struct Splits {
 // So nothing crosses lanes but the maximum, and that only when it moves by more than kLag.
 // 4 bits: codes enter the products as whole numbers (16 + code for K; code - 8 for V, centred, so
 // that sums do not cancel); K's scale is applied to the group's 32-dim partial score, V's to the
-// weights, and what the minima (and the 16) add comes from small products of their own. fp32 calls carry q and the weights as pairs of fp16 (22 bits).
+// weights, and what the minima (and the 16) add comes from small products of their own. fp32 calls
+// carry q and the weights as pairs of fp16 (22 bits).
 template <int HD, bool Q4, typename XT, bool OPTS>
 __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Splits sp) {
     constexpr bool PAIR = sizeof(XT) == 4;
@@ -497,6 +505,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
         float vscale = 0.0f;  // the largest of V's scales that this lane loaded
         if constexpr (Q4) {
             if (!whole && at.parv) t.par = only(t.par, plive);
+            lanes_meet();  // (the last tile's reads are done)
             if (at.parv && (lane & 31) < 4 * NS)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) vscale = fmaxf(vscale, (float)t.par[j]);
@@ -505,6 +514,7 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     reinterpret_cast<_Float16*>(&tp.k[8 * (lane & 3) + j])[lane >> 2] = t.par[j];
+            lanes_meet();
         }
 
         // scores of positions p8 + j
@@ -782,10 +792,10 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 
 // Attention of many columns, the (token, query head) pairs of one sequence and KV head: a workgroup
 // of NW waves takes 16 NQ NW of them, a wave NQ tiles of 16 (column tiles are dealt to the waves in
-// turn, so that under a causal mask all see about as many positions). Tiles of TP positions of K and V lie
-// in LDS twice, the next one being brought in while the current one is worked on; a wave reads each
-// operand once for its NQ column tiles. The products, the running maximum and what a lane holds
-// are step_kernel's, all NQ column tiles beside each other.
+// turn, so that under a causal mask all see about as many positions). Tiles of TP positions of K
+// and V lie in LDS twice, the next one being brought in while the current one is worked on; a wave
+// reads each operand once for its NQ column tiles. The products, the running maximum and what a
+// lane holds are step_kernel's, all NQ column tiles beside each other.
 //
 // fp16 pages go straight to LDS (16 bytes a lane); K's 16-byte chunks of a row are permuted within
 // the row on the way (chunk j of row r at j ^ key(r)), so that the 16 rows of an operand read fall
@@ -827,9 +837,10 @@ prompt_kernel(AttnArgs a, Splits sp) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.hq / pv.hkv;
     // (sequence, KV head) fastest: on a chip of 8 dies that take workgroups in turn, the blocks of
-    // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns, which see
-    // most, first; where a CU takes two workgroups, the second 256 in the opposite order, so that a CU
-    // with the longest of the first has the shortest of the second (4096 tokens: 182 -> 175 us).
+    // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns, which
+    // see most, first; where a CU takes two workgroups, the second 256 in the opposite order, so
+    // that a CU with the longest of the first has the shortest of the second (4096 tokens: 182 ->
+    // 175 us).
     const int pairs = pv.n_seqs * pv.hkv, blocks = gridDim.x / pairs;
     const int bh = blockIdx.x % pairs, around = max(1, 256 / pairs);
     int rank = blockIdx.x / pairs;
@@ -886,8 +897,8 @@ prompt_kernel(AttnArgs a, Splits sp) {
     auto buffer = [&](int buf, int v, int plane) {
         return lds + ((buf * 2 + v) * PLANES + plane) * PLANE;
     };
-    // page ids of a tile's granules of 16 positions (uniform; through the scalar cache 172 -> 168 us
-    // for 4096 tokens on fp16 pages, but 600 -> 644 where 4-bit pages are unpacked between)
+    // page ids of a tile's granules of 16 positions (uniform; through the scalar cache 164 -> 157
+    // us for 4096 tokens on fp16 pages, but 600 -> 644 where 4-bit pages are unpacked between)
     auto pages_at = [&](int tb, int* pg) {
 #pragma unroll
         for (int i = 0; i < GR; ++i)
@@ -1172,11 +1183,11 @@ constexpr int kStepColumns = 64;
 constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
 constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
-// Splits of the positions: for step_kernel 768 workgroups in all (the three that a CU holds at once),
-// or twice as many where sequences may differ in length (one sequence of 131071 on 4-bit pages: 768
-// 50 us, 1536 57; 64 sequences of 4096 to 8192: 148 and 139), 128 positions (a tile per wave) each
-// at least; for prompt_kernel one if there are 512 workgroups, else enough for
-// that, 512 positions at least. A sequence's positions are shared out equally, so a call with
+// Splits of the positions: for step_kernel 768 workgroups in all (the three that a CU holds at
+// once), or twice as many where sequences may differ in length (one sequence of 131071 on 4-bit
+// pages: 768 50 us, 1536 57; 64 sequences of 4096 to 8192: 148 and 139), 128 positions (a tile per
+// wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for that, 512
+// positions at least. A sequence's positions are shared out equally, so a call with
 // sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
 // ever makes fewer splits.
 Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
@@ -1208,8 +1219,8 @@ size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
     return csdr::align_up(parts * 8, 16) + parts * hd * 4;
 }
 
-// Column tiles per wave of prompt_kernel: as many as 256 registers hold (sums, queries, weights), or
-// one where that would leave the chip without two workgroups a CU (SMALL). Waves per workgroup:
+// Column tiles per wave of prompt_kernel: as many as 256 registers hold (sums, queries, weights),
+// or one where that would leave the chip without two workgroups a CU (SMALL). Waves per workgroup:
 // eight where 4-bit rows of 128 are unpacked, which then serves twice the columns.
 template <int HD, bool Q4, typename XT, bool SMALL>
 struct PromptConfig {

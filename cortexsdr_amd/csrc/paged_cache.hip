@@ -31,7 +31,7 @@ using csdr::set_error;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr long long kMaxBlocks = (1LL << 32) / kThreads - 1;  // a launch has fewer than 2^32 threads
+constexpr long long kMaxBlocks = (1LL << 32) / kThreads - 1;  // fewer than 2^32 threads a launch
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
