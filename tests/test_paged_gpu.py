@@ -89,7 +89,7 @@ class Setup:
 
 HEADS = {"qwen": (14, 2, 64), "llama": (4, 4, 128), "gqa": (8, 2, 128), "many": (20, 1, 64),
          "one": (2, 2, 64),
-         "three": (6, 2, 64)}
+         "three": (6, 2, 64), "wide": (80, 1, 64), "wider": (130, 2, 128)}
 
 
 # ---------------------------------------------------------------- append, read
@@ -594,3 +594,88 @@ def test_large_queries_and_keys(gpu):
         got = s.batch.attend(s.dev(q), scale=float(1 / sigma / 8)).cpu().numpy()
         want = ref.attend(q, [59], s.k[0], s.v[0], scale=float(np.float32(1 / sigma / 8)))
         assert rel_l2(got, want) <= TOL32, sigma
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("heads", ["wide", "wider"])
+def test_step_of_many_heads(gpu, kv, x, heads):
+    """More than 64 query heads to a KV head: single tokens, in the form for prompts."""
+    s = Setup(gpu, [700, 1, 40], HEADS[heads], kv, x, ps=32, seed=41)
+    s.append([699, 0, 39], with_q=False)
+    qd, _ = s.append([1, 1, 1])
+    want = s.expect(qd.cpu().numpy(), [1, 1, 1])
+    assert rel_l2(s.batch.attend(qd).cpu().numpy(), want) <= tol(x)
+    assert rel_l2(s.batch.attend(qd, max_len=700).cpu().numpy(), want) <= tol(x)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+def test_largest_pages(gpu, kv, x):
+    s = Setup(gpu, [4200, 17], HEADS["three"], kv, x, ps=4096, seed=42, theta=1e4)
+    s.append([4100, 10], with_q=False)
+    for new in ([1, 1], [99, 6]):
+        qd, _ = s.append(new)
+        got = s.batch.attend(qd, q_start=s.starts(new), max_q=max(new))
+        assert rel_l2(got.cpu().numpy(), s.expect(qd.cpu().numpy(), new)) <= tol(x)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("scale", [-0.125, 1e-3])
+def test_given_scale(gpu, kv, x, tokens, scale):
+    s = Setup(gpu, [200], HEADS["three"], kv, x, seed=43)
+    s.append([150], with_q=False)
+    qd, _ = s.append([tokens])
+    for o in ({}, dict(cap=3.0)):
+        want = s.expect(qd.cpu().numpy(), [tokens], scale=scale, **o)
+        got = s.batch.attend(qd, scale=scale, softcap=o.get("cap", 0.0))
+        assert rel_l2(got.cpu().numpy(), want) <= tol(x)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+def test_a_page_twice(gpu, kv):
+    """One page at two places of a row, and in two rows: read at each."""
+    s = Setup(gpu, [64, 64], HEADS["three"], kv, ps=16, seed=44)
+    s.append([64, 64], with_q=False)
+    s.table[:, 2] = s.table[0, 0]
+    for b in range(2):
+        s.k[b][32:48], s.v[b][32:48] = s.k[0][:16], s.v[0][:16]
+    for tokens in (1, 30):
+        q = s.draw(2 * tokens, 6, 1.5)
+        got = s.batch.attend(s.dev(q))
+        assert rel_l2(got.cpu().numpy(), s.expect(q, [tokens] * 2)) <= TOL32
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+def test_given_pools_queries_in_place_other_stream(gpu, kv):
+    """Pools of the caller's, rotation over the queries themselves, every call on a given stream."""
+    from cortexsdr_amd.paged import PagedCache
+
+    s = Setup(gpu, [90, 50], HEADS["gqa"], kv, seed=45, theta=1e5)
+    s.cache = PagedCache(s.cache.n_pages, 16, 2, 128, kv, k=s.cache.k.view(-1), v=s.cache.v)
+    s.batch = s.cache.batch(s.table, s.lens)
+    s.append([50, 10], with_q=False)
+    s.len = [90, 50]
+    s.lens.copy_(gpu.tensor(s.len, dtype=gpu.int32))
+    q, k, v = s.draw(80, 8), s.draw(80, 2), s.draw(80, 2)
+    qd, kd, vd = s.dev(q), s.dev(k), s.dev(v)
+    side = gpu.cuda.Stream()
+    side.wait_stream(gpu.cuda.current_stream())
+    assert s.batch.append(qd, kd, vd, theta=1e5, q_out=qd, stream=side) is qd
+    got = s.batch.attend(qd, stream=side)
+    rk, rv = s.batch.read(80, stream=side)
+    gpu.cuda.current_stream().wait_stream(side)
+    pos = s.positions([40, 40])
+    qr = np.concatenate([ref.rotate(q[:40], pos[0], 1e5), ref.rotate(q[40:], pos[1], 1e5)])
+    # half a step of fp32, and the rounding of the fp64 pair before it
+    assert float(np.abs(qd.cpu().numpy() - qr).max()) <= 2.0 ** -24 * 1.01 * np.abs(qr).max()
+    for b in range(2):
+        kr = ref.rotate(k[40 * b:40 * b + 40], pos[b], 1e5).astype(np.float32)
+        s.k[b] = np.concatenate([s.k[b], ref.held(kr, kv)])
+        s.v[b] = np.concatenate([s.v[b], ref.held(v[40 * b:40 * b + 40], kv)])
+    last = [np.concatenate([a[0][-40:], a[1][-40:]]) for a in (s.k, s.v)]
+    assert rel_l2(rk.cpu().numpy(), last[0]) <= TOL32
+    assert rel_l2(rv.cpu().numpy(), last[1]) <= TOL32
+    assert rel_l2(got.cpu().numpy(), s.expect(qr, [40, 40])) <= TOL32
