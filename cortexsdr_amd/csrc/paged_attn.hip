@@ -340,23 +340,33 @@ __device__ __forceinline__ h8 only(h8 v, uint32_t live) {
     return __builtin_bit_cast(h8, w);
 }
 
-// Scores with the options, in the log2 domain; `x` the products q.k in units of 1 / unit.
-template <bool OPTS>
-__device__ __forceinline__ float score2(const AttnArgs& a, float x, float unit, float slope,
-                                        int dist) {
-    if constexpr (!OPTS) return x * unit;
-    float s = x * unit;
+// Eight scores with the options, in the log2 domain, of positions `back`, back - 1 .. behind the
+// token (ahead of it below 0); `x` the products q.k in units of 1 / unit. (One branch for all eight:
+// with one at each score, no two are on their way together.)
+__device__ __forceinline__ void shape8(const AttnArgs& a, float* x, float unit, float slope,
+                                       int back) {
     if (a.cap > 0.0f) {
-        const float t = s * a.inv_cap, b = fabsf(t);
-        // tanh: 1 - 2 / (e^2b + 1), absolutely exact to 2^-23, and its series for small b
-        const float e = exp2_fast(2.0f * kLog2e * b);
-        float y = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-        const float t2 = b * b;
-        const float p = b * fmaf(t2, fmaf(t2, fmaf(t2, -17.0f / 315, 2.0f / 15), -1.0f / 3), 1.0f);
-        y = b < 0.2f ? p : y;
-        s = a.cap * copysignf(y, t);
+        const float to = unit * a.inv_cap, cap = a.cap * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = x[j] * to, b = fabsf(t);
+            // tanh: 1 - 2 / (e^2b + 1), absolutely exact to 2^-23, and its series for small b
+            const float e = exp2_fast(2.0f * kLog2e * b);
+            const float y = fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+            const float t2 = t * t;
+            const float p = b * fmaf(t2, fmaf(t2, fmaf(t2, -17.0f / 315, 2.0f / 15), -1.0f / 3), 1.0f);
+            x[j] = cap * copysignf(b < 0.2f ? p : y, t);
+        }
+    } else {
+        const float to = unit * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= to;
     }
-    return (s - slope * (float)abs(dist)) * kLog2e;
+    if (a.slopes) {
+        const float s = -slope * kLog2e, d = (float)back;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(s, fabsf(d - (float)j), x[j]);
+    }
 }
 
 // A column's query as B operand: dims 32 s + 8 g .. for lane group g. fp32: the row scaled by a
@@ -553,10 +563,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
             }
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s8[4 * u + i] = score2<OPTS>(a, acc[u][i], unit, slope, pq - (p8 + 4 * u + i));
+        for (int j = 0; j < 8; ++j) s8[j] = OPTS ? acc[j >> 2][j & 3] : acc[j >> 2][j & 3] * unit;
+        if constexpr (OPTS) shape8(a, s8, unit, slope, pq - p8);
         if constexpr (MORE) {
             const Pages kp = pages_of<HD, Q4>(pv.k, pv, kvh, ng0, ng1);
             load_k<HD, Q4>(t, pv, kp, nb, at);
@@ -1075,11 +1083,8 @@ prompt_kernel(AttnArgs a, Splits sp) {
                     // scores, without options still in the products' units
                     float x[8], top = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        x[j] = acc[q][j >> 2][j & 3];
-                        if constexpr (OPTS)
-                            x[j] = score2<OPTS>(a, x[j], unit[q], slope[q], pq[q] - (p8 + j));
-                    }
+                    for (int j = 0; j < 8; ++j) x[j] = acc[q][j >> 2][j & 3];
+                    if constexpr (OPTS) shape8(a, x, unit[q], slope[q], pq[q] - p8);
                     if (!whole) {
                         const bool row = (have >> ((32 * hb + 8 * g) / 16) & 1) & (pq[q] >= 0);
 #pragma unroll
