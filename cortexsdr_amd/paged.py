@@ -126,7 +126,7 @@ class PagedBatch:
             raise ValueError("table must be (sequences, pages)")
         _ints(torch, "table", table, tuple(table.shape))
         _ints(torch, "lens", lens, (table.shape[0],))
-        _on_device(torch, "table and lens", table, lens)
+        self._device = _on_device(torch, "table, lens and pools", table, lens, cache.k)
         self.cache, self.table, self.lens = cache, table, lens
         self.n_seqs = int(table.shape[0])
         self._kv = _lib.PagedKV(cache.k.data_ptr(), cache.v.data_ptr(), table.data_ptr(),
@@ -137,6 +137,13 @@ class PagedBatch:
         self._lib = _lib.load()
         self._append, self._attn = self._lib.csdr_paged_append, self._lib.csdr_paged_attn
         self._need = {}  # workspace bytes by the call's sizes
+
+    def _here(self, torch, *ts) -> int:
+        """Checks that a call's tensors and the cache are on the current device; its index."""
+        dev = _on_device(torch, "tensors", *ts)
+        if dev != self._device:
+            raise ValueError("the cache must be on the current device")
+        return dev
 
     def _starts(self, torch, q_start, max_q):
         if q_start is None:
@@ -189,7 +196,7 @@ class PagedBatch:
         elif q_out is not None:
             raise ValueError("q_out without q")
         starts, mq = self._starts(torch, q_start, max_q)
-        dev = _on_device(torch, "tensors", q, k, v, q_out, q_start)
+        dev = self._here(torch, q, k, v, q_out, q_start)
         rc = self._append(
             self._ref, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), dt, n,
             starts, mq, nq, qs, ks, vs, theta, q_out.data_ptr() if q_out is not None else None,
@@ -226,7 +233,7 @@ class PagedBatch:
                                            prefix.data_ptr() if prefix is not None else None))
         starts, mq = self._starts(torch, q_start, max_q)
         max_len = min(max_len, _INT_MAX)
-        dev = _on_device(torch, "tensors", q, out, q_start, slopes, prefix, workspace)
+        dev = self._here(torch, q, out, q_start, slopes, prefix, workspace)
         if workspace is None:
             key = (n, starts is None, mq, nq, max_len)
             need = self._need.get(key)
@@ -263,7 +270,7 @@ class PagedBatch:
                       torch.float16 if dtype == "f16" else torch.float32, c.k.device,
                       stream).unbind(0)
         starts, mq = self._starts(torch, q_start, max_q)
-        dev = _on_device(torch, "tensors", k, q_start)
+        dev = self._here(torch, k, q_start)
         _check(self._lib.csdr_paged_read(self._ref, n_tokens, starts, mq, k.data_ptr(),
                                          v.data_ptr(), int(dtype == "f16"),
                                          _stream_of(torch, dev, stream)))

@@ -387,6 +387,24 @@ def test_python_refusals(gpu):
             call()
 
 
+def test_cache_of_another_device(gpu):
+    """The current device is another than the cache's, and the call's tensors are on it."""
+    from cortexsdr_amd.paged import PagedBatch
+
+    s = Setup(gpu, [16], HEADS["three"], "f16", seed=24)
+    s.append([4], with_q=False)
+    s.batch._device += 1  # as if
+    q, k = gpu.zeros(1, 6, 64, device="cuda"), gpu.zeros(1, 2, 64, device="cuda")
+    for call in (lambda: s.batch.append(q, k, k), lambda: s.batch.attend(q),
+                 lambda: s.batch.read(1)):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+    pools, s.cache.k = s.cache.k, s.cache.k.cpu()
+    with pytest.raises(ValueError, match="current device"):
+        PagedBatch(s.cache, s.table, s.lens)
+    s.cache.k = pools
+
+
 def test_bounds_past_an_int(gpu):
     """A window, a length bound and a most of tokens past 2^31 bound nothing."""
     s = Setup(gpu, [300], HEADS["three"], "f16", seed=23)
