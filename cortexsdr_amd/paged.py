@@ -49,6 +49,11 @@ def _on_device(torch, what: str, *ts) -> int:
     return dev
 
 
+def _stream_on(stream, dev: int) -> None:
+    if stream.device_index != dev:
+        raise ValueError("stream must be one of the current device")
+
+
 def _stream_of(torch, dev: int, stream) -> int:
     """The hipStream_t of `stream`, or of the device's current stream."""
     global _raw
@@ -57,6 +62,7 @@ def _stream_of(torch, dev: int, stream) -> int:
             _raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
                 (lambda d: int(torch.cuda.current_stream(d).cuda_stream))
         return _raw(dev)
+    _stream_on(stream, dev)
     return int(stream.cuda_stream)
 
 
@@ -64,6 +70,7 @@ def _empty(torch, shape, dtype, device, stream):
     """A tensor of the stream that will write it (the current one if None)."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
+    _stream_on(stream, torch.cuda.current_device())
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
 

@@ -399,6 +399,15 @@ def test_cache_of_another_device(gpu):
                  lambda: s.batch.read(1)):
         with pytest.raises(ValueError, match="current device"):
             call()
+    s.batch._device -= 1
+
+    class Elsewhere(gpu.cuda.Stream):
+        device_index = 1
+
+    for call in (lambda: s.batch.append(q, k, k, q_out=q, stream=Elsewhere()),
+                 lambda: s.batch.attend(q, out=q.clone(), max_len=1, stream=Elsewhere())):
+        with pytest.raises(ValueError, match="stream"):
+            call()
     pools, s.cache.k = s.cache.k, s.cache.k.cpu()
     with pytest.raises(ValueError, match="current device"):
         PagedBatch(s.cache, s.table, s.lens)
