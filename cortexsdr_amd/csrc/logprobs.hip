@@ -201,8 +201,10 @@ __global__ __launch_bounds__(kThreads) void segment_kernel(Args a) {
         const float top = wave_max(fmaxf(big[0], big[1]));
         if (top == -INFINITY) continue;
         if (top > m) {
-            const float f = m == -INFINITY ? 0.0f : exp2f((m - top) * kLog2e);
-            w = f * (w + (m == -INFINITY ? 0.0f : z * (m - top)));
+            // (f = 0: what came before is nothing beside this round, and its z (m - top) may be
+            // past fp32, as after rounds of the type's lowest value)
+            const float d = m - top, f = exp2f(d * kLog2e);
+            w = f > 0.0f ? f * fmaf(z, d, w) : 0.0f;
             z *= f;
             m = top;
         }
