@@ -1,9 +1,10 @@
 // logprobs.hip — log probabilities of given tokens, entropy and the most likely tokens of rows of
 // logits (gfx950).
 //
-//   y = x / temperature; m = max y; Z = sum exp(y - m); logprob_t = y_t - m - log Z
-//   entropy = log Z - sum exp(y - m) (y - m) / Z
-// The order of the top: larger y first, among equals the lower id.
+//   m = max x; d = (x - m) / temperature; Z = sum exp d; logprob_t = d_t - log Z
+//   entropy = log Z - sum exp(d) d / Z
+// (Differences first: x / temperature alone may be past fp32 where d is not.)
+// The order of the top: larger x first, among equals the lower id.
 //
 // Bound by the read of the logits: 2048 rows of 151936 fp32 with the top 5 take 232 us, 5.4 TB/s.
 // segment_kernel reads them once: a wave takes a segment of a row in rounds of 2048 values that
@@ -179,13 +180,13 @@ __global__ __launch_bounds__(kThreads) void segment_kernel(Args a) {
     };
     if (rounds > 0) load(0);
     for (int r = 0; r < rounds; ++r) {
-        float y[kPer];
+        float y[kPer];                          // the round's logits
         float big[2] = {-INFINITY, -INFINITY};  // maxima of the lane's two groups of 16
         int hi = 0x80000000;                    // NaN and +infinity, by their bits
         uint32_t lo = 0u;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            y[k] = element<XT>(next[k / VEC], k % VEC) * a.inv_t;
+            y[k] = element<XT>(next[k / VEC], k % VEC);
             hi = max(hi, __float_as_int(y[k]));
             lo = max(lo, __float_as_uint(y[k]));
         }
@@ -201,9 +202,9 @@ __global__ __launch_bounds__(kThreads) void segment_kernel(Args a) {
         const float top = wave_max(fmaxf(big[0], big[1]));
         if (top == -INFINITY) continue;
         if (top > m) {
-            // (f = 0: what came before is nothing beside this round, and its z (m - top) may be
-            // past fp32, as after rounds of the type's lowest value)
-            const float d = m - top, f = exp2f(d * kLog2e);
+            // (f = 0: what came before is nothing beside this round, and its z d may be past
+            // fp32, as after rounds of the type's lowest value)
+            const float d = (m - top) * a.inv_t, f = exp2f(d * kLog2e);
             w = f > 0.0f ? f * fmaf(z, d, w) : 0.0f;
             z *= f;
             m = top;
@@ -211,7 +212,8 @@ __global__ __launch_bounds__(kThreads) void segment_kernel(Args a) {
         float zr = 0.0f, wr = 0.0f;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
-            const float d = fmaxf(y[k] - m, -200.0f);  // exp(-200) is 0 here, 0 * -200 too
+            // exp(-200) is 0 here, 0 * -200 too
+            const float d = fmaxf((y[k] - m) * a.inv_t, -200.0f);
             const float e = __builtin_amdgcn_exp2f(d * kLog2e);
             zr += e;
             wr = fmaf(e, d, wr);
@@ -308,15 +310,15 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
                 id[i] = (uint32_t)e[k];
             }
         }
-    float yt = 0.0f;
+    float xt = 0.0f;
     if (token >= 0 && token < a.n)
-        yt = (float)static_cast<const XT*>(a.x)[(long long)row * a.stride + token] * a.inv_t;
+        xt = (float)static_cast<const XT*>(a.x)[(long long)row * a.stride + token];
     const float m = wave_max(fmaxf(p[0].x, p[1].x));
     float z = 0.0f, w = 0.0f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         if (p[k].x == -INFINITY) continue;
-        const float d = p[k].x - m, f = expf(d);
+        const float d = (p[k].x - m) * a.inv_t, f = expf(d);
         z = fmaf(f, p[k].y, z);
         w += f * (p[k].z + (f > 0.0f ? p[k].y * d : 0.0f));
     }
@@ -328,7 +330,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
         if (a.entropy) a.entropy[row] = none ? lz : lz - w / z;
         if (a.tokens) {
             float lp = token < 0 ? 0.0f : NAN;
-            if (token >= 0 && token < a.n && !bad) lp = yt == -INFINITY ? yt : yt - m - lz;
+            if (token >= 0 && token < a.n && !bad)
+                lp = xt == -INFINITY ? xt : (xt - m) * a.inv_t - lz;
             a.logprobs[row] = lp;
         }
     }
@@ -424,7 +427,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
             }
             if (rank < n) {
                 a.top_ids[(long long)row * n + rank] = e.i;
-                a.top_logprobs[(long long)row * n + rank] = e.v - m - lz;
+                a.top_logprobs[(long long)row * n + rank] = (e.v - m) * a.inv_t - lz;
             }
         }
         for (int i = nbest + threadIdx.x; i < n; i += kThreads) {

@@ -645,16 +645,17 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
  * ==================================================================== */
 
 /* For each of `rows` rows of n logits (dtype CSDR_F32 or CSDR_F16, row_stride elements apart, 0 =
- * n), y = logits / temperature (temperature <= 0: 1, a denormal one is refused, as select_best_from_logits,
- * cortex_sdk.cpp:1005-1030): logprobs[r] = y[tokens[r]] - log sum exp y (tokens NULL: not
+ * n), y = logits / temperature (as select_best_from_logits, cortex_sdk.cpp:1005-1030; temperature
+ * <= 0: 1, a denormal one is refused): logprobs[r] = y[tokens[r]] - log sum exp y (tokens NULL: not
  * computed; a negative token: 0; one >= n: NaN), entropy[r] = -sum p log p in nats (may be NULL),
- * and the top_n (0..64) largest y, largest first and lower ids first among equals:
+ * and the top_n (0..64) largest logits, largest first and lower ids first among equals:
  * top_ids[r * top_n + i], top_logprobs likewise; ids -1 and -infinity where fewer tokens have a
- * logit above -infinity. -infinity is a token that cannot be (probability 0, nothing in the
- * entropy); a row of nothing else has log probabilities -infinity and entropy 0; a NaN or
- * +infinity in a row makes its log probabilities and entropy NaN, and NaN is never among the
- * top. workspace: csdr_token_logprobs_workspace_bytes device bytes, 16-byte aligned, for this
- * call only. */
+ * logit above -infinity. y itself may pass fp32 (only its differences are formed): the lowest
+ * value is a mask at any temperature, and rows of nothing else are uniform. A logit of -infinity is
+ * a token that cannot be (probability 0, nothing in the entropy); a row of nothing else has log
+ * probabilities -infinity and entropy 0; a NaN or +infinity in a row makes its log probabilities
+ * and entropy NaN, and NaN is never among the top. workspace:
+ * csdr_token_logprobs_workspace_bytes device bytes, 16-byte aligned, for this call only. */
 CSDR_API size_t csdr_token_logprobs_workspace_bytes(int rows, int n, int top_n);
 CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
                                  int64_t row_stride, float temperature, const int32_t* tokens,
