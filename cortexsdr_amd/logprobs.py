@@ -21,7 +21,8 @@ class TokenLogprobs(typing.NamedTuple):
 def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0, workspace=None,
                    stream=None) -> TokenLogprobs:
     """logits: (rows, n) float32 or float16 on the device, rows any stride apart; tokens: (rows,)
-    int32, negative for none. With `stream` the call runs and allocates there, ordered by the
+    int32, negative for none. A row with a NaN or +infinity has NaN log probabilities, and only its
+    finite logits among the top. With `stream` the call runs and allocates there, ordered by the
     caller."""
     torch = _torch()
     lib = _lib.load()

@@ -654,8 +654,9 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
  * value is a mask at any temperature, and rows of nothing else are uniform. A logit of -infinity is
  * a token that cannot be (probability 0, nothing in the entropy); a row of nothing else has log
  * probabilities -infinity and entropy 0; a NaN or +infinity in a row makes its log probabilities
- * and entropy NaN, and NaN is never among the top. workspace:
- * csdr_token_logprobs_workspace_bytes device bytes, 16-byte aligned, for this call only. */
+ * and entropy NaN, and its top is of its finite logits alone (a +infinity is no largest value but a
+ * fault of the row, as a NaN is). workspace: csdr_token_logprobs_workspace_bytes device bytes,
+ * 16-byte aligned, for this call only. */
 CSDR_API size_t csdr_token_logprobs_workspace_bytes(int rows, int n, int top_n);
 CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
                                  int64_t row_stride, float temperature, const int32_t* tokens,
