@@ -152,8 +152,12 @@ constexpr float kLog2e = 1.44269504088896341f;
 // Weights are 2^(s - m + bias) in the log2 domain, m a maximum that may lag `lag` behind, so that m
 // moves, and the sums with it, only now and then: at most 2^15, near the top of fp16. fp32 calls: a
 // pair keeps its 22 bits down to 2^(bias - 30) of the largest weight (the step of its low half is
-// 2^-24); with a bias of 8, rows with a high maximum were 2e-5 to 1.6e-4 off. fp16 calls: one
-// rounding to 11 bits down to 2^-21 of it, which leaves more room to lag.
+// 2^-24); with a bias of 8, rows with a high maximum were 2e-5 to 1.6e-4 off. fp16 calls: 11 bits
+// down to 2^-21 of it do, which leaves more room to lag. One rounding to those 11 bits is a choice
+// of speed: outputs are 2.7e-4 to 3.0e-4 off where their own rounding makes 2.05e-4, and pairs, which
+// leave just that, cost 161 -> 205 us (prompt of 4096 on fp16 pages), 461 -> 537 (prompts on 4-bit
+// pages), 118 -> 135 and 46 -> 52 (single tokens on 4-bit pages). Single tokens on fp16 pages take
+// pairs in fp16 calls too: there they cost nothing (78.1 us both, 32 sequences of 4096).
 template <typename XT>
 constexpr float kLag = sizeof(XT) == 4 ? 2.0f : 8.0f;
 template <typename XT>
@@ -419,13 +423,14 @@ struct Splits {
 // 4 bits: codes enter the products as whole numbers (16 + code for K; code - 8 for V, centred, so
 // that sums do not cancel); K's scale is applied to the group's 32-dim partial score, V's to the
 // weights, and what the minima (and the 16) add comes from small products of their own. fp32 calls
-// carry q and the weights as pairs of fp16 (22 bits).
+// carry q and the weights as pairs of fp16 (22 bits), fp16 calls on fp16 pages the weights; those on
+// 4-bit pages round weights, and sum what they rounded (so that constant values come back).
 // fp16 pages: bound by their stream (32 sequences, fp16 calls: 81 us, 4.7 TB/s). 4 bits: by vector
 // instructions, about 450 beside 39 matrix ones a tile (64 sequences of 4096 to 8192, fp32 calls:
 // 143 us, 3.4 TB/s; one of 131071, fp16 calls: 48.5 us).
 template <int HD, bool Q4, typename XT, bool OPTS>
 __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Splits sp) {
-    constexpr bool PAIR = sizeof(XT) == 4;
+    constexpr bool PAIR = sizeof(XT) == 4, WPAIR = PAIR || !Q4;  // queries, weights
     constexpr int NS = HD / 32, ND = HD / 16;
     const PagedView& pv = a.pv;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -475,6 +480,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f4{0.f, 0.f, 0.f, 0.f};
     f4 par = {0.f, 0.f, 0.f, 0.f};  // 4 bits: sums of weights times what code 8 stands for
+    f4 lw = {0.f, 0.f, 0.f, 0.f};   // sums of weights rounded once, in par's units, in all rows
+    const h8 ones = h8{} + (_Float16)1.0f;
     float m = kNoMax, l = 0.0f;       // the (lagging) maximum, log2 domain; this lane's sum
     // exponent above V's largest scale (from fp16's smallest): weights are 2^-ev of the above
     float ev = Q4 ? -24.0f : 0.0f, vtop = 0x1p-24f;
@@ -605,7 +612,11 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
             l *= f;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= f;
-            if constexpr (Q4) par *= exp2_fast(m - mn);
+            if constexpr (Q4) {
+                const float fp = exp2_fast(m - mn);
+                par *= fp;
+                if constexpr (!WPAIR) lw *= fp;
+            }
             m = mn;
             ev = en;
         }
@@ -614,15 +625,15 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             w8[j] = exp2_fast(s8[j] + off);
-            l += w8[j];
+            if constexpr (WPAIR) l += w8[j];
         }
         if constexpr (!Q4) {
             h8 wh, wl;
-            split8<PAIR>(w8, wh, wl);
+            split8<WPAIR>(w8, wh, wl);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.v[d], wh, o[d], 0, 0, 0);
-                if constexpr (PAIR)
+                if constexpr (WPAIR)
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.v[d], wl, o[d], 0, 0, 0);
             }
         } else {
@@ -639,19 +650,21 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
                 ch[j] = (_Float16)ctr;
                 cl[j] = (_Float16)(ctr - (float)ch[j]);
             }
-            split8<PAIR>(w8, h8{} + (_Float16)vtop, wh, wl);
+            split8<WPAIR>(w8, h8{} + (_Float16)vtop, wh, wl);
             par = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, wh, par, 0, 0, 0);
             par = __builtin_amdgcn_mfma_f32_16x16x32_f16(cl, wh, par, 0, 0, 0);
-            if constexpr (PAIR)
+            if constexpr (WPAIR)
                 par = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, wl, par, 0, 0, 0);
+            else
+                lw = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wh, lw, 0, 0, 0);
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
-                split8<PAIR>(w8, tp.at(TileParams<HD>::kV + s, g), wh, wl);
+                split8<WPAIR>(w8, tp.at(TileParams<HD>::kV + s, g), wh, wl);
 #pragma unroll
                 for (int d = 2 * s; d < 2 * s + 2; ++d) {
                     const h8 vc = codes8(t.v[d], m0, m1);
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wh, o[d], 0, 0, 0);
-                    if constexpr (PAIR)
+                    if constexpr (WPAIR)
                         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vc, wl, o[d], 0, 0, 0);
                 }
             }
@@ -692,7 +705,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
     // join the waves: sums in units of 2^(m + ev)
     __shared__ float stat[kStepWaves][2][kCols];
     __shared__ float vec[kStepWaves][kCols][HD + 4];
-    l = lanes16_sum(l);
+    if constexpr (WPAIR) l = lanes16_sum(l);
+    else l = lw[0] * (1.0f / vtop);
     float corr[Q4 ? NS : 1];
     if constexpr (Q4) {
         // row 4 g + i of the product is group (4 g + i) mod NS

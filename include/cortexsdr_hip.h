@@ -629,7 +629,8 @@ typedef struct csdr_attn_options {
  * with a token each are better off in a call of their own than beside a prompt.
  *
  * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
- * CSDR_F16: weights rounded to fp16 once, fp32 sums. workspace:
+ * CSDR_F16: fp32 sums of weights rounded to fp16 once, in pairs too in the form for single tokens on
+ * fp16 pages. workspace:
  * csdr_paged_attn_workspace_bytes (may be 0) device bytes, 16-byte aligned, needed by this call
  * only: calls that may run at the same time need one each. */
 CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_tokens,
