@@ -1213,8 +1213,13 @@ constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt
 // wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for that, 512
 // positions at least. A sequence's positions are shared out equally, so a call with
 // sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
-// ever makes fewer splits.
-Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
+// ever makes fewer splits; beside a prefix, whose length is device memory, no fewer than 4096
+// positions have (one sequence, a window of 256 and a prefix of 32000: 80 -> 26 us, 128 tokens of
+// one: 259 -> 122; a window of 1024 and a prefix of 4: 14 us either way, but for all of the length's
+// splits 0 to 2 us more).
+constexpr long long kPrefixSeen = 4096;
+
+Splits splits_of(const PagedView& pv, int hq, int max_len, int window, bool prefix) {
     const int G = hq / pv.hkv;
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
@@ -1224,8 +1229,8 @@ Splits splits_of(const PagedView& pv, int hq, int max_len, int window) {
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
     const long long target = !step ? kPromptBlocks : pv.n_seqs == 1 ? 768 : 1536;
     // (a block's columns see a window each, and two tiles more where these do not fall on tiles)
-    const long long seen =
-        window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
+    long long seen = window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
+    if (prefix) seen = std::max(seen, std::min(len, kPrefixSeen));
     Splits s{};
     s.n = (int)std::max(1LL, std::min((seen + unit - 1) / unit,
                                       step ? (target + wgs - 1) / wgs : target / wgs));
@@ -1317,7 +1322,7 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
         Hq % kv->n_kv_heads || max_len < 0)
         return 0;
-    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len, 0));
+    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len, 0, false));
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
@@ -1356,7 +1361,7 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.q = q;
     a.out = out;
     a.hq = Hq;
-    Splits s = splits_of(a.pv, Hq, max_len, a.window);
+    Splits s = splits_of(a.pv, Hq, max_len, a.window, a.prefix != nullptr);
     // fewer than 2^32 threads a launch: workgroups of at most 256 (prompt_kernel: two threads a
     // column, except where it has few), join_kernel's only where there is one
     const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);

@@ -1,0 +1,36 @@
+"""How far csdr_paged_attn splits a sequence's positions, read off the workspace that a call asks
+for, without a GPU: the refused calls end before a launch."""
+import ctypes as C
+
+import pytest
+
+from cortexsdr_amd import _lib
+from test_paged_refusals import OUT, WORKSPACE, P, kv
+
+
+def refuses(n_bytes, tokens, **opt):
+    """Whether a workspace of n_bytes is too small for a call of one long sequence."""
+    rc = _lib.load().csdr_paged_attn(
+        kv(n_seqs=1, table_stride=4096), P, 0, tokens, None, 0, 4, 0, 0, 0.0,
+        C.byref(_lib.AttnOptions(**opt)), OUT, P, n_bytes, None)
+    return rc == WORKSPACE
+
+
+def bytes_of(tokens, splits):
+    return tokens * 4 * splits * (8 + 64 * 4)
+
+
+@pytest.mark.parametrize("tokens,unit", [(1, 128), (40, 512)])
+@pytest.mark.parametrize("window", [1, 256])
+def test_a_prefix_beside_a_window_is_split(tokens, unit, window):
+    """A prefix may be long, whatever the window: at least as many splits as 4096 positions have."""
+    assert refuses(bytes_of(tokens, 4096 // unit) - 1, tokens, window=window, prefix=P)
+
+
+@pytest.mark.parametrize("tokens,window", [(1, 256), (40, 2048), (1, 0)])
+def test_the_workspace_function_is_enough(tokens, window):
+    """What csdr_paged_attn_workspace_bytes says is no less than any options need."""
+    need = _lib.load().csdr_paged_attn_workspace_bytes(kv(n_seqs=1, table_stride=4096), tokens, None,
+                                                       0, 4, 0)
+    assert need >= bytes_of(tokens, 8)
+    assert refuses(bytes_of(tokens, 2) - 1, tokens, window=window)
