@@ -134,7 +134,7 @@ class PagedBatch:
         _ints(torch, "table", table, tuple(table.shape))
         _ints(torch, "lens", lens, (table.shape[0],))
         self._device = _on_device(torch, "table, lens and pools", table, lens, cache.k)
-        self.cache, self.table, self.lens = cache, table, lens
+        self.cache, self._table, self._lens = cache, table, lens
         self.n_seqs = int(table.shape[0])
         self._kv = _lib.PagedKV(cache.k.data_ptr(), cache.v.data_ptr(), table.data_ptr(),
                                 lens.data_ptr(), KV_DTYPES[cache.kv_dtype], cache.page_size,
@@ -144,6 +144,16 @@ class PagedBatch:
         self._lib = _lib.load()
         self._append, self._attn = self._lib.csdr_paged_append, self._lib.csdr_paged_attn
         self._need = {}  # workspace bytes by the call's sizes
+
+    @property
+    def table(self):
+        """Page ids, to be changed in place: a batch keeps the tensor it was made with."""
+        return self._table
+
+    @property
+    def lens(self):
+        """Lengths, to be changed in place as `table` is."""
+        return self._lens
 
     def _here(self, torch, *ts) -> int:
         """Checks that a call's tensors and the cache are on the current device; its index."""
