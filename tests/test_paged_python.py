@@ -12,6 +12,7 @@ def batch(monkeypatch):
     """A batch over host tensors (its pointers are used by no call that these tests make)."""
     from cortexsdr_amd import paged
 
+    monkeypatch.setattr(paged, "_torch", lambda: torch)
     monkeypatch.setattr(paged, "_on_device", lambda torch, what, *ts: 0)
     cache = types.SimpleNamespace(k=torch.zeros(4096, dtype=torch.uint8), kv_dtype="f16",
                                   v=torch.zeros(4096, dtype=torch.uint8), page_size=16, n_pages=1,
