@@ -22,8 +22,8 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
                    stream=None) -> TokenLogprobs:
     """logits: (rows, n) float32 or float16 on the device, rows any stride apart; tokens: (rows,)
     int32, negative for none. A row with a NaN or +infinity has NaN log probabilities, and only its
-    finite logits among the top. With `stream` the call runs and allocates there, ordered by the
-    caller."""
+    finite logits among the top. Without rows nothing is done. With `stream` the call runs and
+    allocates there, ordered by the caller."""
     torch = _torch()
     lib = _lib.load()
     dt = _dtype(logits)
@@ -37,7 +37,7 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         raise ValueError("tokens must be a contiguous int32 tensor, one per row")
     index = _on_device(torch, "tensors", logits, tokens, workspace)
     dev = logits.device
-    if workspace is None:
+    if workspace is None and rows > 0:
         need = lib.csdr_token_logprobs_workspace_bytes(rows, n, top_n)
         workspace = _empty(torch, need, torch.uint8, dev, stream) if need else None
     lp, entropy = _empty(torch, (2, rows), torch.float32, dev, stream).unbind(0)
@@ -47,6 +47,8 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         top = _empty(torch, (rows, top_n), torch.float32, dev, stream)
     if tokens is None:
         lp = None
+    if rows == 0:
+        return TokenLogprobs(lp, entropy, ids, top)
     _check(lib.csdr_token_logprobs(
         logits.data_ptr(), dt, rows, n, logits.stride(0) if rows > 1 else 0, temperature,
         tokens.data_ptr() if tokens is not None else None,

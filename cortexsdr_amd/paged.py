@@ -14,7 +14,7 @@ the caller's scheduler fills and may change between calls):
 With `stream`, a call runs on that stream, its outputs and workspace are allocated there, and the
 caller orders it against the streams its tensors come from. Workspaces are allocated per call
 (inside a graph capture, from that graph's pool), so calls on different streams and captured graphs
-share none unless the caller passes one to both.
+share none unless the caller passes one to both. A call of no tokens does nothing.
 """
 from __future__ import annotations
 
@@ -214,6 +214,8 @@ class PagedBatch:
             raise ValueError("q_out without q")
         starts, mq = self._starts(torch, q_start, max_q)
         dev = self._here(torch, q, k, v, q_out, q_start)
+        if n == 0:
+            return q_out
         rc = self._append(
             self._ref, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), dt, n,
             starts, mq, nq, qs, ks, vs, theta, q_out.data_ptr() if q_out is not None else None,
@@ -251,6 +253,8 @@ class PagedBatch:
         starts, mq = self._starts(torch, q_start, max_q)
         max_len = min(max_len, _INT_MAX)
         dev = self._here(torch, q, out, q_start, slopes, prefix, workspace)
+        if n == 0:
+            return out
         if workspace is None:
             key = (n, starts is None, mq, nq, max_len)
             need = self._need.get(key)
@@ -288,6 +292,8 @@ class PagedBatch:
                       stream).unbind(0)
         starts, mq = self._starts(torch, q_start, max_q)
         dev = self._here(torch, k, q_start)
+        if n_tokens == 0:
+            return k, v
         _check(self._lib.csdr_paged_read(self._ref, n_tokens, starts, mq, k.data_ptr(),
                                          v.data_ptr(), int(dtype == "f16"),
                                          _stream_of(torch, dev, stream)))

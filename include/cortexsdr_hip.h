@@ -584,8 +584,8 @@ typedef struct csdr_paged_kv {
 /* Bytes of one K page (and of one V page); 0 for a shape that is not supported. */
 CSDR_API size_t csdr_paged_page_bytes(int kv_dtype, int page_size, int n_kv_heads, int head_dim);
 
-/* The tokens of a call are n_tokens rows. q_start NULL: n_tokens / n_seqs rows of each sequence,
- * sequence-major. Else n_seqs + 1 row numbers (device): sequence b has rows q_start[b] up to
+/* The tokens of a call are n_tokens rows, one at least. q_start NULL: n_tokens / n_seqs rows of each
+ * sequence, sequence-major. Else n_seqs + 1 row numbers (device): sequence b has rows q_start[b] up to
  * q_start[b + 1], none if they are equal, and max_q (host) is the most that one has; rows past
  * max_q of a sequence and rows behind the last sequence are left as they were. Row i of the n rows
  * of a sequence is its position lens[b] - n + i; a row whose position is negative is no token.
@@ -621,16 +621,16 @@ typedef struct csdr_attn_options {
 /* out (n_tokens x Hq x head_dim, of dtype) = softmax attention of the tokens (rotated queries q,
  * as csdr_paged_append writes them) to the positions of their sequences that they see, after the
  * call's tokens were appended; GQA as repeat_kv_heads (cortex_sdk.cpp:1453-1478); scale 0 =
- * 1/sqrt(head_dim); out must not overlap q. A row that sees nothing is zero. What a token does not see has no influence on
- * it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
+ * 1/sqrt(head_dim); out must not overlap q. A row that sees nothing is zero. What a token does not
+ * see has no influence on it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
  * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
  * right, with less parallelism). One kernel serves a whole call, chosen by the most (token, query
  * head) pairs of a sequence and KV head: up to 64 take the form for single tokens, so sequences
  * with a token each are better off in a call of their own than beside a prompt.
  *
  * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
- * CSDR_F16: fp32 sums of weights rounded to fp16 once, in pairs too in the form for single tokens on
- * fp16 pages. workspace:
+ * CSDR_F16: fp32 sums of weights rounded to fp16 once, or in pairs too in the form for single
+ * tokens on fp16 pages. workspace:
  * csdr_paged_attn_workspace_bytes (may be 0) device bytes, 16-byte aligned, needed by this call
  * only: calls that may run at the same time need one each. */
 CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_tokens,

@@ -29,3 +29,43 @@ def test_table_and_lens_are_not_replaced(batch):
             setattr(batch, name, torch.zeros(2, dtype=torch.int32))
     batch.lens.fill_(5)
     assert batch.lens is lens and lens.tolist() == [5, 5]
+
+
+@pytest.fixture
+def calls(batch, monkeypatch):
+    """The batch's launches, recorded in place of being made."""
+    from cortexsdr_amd import paged
+
+    monkeypatch.setattr(paged, "_stream_of", lambda torch, dev, stream: 0)
+    made = []
+    batch._append = lambda *a: made.append(("append", a)) or 0
+    batch._attn = lambda *a: made.append(("attn", a)) or 0
+    batch._lib = types.SimpleNamespace(
+        csdr_paged_read=lambda *a: made.append(("read", a)) or 0,
+        csdr_paged_attn_workspace_bytes=lambda *a: made.append(("bytes", a)) or 0)
+    return made
+
+
+def test_no_tokens_is_no_call(batch, calls, monkeypatch):
+    """A scheduler's empty step: empty results, nothing launched."""
+    from cortexsdr_amd import logprobs
+
+    q, k = torch.zeros(0, 4, 64), torch.zeros(0, 2, 64)
+    start = torch.zeros(3, dtype=torch.int32)
+    assert batch.append(q, k, k, theta=1e4).shape == (0, 4, 64)
+    assert batch.append(q, k, k, q_start=start, max_q=0).shape == (0, 4, 64)
+    assert batch.append(None, k, k) is None
+    assert batch.attend(q).shape == (0, 4, 64)
+    assert batch.attend(q, q_start=start, max_q=0, out=q) is q
+    for t in batch.read(0):
+        assert t.shape == (0, 2, 64)
+    with pytest.raises(ValueError):
+        batch.attend(torch.zeros(0, 4, 32))  # still checked
+    assert not calls
+
+    monkeypatch.setattr(logprobs, "_torch", lambda: torch)
+    monkeypatch.setattr(logprobs, "_on_device", lambda torch, what, *ts: 0)
+    r = logprobs.token_logprobs(torch.zeros(0, 100), torch.zeros(0, dtype=torch.int32), top_n=3)
+    assert r.logprobs.shape == r.entropy.shape == (0,)
+    assert r.top_ids.shape == r.top_logprobs.shape == (0, 3)
+    assert logprobs.token_logprobs(torch.zeros(0, 100)).top_ids is None
