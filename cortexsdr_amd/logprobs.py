@@ -8,7 +8,7 @@ import typing
 
 from . import _lib
 from .hsdr import _check, _torch
-from .paged import _bytes, _dtype, _empty, _on_device, _stream_of
+from .paged import _bytes, _dtype, _empty, _int, _on_device, _stream_of
 
 
 class TokenLogprobs(typing.NamedTuple):
@@ -25,7 +25,7 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
     finite logits among the top. Without rows nothing is done. With `stream` the call runs and
     allocates there, ordered by the caller."""
     torch = _torch()
-    lib = _lib.load()
+    lib, top_n = _lib.load(), _int(top_n)
     dt = _dtype(logits)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be (rows, n) with a row's values side by side")
@@ -42,7 +42,7 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         workspace = _empty(torch, need, torch.uint8, dev, stream) if need else None
     lp, entropy = _empty(torch, (2, rows), torch.float32, dev, stream).unbind(0)
     ids = top = None
-    if top_n > 0:
+    if 0 < top_n <= 64:  # (else the library refuses it)
         ids = _empty(torch, (rows, top_n), torch.int32, dev, stream)
         top = _empty(torch, (rows, top_n), torch.float32, dev, stream)
     if tokens is None:
@@ -53,7 +53,7 @@ def token_logprobs(logits, tokens=None, top_n: int = 0, temperature: float = 1.0
         logits.data_ptr(), dt, rows, n, logits.stride(0) if rows > 1 else 0, temperature,
         tokens.data_ptr() if tokens is not None else None,
         lp.data_ptr() if lp is not None else None, entropy.data_ptr(), top_n,
-        ids.data_ptr() if top_n > 0 else None, top.data_ptr() if top_n > 0 else None,
+        ids.data_ptr() if ids is not None else None, top.data_ptr() if top is not None else None,
         workspace.data_ptr() if workspace is not None else None,
         _bytes(workspace) if workspace is not None else 0, _stream_of(torch, index, stream)))
     return TokenLogprobs(lp, entropy, ids, top)

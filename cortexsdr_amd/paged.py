@@ -78,6 +78,11 @@ def _empty(torch, shape, dtype, device, stream):
 _INT_MAX = 2 ** 31 - 1
 
 
+def _int(v) -> int:
+    """v as a C int holds it: past its ends the largest, or -1 (which the library refuses)."""
+    return max(-1, min(int(v), _INT_MAX))
+
+
 def _bytes(workspace) -> int:
     """What a caller's workspace holds: all of it has to be there (an expanded tensor's is not)."""
     if not workspace.is_contiguous():
@@ -100,8 +105,8 @@ class PagedCache:
         if kv_dtype not in KV_DTYPES:
             raise ValueError("kv_dtype must be 'f16' or 'q4'")
         self.page_bytes = int(_lib.load().csdr_paged_page_bytes(
-            KV_DTYPES[kv_dtype], page_size, n_kv_heads, head_dim))
-        if not self.page_bytes or n_pages <= 0:
+            KV_DTYPES[kv_dtype], _int(page_size), _int(n_kv_heads), _int(head_dim)))
+        if not self.page_bytes or not 0 < n_pages <= _INT_MAX:
             raise ValueError("page_size must be a power of two from 16 to 4096, head_dim 64 or "
                              "128, the numbers of pages and heads positive")
         self.n_pages, self.page_size = int(n_pages), int(page_size)
@@ -168,7 +173,7 @@ class PagedBatch:
         _ints(torch, "q_start", q_start, (self.n_seqs + 1,))
         if max_q is None:
             raise ValueError("q_start needs max_q, the most tokens of one sequence")
-        return q_start.data_ptr(), min(int(max_q), _INT_MAX)
+        return q_start.data_ptr(), _int(max_q)
 
     def _heads(self, what: str, t, n_heads=None):
         """The token stride of (tokens, heads, head_dim) or (tokens, heads * head_dim)."""
@@ -247,11 +252,11 @@ class PagedBatch:
                 raise ValueError("slopes must be a contiguous float32 tensor, one per head")
             if prefix is not None:
                 _ints(torch, "prefix", prefix, (self.n_seqs,))
-            opt = C.byref(_lib.AttnOptions(softcap, min(window, _INT_MAX),
+            opt = C.byref(_lib.AttnOptions(softcap, _int(window),
                                            slopes.data_ptr() if slopes is not None else None,
                                            prefix.data_ptr() if prefix is not None else None))
         starts, mq = self._starts(torch, q_start, max_q)
-        max_len = min(max_len, _INT_MAX)
+        max_len = _int(max_len)
         dev = self._here(torch, q, out, q_start, slopes, prefix, workspace)
         if n == 0:
             return out
@@ -277,8 +282,8 @@ class PagedBatch:
                         max_len: int = 0) -> int:
         """Bytes of attend's workspace, for callers that keep one."""
         starts, mq = self._starts(_torch(), q_start, max_q)
-        return int(self._lib.csdr_paged_attn_workspace_bytes(self._ref, n_tokens, starts, mq,
-                                                            n_heads, min(max_len, _INT_MAX)))
+        return int(self._lib.csdr_paged_attn_workspace_bytes(
+            self._ref, _int(n_tokens), starts, mq, _int(n_heads), _int(max_len)))
 
     def read(self, n_tokens: int, q_start=None, max_q=None, dtype: str = "f32", stream=None):
         """The cached keys and values of the sequences' last n_tokens rows (laid out as append's
