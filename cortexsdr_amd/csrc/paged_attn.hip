@@ -1320,7 +1320,7 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
                                                 int max_len) {
     PagedView pv;
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
-        Hq % kv->n_kv_heads || max_len < 0)
+        Hq > 65535 || Hq % kv->n_kv_heads || max_len < 0)
         return 0;
     return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len, 0, false));
 }

@@ -405,7 +405,8 @@ extern "C" {
 
 CSDR_API size_t csdr_paged_page_bytes(int kv_dtype, int page_size, int n_kv_heads, int head_dim) {
     if ((kv_dtype != CSDR_F16 && kv_dtype != CSDR_Q4) || page_size < 16 || page_size > 4096 ||
-        (page_size & (page_size - 1)) || n_kv_heads <= 0 || (head_dim != 64 && head_dim != 128))
+        (page_size & (page_size - 1)) || n_kv_heads <= 0 || n_kv_heads > 65535 ||
+        (head_dim != 64 && head_dim != 128))
         return 0;
     return (size_t)n_kv_heads * csdr::paged_head_bytes(kv_dtype == CSDR_Q4, page_size, head_dim);
 }

@@ -34,3 +34,15 @@ def test_the_workspace_function_is_enough(tokens, window):
                                                        0, 4, 0)
     assert need >= bytes_of(tokens, 8)
     assert refuses(bytes_of(tokens, 2) - 1, tokens, window=window)
+
+
+def test_page_bytes_of_more_heads_than_a_cache_has():
+    """A shape that no call takes has no size."""
+    f = _lib.load().csdr_paged_page_bytes
+    assert f(1, 16, 65535, 64) > 0 and f(1, 16, 65536, 64) == 0 and f(2, 4096, 2 ** 31 - 1, 128) == 0
+
+
+@pytest.mark.parametrize("heads", [65536, 131070])
+def test_workspace_of_more_heads_than_a_call_has(heads):
+    f = _lib.load().csdr_paged_attn_workspace_bytes
+    assert f(kv(), 2, None, 0, heads, 0) == 0 and f(kv(), 2, None, 0, 65534, 0) > 0
