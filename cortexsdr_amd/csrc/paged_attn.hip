@@ -87,7 +87,8 @@ __device__ __forceinline__ float shaped(const AttnArgs& a, float s, float slope,
 }
 
 // One row (token, head) by one wave, position by position: lanes over 64 positions for the scores,
-// over the dims for the values. Nothing of an unseen position is used.
+// over the dims for the values. Nothing of an unseen position is used. (The sum is 0 for a row that
+// sees nothing, and for one whose scores are all -infinity: zeros and NaN.)
 template <int HD, bool Q4, typename XT>
 __device__ void attend_row(const AttnArgs& a, int b, const SeqRows& r, int t, int h) {
     const PagedView& pv = a.pv;
@@ -99,12 +100,14 @@ __device__ void attend_row(const AttnArgs& a, int b, const SeqRows& r, int t, in
     const XT* q = static_cast<const XT*>(a.q) + row * a.q_stride + (long long)h * HD;
     const float slope = a.slopes ? a.slopes[h] : 0.0f;
     float m = -INFINITY, l = 0.0f, o[HD / 64] = {};
+    bool sees = false;
     const int end = pq < 0 ? 0 : max(min(pq + 1, seen.keys), min(seen.prefix, seen.keys));
     for (int p0 = 0; p0 < end; p0 += 64) {
         const int p = p0 + lane;
         const int page = seen.at(pq, p) ? csdr::page_of(pv, b, p) : -1;
         const uint64_t live = __ballot(page >= 0);
         if (!live) continue;
+        sees = true;
         float s = -INFINITY;
         if (page >= 0) {
             const uint8_t* kp = pv.k + csdr::head_offset<Q4>(pv, HD, page, kvh);
@@ -134,7 +137,7 @@ __device__ void attend_row(const AttnArgs& a, int b, const SeqRows& r, int t, in
     }
     XT* out = static_cast<XT*>(a.out) + (row * a.hq + h) * HD;
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (XT)(l == 0.0f ? 0.0f : o[c] / l);
+    for (int c = 0; c < HD / 64; ++c) out[lane + 64 * c] = (XT)(sees ? o[c] / l : 0.0f);
 }
 
 // ---------------------------------------------------------------- few tokens: split positions

@@ -621,8 +621,9 @@ typedef struct csdr_attn_options {
 /* out (n_tokens x Hq x head_dim, of dtype) = softmax attention of the tokens (rotated queries q,
  * as csdr_paged_append writes them) to the positions of their sequences that they see, after the
  * call's tokens were appended; GQA as repeat_kv_heads (cortex_sdk.cpp:1453-1478); scale 0 =
- * 1/sqrt(head_dim); out must not overlap q. A row that sees nothing is zero. What a token does not
- * see has no influence on it, NaN and infinities included. q_stride as above. max_len (host): at least the largest
+ * 1/sqrt(head_dim); out must not overlap q. A row that sees nothing is zero (one that sees only
+ * scores of -infinity NaN). What a token does not see has no influence on it, NaN and infinities
+ * included. q_stride as above. max_len (host): at least the largest
  * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
  * right, with less parallelism). One kernel serves a whole call, chosen by the most (token, query
  * head) pairs of a sequence and KV head: up to 64 take the form for single tokens, so sequences
