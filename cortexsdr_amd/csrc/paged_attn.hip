@@ -869,12 +869,13 @@ prompt_kernel(AttnArgs a, Splits sp) {
     // (sequence, KV head) fastest: on a chip of 8 dies that take workgroups in turn, the blocks of
     // one KV head meet in one L2 where there are 8 (or a multiple) of them. Latest columns, which
     // see most, first; where a CU takes two workgroups, the second 256 in the opposite order, so
-    // that a CU with the longest of the first has the shortest of the second (4096 tokens: 182 ->
-    // 175 us).
+    // that a CU with the longest of the first has the shortest of the second (14 heads of 64, two
+    // prompts of 4096 tokens: 111 -> 106 us, one of 8192: 215 -> 203). Where it takes three, that
+    // gains nothing (32 heads of 128, 4096 tokens: 167 and 168, 8192: 567 and 572).
     const int pairs = pv.n_seqs * pv.hkv, blocks = gridDim.x / pairs;
     const int bh = blockIdx.x % pairs, around = max(1, 256 / pairs);
     int rank = blockIdx.x / pairs;
-    if (NW == 4 && rank >= around && rank < min(2 * around, blocks))
+    if (NW == 4 && Shape::kSimdWaves == 2 && rank >= around && rank < min(2 * around, blocks))
         rank = around + min(2 * around, blocks) - 1 - rank;
     const int block = blocks - 1 - rank;
     const int b = bh / pv.hkv, kvh = bh % pv.hkv, split = blockIdx.y;
