@@ -1212,9 +1212,12 @@ constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
 constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
 // Splits of the positions: for step_kernel 768 workgroups in all (the three that a CU holds at
-// once), or twice as many where sequences may differ in length (one sequence of 131071 on 4-bit
-// pages: 768 50 us, 1536 57; 64 sequences of 4096 to 8192: 148 and 139), 128 positions (a tile per
-// wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for that, 512
+// once), or 1536, which even out sequences of different lengths, where there is work enough for
+// their joins: 2^21 positions of a head and 16 columns on 4-bit pages, 2^20 on fp16 ones (heads of
+// 128, 768 and 1536 workgroups: 4-bit pages, 2^20 positions 26.9 and 30.4, 38.1 and 39.6 us, 2^21
+// 66.5 and 61.5, 71.1 and 64.3, 64.9 and 62.8; fp16 pages, 2^18 positions 23.8 and 24.1, 15.4 and
+// 16.6, 2^20 79.6 and 78.5, 87.9 and 90.2, 2^21 154.8 and 156.5, 155.7 and 154.2),
+// 128 positions (a tile per wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for that, 512
 // positions at least. A sequence's positions are shared out equally, so a call with
 // sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
 // ever makes fewer splits; beside a prefix, whose length is device memory, no fewer than 4096
@@ -1223,7 +1226,7 @@ constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt
 // splits 0 to 2 us more).
 constexpr long long kPrefixSeen = 4096;
 
-Splits splits_of(const PagedView& pv, int hq, int max_len, int window, bool prefix) {
+Splits splits_of(const PagedView& pv, bool q4, int hq, int max_len, int window, bool prefix) {
     const int G = hq / pv.hkv;
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
@@ -1231,7 +1234,8 @@ Splits splits_of(const PagedView& pv, int hq, int max_len, int window, bool pref
     const bool step = cols <= kStepColumns;
     const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
-    const long long target = !step ? kPromptBlocks : pv.n_seqs == 1 ? 768 : 1536;
+    const long long target =
+        !step ? kPromptBlocks : (double)wgs * (double)len < (q4 ? 0x1p21 : 0x1p20) ? 768 : 1536;
     // (a block's columns see a window each, and two tiles more where these do not fall on tiles)
     long long seen = window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
     if (prefix) seen = std::max(seen, std::min(len, kPrefixSeen));
@@ -1326,7 +1330,7 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
         Hq > 65535 || Hq % kv->n_kv_heads || max_len < 0)
         return 0;
-    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, Hq, max_len, 0, false));
+    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, kv->kv_dtype == CSDR_Q4, Hq, max_len, 0, false));
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
@@ -1365,7 +1369,8 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.q = q;
     a.out = out;
     a.hq = Hq;
-    Splits s = splits_of(a.pv, Hq, max_len, a.window, a.prefix != nullptr);
+    const bool q4 = kv->kv_dtype == CSDR_Q4;
+    Splits s = splits_of(a.pv, q4, Hq, max_len, a.window, a.prefix != nullptr);
     // fewer than 2^32 threads a launch: workgroups of at most 256 (prompt_kernel: two threads a
     // column, except where it has few), join_kernel's only where there is one
     const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);
@@ -1379,7 +1384,6 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     s.stats = static_cast<float*>(workspace);
     s.vecs = s.stats + csdr::align_up((size_t)n_tokens * Hq * s.n * 2, 4);
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const bool q4 = kv->kv_dtype == CSDR_Q4;
     if (hd == 64) {
         if (q4) launch<64, true>(a, dtype, s, st);
         else launch<64, false>(a, dtype, s, st);
