@@ -411,6 +411,7 @@ __device__ __forceinline__ float load_query(const AttnArgs& a, const XT* qp, int
 }
 
 struct Splits {
+    bool step;     // step_kernel, else prompt_kernel
     int n;         // of the tiles that a workgroup's columns see
     float* stats;  // 2 per (row, head, split): exponent offset and sum
     float* vecs;   // HD per (row, head, split)
@@ -1206,8 +1207,23 @@ prompt_kernel(AttnArgs a, Splits sp) {
     }
 }
 
-// Up to this many columns of a KV head go to step_kernel (16 at a time), more to prompt_kernel.
-constexpr int kStepColumns = 64;
+// Whether step_kernel takes the columns of a KV head, 16 at a time, or prompt_kernel all. A second
+// block of 16 reads the pages once more, which on fp16 pages pays while that is little: up to 128 MB
+// in all (17 to 64 columns, step and prompt: 20 MB 13.6 and 12.9 us, 39 MB 15.3 and 19.9, 14.9 and
+// 18.5, 79 MB 20.4 and 21.6, 118 MB 21.6 both, 17.6 and 21.1, 157 MB 27.3 and 24.3, 21.5 and 23.1,
+// 1.26 GB 279 and 104). On 4-bit pages, which prompt_kernel unpacks for 128 columns at once or more, it pays up
+// to 64 columns (32: 18.5 and 39.3, 57 and 100; 64: 24 and 39, 92.6 and 108; but short sequences
+// that are many, 16 of 300 positions: 49 and 29), and from 1024 positions on up to 128 (80: 25.8 and
+// 41.0, 86 and 182; 128: 31 and 41, 144 and 183, 155 and 169; 300 positions 13 and 25, or 85 and 54).
+bool takes_step(const PagedView& pv, bool q4, int hd, long long cols, long long len) {
+    if (cols <= kCols) return true;
+    if (q4)  // (the last: more would be too many for its join)
+        return cols <= 64 ||
+               (cols <= 128 && len > 1024 && (long long)pv.n_seqs * pv.max_q < 1LL << 24);
+    const double blocks = (double)pv.n_seqs * pv.hkv * (double)((cols + kCols - 1) / kCols);
+    return cols <= 64 && blocks * (double)len * (4 * hd) <= 128e6;
+}
+
 constexpr long long kPromptBlocks = 512;  // two workgroups to a CU
 constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt_kernel
 
@@ -1226,12 +1242,14 @@ constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt
 // splits 0 to 2 us more).
 constexpr long long kPrefixSeen = 4096;
 
-Splits splits_of(const PagedView& pv, bool q4, int hq, int max_len, int window, bool prefix) {
+Splits splits_of(const PagedView& pv, const csdr_paged_kv& kv, int hq, int max_len, int window,
+                 bool prefix) {
+    const bool q4 = kv.kv_dtype == CSDR_Q4;
     const int G = hq / pv.hkv;
     const long long len =
         std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
     const long long cols = (long long)pv.max_q * G;
-    const bool step = cols <= kStepColumns;
+    const bool step = takes_step(pv, q4, kv.head_dim, cols, len);
     const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
     const long long target =
@@ -1240,18 +1258,17 @@ Splits splits_of(const PagedView& pv, bool q4, int hq, int max_len, int window, 
     long long seen = window > 0 ? std::min(len, window + std::min(cols, per) / G + 2 * 64) : len;
     if (prefix) seen = std::max(seen, std::min(len, kPrefixSeen));
     Splits s{};
+    s.step = step;
     s.n = (int)std::max(1LL, std::min((seen + unit - 1) / unit,
                                       step ? (target + wgs - 1) / wgs : target / wgs));
     return s;
 }
 
 // A call of prompt_kernel without splits needs none.
-bool one_launch(const PagedView& pv, int hq, const Splits& s) {
-    return (long long)pv.max_q * (hq / pv.hkv) > kStepColumns && s.n == 1;
-}
+bool one_launch(const Splits& s) { return !s.step && s.n == 1; }
 
 size_t workspace_of(const PagedView& pv, int hq, int hd, const Splits& s) {
-    if (one_launch(pv, hq, s)) return 0;
+    if (one_launch(s)) return 0;
     const size_t parts = (size_t)pv.n_tokens * hq * s.n;
     return csdr::align_up(parts * 8, 16) + parts * hd * 4;
 }
@@ -1292,7 +1309,7 @@ void launch_prompt(const AttnArgs& a, const Splits& s, hipStream_t st) {
 template <int HD, bool Q4, typename XT, bool OPTS>
 void launch_kernel(const AttnArgs& a, const Splits& s, hipStream_t st) {
     const int cols = a.pv.max_q * (a.hq / a.pv.hkv);
-    if (cols > kStepColumns) {
+    if (!s.step) {
         const long long columns = PromptConfig<HD, Q4, XT, false>::Shape::kColumns;
         if ((long long)a.pv.n_seqs * a.pv.hkv * cols < kPromptBlocks * columns)
             launch_prompt<HD, Q4, XT, OPTS, true>(a, s, st);
@@ -1330,7 +1347,7 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
         Hq > 65535 || Hq % kv->n_kv_heads || max_len < 0)
         return 0;
-    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, kv->kv_dtype == CSDR_Q4, Hq, max_len, 0, false));
+    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, *kv, Hq, max_len, 0, false));
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
@@ -1370,12 +1387,12 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.out = out;
     a.hq = Hq;
     const bool q4 = kv->kv_dtype == CSDR_Q4;
-    Splits s = splits_of(a.pv, q4, Hq, max_len, a.window, a.prefix != nullptr);
+    Splits s = splits_of(a.pv, *kv, Hq, max_len, a.window, a.prefix != nullptr);
     // fewer than 2^32 threads a launch: workgroups of at most 256 (prompt_kernel: two threads a
-    // column, except where it has few), join_kernel's only where there is one
+    // column, except where it has few), join_kernel's where there may be one
     const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);
     if ((long long)kv->n_seqs * kv->n_kv_heads * ((cols + 127) / 128) >= 1LL << 24 ||
-        (!one_launch(a.pv, Hq, s) && (long long)kv->n_seqs * a.pv.max_q >= 1LL << 24))
+        ((!one_launch(s) || cols <= 64) && (long long)kv->n_seqs * a.pv.max_q >= 1LL << 24))
         return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");
     const size_t need = workspace_of(a.pv, Hq, hd, s);
     if (need && (!workspace || workspace_bytes < need ||

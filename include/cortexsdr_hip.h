@@ -626,8 +626,9 @@ typedef struct csdr_attn_options {
  * included. q_stride as above. max_len (host): at least the largest
  * lens[b], 0 for the table's capacity; it only sizes the launch (longer sequences are still
  * right, with less parallelism). One kernel serves a whole call, chosen by the most (token, query
- * head) pairs of a sequence and KV head: up to 64 take the form for single tokens, so sequences
- * with a token each are better off in a call of their own than beside a prompt.
+ * head) pairs of a sequence and KV head: up to 16 take the form for single tokens, more than 128
+ * that for prompts, and between the cache's format and max_len decide; so sequences with a token
+ * each are better off in a call of their own than beside a prompt.
  *
  * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
  * CSDR_F16: fp32 sums of weights rounded to fp16 once, or in pairs too in the form for single

@@ -106,3 +106,25 @@ def test_captured_prompts(gpu, kv, x):
             row += c
     want = s.expect(qd[:m].cpu().numpy(), part)
     assert rel_l2(out[:m].cpu().numpy(), want) <= tol(x)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4"])
+@pytest.mark.parametrize("x", ["f32", "f16"])
+@pytest.mark.parametrize("heads,tokens", [
+    ("three", 6), ("three", 21), ("three", 30), ("three", 42), ("gqa", 5), ("gqa", 16), ("gqa", 17),
+    ("gqa", 32), ("llama", 18), ("llama", 64), ("llama", 128), ("qwen", 18), ("many", 3),
+])
+def test_both_forms_for_few_tokens(gpu, kv, x, heads, tokens):
+    """17 to 128 pairs of token and query head: the bound of the lengths, here a table's capacity,
+    decides between the kernels; either is right."""
+    s = Setup(gpu, [150 + tokens, 40 + tokens], HEADS[heads], kv, x, ps=16, seed=64)
+    s.append([150, 40], with_q=False)
+    qd, _ = s.append([tokens, tokens])
+    wide = gpu.full((2, 65536), -1, dtype=gpu.int32, device="cuda")
+    wide[:, :s.table.shape[1]] = s.table
+    far = s.cache.batch(wide, s.lens)
+    prefix = gpu.tensor([3, 170], dtype=gpu.int32, device="cuda")
+    for a, e in (({}, {}), (dict(window=50, prefix=prefix), dict(window=50, prefix=[3, 170]))):
+        want = s.expect(qd.cpu().numpy(), [tokens, tokens], **e)
+        for batch, n in ((s.batch, 0), (far, 0), (far, 200), (far, 5000)):
+            assert rel_l2(batch.attend(qd, max_len=n, **a).cpu().numpy(), want) <= tol(x)
