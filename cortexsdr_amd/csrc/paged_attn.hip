@@ -144,7 +144,6 @@ __device__ void attend_row(const AttnArgs& a, int b, const SeqRows& r, int t, in
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -431,7 +430,8 @@ struct Splits {
 // 4-bit pages round weights, and sum what they rounded (so that constant values come back).
 // fp16 pages: bound by their stream (32 sequences, fp16 calls: 81 us, 4.7 TB/s). 4 bits: by vector
 // instructions, about 450 beside 39 matrix ones a tile (64 sequences of 4096 to 8192, fp32 calls:
-// 143 us, 3.4 TB/s; one of 131071, fp16 calls: 48.5 us).
+// 137 to 143 us, 3.5 TB/s; one of 131071, fp16 calls: 47 us); with fewer than 16 query heads to a KV
+// head and a token each, the columns past them repeat the last one, and that work with them.
 template <int HD, bool Q4, typename XT, bool OPTS>
 __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Splits sp) {
     constexpr bool PAIR = sizeof(XT) == 4, WPAIR = PAIR || !Q4;  // queries, weights
@@ -496,8 +496,8 @@ __global__ __launch_bounds__(64 * kStepWaves, 3) void step_kernel(AttnArgs a, Sp
     const LaneOffsets<HD, Q4> at(pv, lane);
     Tile<HD, Q4> t;
     // One tile at tb (pages pg0, pg1); with MORE, the loads of the next one (nb, ng0, ng1) are
-    // issued as soon as its registers are free. (The last tile is code of its own: a loop whose
-    // loads and exit hang on one condition was compiled with registers of the tile overwritten.)
+    // issued as soon as its registers are free. (The last tile, which has no next one, is code of
+    // its own.)
     auto tile = [&](auto more, int tb, int pg0, int pg1, int nb, int ng0, int ng1) {
         constexpr bool MORE = decltype(more)::value;
         // the lane's positions that its column sees; whole tiles need no mask
@@ -832,8 +832,9 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // values by the threads, in two planes: value = hi + lo to 22 bits, and products hi hi, lo hi and
 // for fp32 calls hi lo. (One plane, values rounded to 11 bits, would do with half the products for
 // fp16 calls, but left them 2.2 times as far off as the rounding of their outputs alone.)
-// Bound by matrix and vector instructions in turn: 4096 tokens on fp16 pages, fp16 calls, 158 us,
-// 861 TFLOP/s; prompts on 4-bit pages, fp32 calls, 603 us, 261 TFLOP/s, three products for each.
+// Bound by matrix and vector instructions in turn: 4096 tokens on fp16 pages, fp16 calls, 159 to
+// 168 us from card to card, 820 to 865 TFLOP/s (fp32 calls 269); prompts on 4-bit pages, fp32 calls,
+// 598 us, 263 TFLOP/s, three products for each (fp16 calls 461, two).
 template <int HD, bool Q4, typename XT, int NQ, int NW>
 struct PromptShape {
     static constexpr bool kPair = sizeof(XT) == 4;
@@ -1060,7 +1061,7 @@ prompt_kernel(AttnArgs a, Splits sp) {
             clear(tb, buf, pg);
             __syncthreads();
         }
-        if (Q4 || i + 1 < hi) {  // (4 bits: the last tile again, so that the registers are set)
+        if (Q4 || i + 1 < hi) {  // (4 bits: the last tile again, which nobody reads)
             const int nb = tiles.at(min(i + 1, hi - 1));
             pages_at(nb, pg);
             fetch(nb, buf ^ 1, pg);
