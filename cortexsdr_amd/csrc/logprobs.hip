@@ -6,8 +6,8 @@
 // (Differences first: x / temperature alone may be past fp32 where d is not.)
 // The order of the top: larger x first, among equals the lower id.
 //
-// Bound by the read of the logits: 2048 rows of 151936 fp32 with the top 5 take 233 us, 5.3 TB/s; of
-// fp16 196 us, 3.2 TB/s, since a value's vector work stays.
+// Bound by the read of the logits: 2048 rows of 151936 fp32 with the top 5 take 233 us, 5.3 TB/s
+// (of fp16 196 us, 3.2 TB/s, since a value's vector work stays).
 // segment_kernel reads them once: a wave takes a segment of a row in rounds of 2048 values that
 // stay in registers, the next round's loads issued before the current one is worked on. Per round:
 // the maximum, then the two sums about the running maximum; for the top, values that beat the

@@ -17,9 +17,9 @@
 // positions, aligned to 8: the unit in which V's pages are laid out, so that one thread writes all
 // of a word or piece that the block's tokens share, and no two threads of a call write one word.
 //
-// Bound by memory: 5751 fp32 tokens of 32 + 2 x 8 heads of 128 take 43 us into fp16 pages, 6.0 TB/s,
-// and 58 into 4-bit ones, 4.2 TB/s (243 MB, and the codes' work beside them); a step's tokens are one
-// round trip (64 sequences 5 us, one 3). The read of their rows as fp16 takes 10 and 12 us where 47
+// Bound by memory: 5751 fp32 tokens of 32 + 2 x 8 heads of 128 take 43 us into fp16 pages, 6.0
+// TB/s, and 58 into 4-bit ones, 4.2 TB/s (243 MB, and the codes' work beside them); a step's tokens
+// are one round trip (64 sequences 5 us, one 3). The read of their rows as fp16 takes 10 and 12 us where 47
 // and 31 MB are 9 and 6: a lane stores 4 bytes a row, and on 4-bit pages four lanes share a word.
 #include <hip/hip_runtime.h>
 
