@@ -80,7 +80,7 @@ _INT_MAX = 2 ** 31 - 1
 
 def _int(v) -> int:
     """v as a C int holds it: past its ends the largest, or -1 (which the library refuses)."""
-    return max(-1, min(int(v), _INT_MAX))
+    return v if 0 <= v <= _INT_MAX else -1 if v < 0 else _INT_MAX
 
 
 def _bytes(workspace) -> int:
@@ -173,7 +173,7 @@ class PagedBatch:
         _ints(torch, "q_start", q_start, (self.n_seqs + 1,))
         if max_q is None:
             raise ValueError("q_start needs max_q, the most tokens of one sequence")
-        return q_start.data_ptr(), _int(max_q)
+        return q_start.data_ptr(), _int(int(max_q))
 
     def _heads(self, what: str, t, n_heads=None):
         """The token stride of (tokens, heads, head_dim) or (tokens, heads * head_dim)."""

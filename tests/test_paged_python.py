@@ -71,6 +71,13 @@ def test_no_tokens_is_no_call(batch, calls, monkeypatch):
     assert logprobs.token_logprobs(torch.zeros(0, 100)).top_ids is None
 
 
+def test_most_of_the_tokens_as_a_tensor(batch, calls):
+    """max_q as what the caller's own arithmetic left it in."""
+    q, start = torch.zeros(2, 4, 64), torch.tensor([0, 2, 2], dtype=torch.int32)
+    batch.attend(q, q_start=start, max_q=start.diff().max())
+    assert type(calls[-1][1][5]) is int and calls[-1][1][5] == 2
+
+
 FAR = -2 ** 32  # FAR + 5 is 5 to a C int
 
 
