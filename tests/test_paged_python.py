@@ -115,8 +115,9 @@ def test_cache_shapes_past_an_int(monkeypatch, over):
 @pytest.mark.parametrize("top_n", [2 ** 32 + 3, 2 ** 31, 65, -1, FAR + 3])
 def test_more_places_than_the_top_has(monkeypatch, top_n):
     """Refused by the library as it is, without a list of that length first."""
-    from cortexsdr_amd import _lib, logprobs
+    from cortexsdr_amd import _lib, logprobs, paged
 
+    monkeypatch.setattr(paged, "_torch", lambda: torch)
     monkeypatch.setattr(logprobs, "_torch", lambda: torch)
     monkeypatch.setattr(logprobs, "_on_device", lambda torch, what, *ts: 0)
     monkeypatch.setattr(logprobs, "_stream_of", lambda torch, dev, stream: 0)
