@@ -1212,10 +1212,11 @@ prompt_kernel(AttnArgs a, Splits sp) {
 // block of 16 reads the pages once more, which on fp16 pages pays while that is little: up to 128 MB
 // in all (17 to 64 columns, step and prompt: 20 MB 13.6 and 12.9 us, 39 MB 15.3 and 19.9, 14.9 and
 // 18.5, 79 MB 20.4 and 21.6, 118 MB 21.6 both, 17.6 and 21.1, 157 MB 27.3 and 24.3, 21.5 and 23.1,
-// 1.26 GB 279 and 104). On 4-bit pages, which prompt_kernel unpacks for 128 columns at once or more, it pays up
-// to 64 columns (32: 18.5 and 39.3, 57 and 100; 64: 24 and 39, 92.6 and 108; but short sequences
-// that are many, 16 of 300 positions: 49 and 29), and from 1024 positions on up to 128 (80: 25.8 and
-// 41.0, 86 and 182; 128: 31 and 41, 144 and 183, 155 and 169; 300 positions 13 and 25, or 85 and 54).
+// 1.26 GB 279 and 104). On 4-bit pages, which prompt_kernel unpacks for 128 columns at once or
+// more, it pays up to 64 columns (32: 18.5 and 39.3, 57 and 100; 64: 24 and 39, 92.6 and 108; but
+// short sequences that are many, 16 of 300 positions: 49 and 29), and from 1024 positions on up to
+// 128 (80: 25.8 and 41.0, 86 and 182; 128: 31 and 41, 144 and 183, 170 and 155; 300 positions 13 and
+// 25, or 85 and 54).
 bool takes_step(const PagedView& pv, bool q4, int hd, long long cols, long long len) {
     if (cols <= kCols) return true;
     if (q4)  // (the last: more would be too many for its join)
@@ -1234,23 +1235,19 @@ constexpr int kSmallColumns = 64;         // of the smallest workgroup of prompt
 // 128, 768 and 1536 workgroups: 4-bit pages, 2^20 positions 26.9 and 30.4, 38.1 and 39.6 us, 2^21
 // 66.5 and 61.5, 71.1 and 64.3, 64.9 and 62.8; fp16 pages, 2^18 positions 23.8 and 24.1, 15.4 and
 // 16.6, 2^20 79.6 and 78.5, 87.9 and 90.2, 2^21 154.8 and 156.5, 155.7 and 154.2),
-// 128 positions (a tile per wave) each at least; for prompt_kernel one if there are 512 workgroups, else enough for that, 512
-// positions at least. A sequence's positions are shared out equally, so a call with
-// sequences of different lengths, or of lengths far below the bound, stays balanced. A window only
-// ever makes fewer splits; beside a prefix, whose length is device memory, no fewer than 4096
+// 128 positions (a tile per wave) each at least; for prompt_kernel one if there are 512 workgroups,
+// else enough for that, 512 positions at least. A sequence's positions are shared out equally, so a
+// call with sequences of different lengths, or of lengths far below the bound, stays balanced. A
+// window, or a smaller bound, only ever makes fewer splits; beside a prefix, whose length is device memory, no fewer than 4096
 // positions have (one sequence, a window of 256 and a prefix of 32000: 80 -> 26 us, 128 tokens of
 // one: 259 -> 122; a window of 1024 and a prefix of 4: 14 us either way, but for all of the length's
 // splits 0 to 2 us more).
 constexpr long long kPrefixSeen = 4096;
 
-Splits splits_of(const PagedView& pv, const csdr_paged_kv& kv, int hq, int max_len, int window,
+Splits splits_of(const PagedView& pv, bool q4, int hq, bool step, long long len, int window,
                  bool prefix) {
-    const bool q4 = kv.kv_dtype == CSDR_Q4;
     const int G = hq / pv.hkv;
-    const long long len =
-        std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
     const long long cols = (long long)pv.max_q * G;
-    const bool step = takes_step(pv, q4, kv.head_dim, cols, len);
     const long long per = step ? kCols : kSmallColumns, unit = step ? kTile * kStepWaves : 512;
     const long long wgs = (long long)pv.n_seqs * pv.hkv * ((cols + per - 1) / per);
     const long long target =
@@ -1263,6 +1260,10 @@ Splits splits_of(const PagedView& pv, const csdr_paged_kv& kv, int hq, int max_l
     s.n = (int)std::max(1LL, std::min((seen + unit - 1) / unit,
                                       step ? (target + wgs - 1) / wgs : target / wgs));
     return s;
+}
+
+long long bound_of(const PagedView& pv, int max_len) {
+    return std::max(1, max_len > 0 ? std::min(max_len, pv.capacity()) : pv.capacity());
 }
 
 // A call of prompt_kernel without splits needs none.
@@ -1348,7 +1349,16 @@ CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_t
     if (csdr::paged_check("paged_attn", kv, n_tokens, q_start, max_q, &pv) != CSDR_OK || Hq <= 0 ||
         Hq > 65535 || Hq % kv->n_kv_heads || max_len < 0)
         return 0;
-    return workspace_of(pv, Hq, kv->head_dim, splits_of(pv, *kv, Hq, max_len, 0, false));
+    // (a smaller bound, which may choose the other kernel, needs no more)
+    const bool q4 = kv->kv_dtype == CSDR_Q4;
+    const long long cols = (long long)pv.max_q * (Hq / kv->n_kv_heads), len = bound_of(pv, max_len);
+    size_t need = 0;
+    if (takes_step(pv, q4, kv->head_dim, cols, 1) || takes_step(pv, q4, kv->head_dim, cols, len))
+        need = workspace_of(pv, Hq, kv->head_dim, splits_of(pv, q4, Hq, true, len, 0, false));
+    if (!takes_step(pv, q4, kv->head_dim, cols, 1) || !takes_step(pv, q4, kv->head_dim, cols, len))
+        need = std::max(need, workspace_of(pv, Hq, kv->head_dim,
+                                           splits_of(pv, q4, Hq, false, len, 0, false)));
+    return need;
 }
 
 CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, int n_tokens,
@@ -1388,10 +1398,12 @@ CSDR_API int csdr_paged_attn(const csdr_paged_kv* kv, const void* q, int dtype, 
     a.out = out;
     a.hq = Hq;
     const bool q4 = kv->kv_dtype == CSDR_Q4;
-    Splits s = splits_of(a.pv, *kv, Hq, max_len, a.window, a.prefix != nullptr);
+    const long long len = bound_of(a.pv, max_len);
+    const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);
+    Splits s = splits_of(a.pv, q4, Hq, takes_step(a.pv, q4, hd, cols, len), len, a.window,
+                         a.prefix != nullptr);
     // fewer than 2^32 threads a launch: workgroups of at most 256 (prompt_kernel: two threads a
     // column, except where it has few), join_kernel's where there may be one
-    const long long cols = (long long)a.pv.max_q * (Hq / kv->n_kv_heads);
     if ((long long)kv->n_seqs * kv->n_kv_heads * ((cols + 127) / 128) >= 1LL << 24 ||
         ((!one_launch(s) || cols <= 64) && (long long)kv->n_seqs * a.pv.max_q >= 1LL << 24))
         return set_error(CSDR_E_INVALID, "paged_attn: too many tokens");

@@ -47,3 +47,18 @@ def test_workspace_of_more_heads_than_a_call_has(heads):
     f = _lib.load().csdr_paged_attn_workspace_bytes
     wide = kv(n_kv_heads=32768)
     assert f(wide, 2, None, 0, heads, 0) == 0 and f(wide, 2, None, 0, 32768, 0) > 0
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("n_seqs", [1, 8, 256])
+@pytest.mark.parametrize("tokens", [1, 8, 20, 32, 50, 64, 100])
+def test_a_workspace_for_the_table_is_enough_for_less(dtype, n_seqs, tokens):
+    """What is asked for without a bound of the lengths does for every bound (which may choose
+    another kernel)."""
+    f = _lib.load().csdr_paged_attn_workspace_bytes
+    for stride in (4, 64, 4096):
+        c = kv(kv_dtype=dtype, n_seqs=n_seqs, table_stride=stride)
+        n = n_seqs * tokens
+        most = f(c, n, None, 0, 4, 0)
+        for bound in (1, 16, 300, 1024, 1025, 5000, 40000, 65536):
+            assert f(c, n, None, 0, 4, bound) <= most, (stride, bound)
