@@ -633,8 +633,9 @@ typedef struct csdr_attn_options {
  * CSDR_F32: products of fp32 quality (queries and softmax weights in pairs of fp16, fp32 sums);
  * CSDR_F16: fp32 sums of weights rounded to fp16 once, or in pairs too in the form for single
  * tokens on fp16 pages. workspace:
- * csdr_paged_attn_workspace_bytes (may be 0) device bytes, 16-byte aligned, needed by this call
- * only: calls that may run at the same time need one each. */
+ * csdr_paged_attn_workspace_bytes (may be 0; enough for any options and any smaller max_len) device
+ * bytes, 16-byte aligned, needed by this call only: calls that may run at the same time need one
+ * each. */
 CSDR_API size_t csdr_paged_attn_workspace_bytes(const csdr_paged_kv* kv, int n_tokens,
                                                 const int32_t* q_start, int max_q, int Hq,
                                                 int max_len);
