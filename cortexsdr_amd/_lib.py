@@ -291,6 +291,15 @@ SIGNATURES.update({
     "csdr_token_logprobs_workspace_bytes": (_sz, [C.c_int, C.c_int, C.c_int]),
     "csdr_token_logprobs": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, _i64, C.c_float, _vp, _vp,
                                       _vp, C.c_int, _vp, _vp, _vp, _sz, _vp]),
+    "csdr_q8_pitch": (_sz, [C.c_int]),
+    "csdr_q8_quantize": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _i64, _i64, _vp, _vp, _vp]),
+    "csdr_q8_dequantize": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp]),
+    "csdr_add_rms_norm": (C.c_int, [_vp, C.c_int, _i64, _vp, C.c_int, _i64, _vp, _vp, C.c_float,
+                                    C.c_int, C.c_int, _vp, _vp, _vp, _vp]),
+    "csdr_q8_linear": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, _vp, _vp, _i64, _vp,
+                                 C.c_int, _i64, _vp]),
+    "csdr_rotary": (C.c_int, [_vp, _vp, C.c_int, _i64, _i64, _vp, _vp, C.c_int, _i64, _i64, C.c_int,
+                              C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_float, _vp]),
 })
 
 

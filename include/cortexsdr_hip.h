@@ -669,6 +669,67 @@ CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
                                  void* hip_stream);
 
 /* ======================================================================
+ * A layer in 8 bits: rows of codes with a scale each, and their products
+ * ==================================================================== */
+
+/* A row of n values v as 8-bit codes: code = round(127 v / max|v|), ties to even, in exact arithmetic,
+ * scale = max|v| / 127 (fp32), a value being scale * code. A row of zeros has the scale 0; one that
+ * holds a value which is not finite, or whose scale passes fp32, the scale NaN and codes 0. Rows of codes
+ * lie csdr_q8_pitch(n) bytes apart (n up to a whole number of 128; 0 for an n outside 1..131071), zeros
+ * behind the last value, 16-byte aligned, with `rows` scales (device memory throughout). At most
+ * 2^22 - 1 rows. */
+CSDR_API size_t csdr_q8_pitch(int n);
+/* The rows of x, or of silu(gate) * x (silu_mul, cortex_sdk.cpp:1245-1256) if gate is not NULL: `rows`
+ * rows of n values of `dtype` (CSDR_F32 or CSDR_F16), x_stride and gate_stride elements apart (0 = n), so
+ * that gate and x may lie in one projection's output. A weight matrix so becomes codes with a scale per
+ * output channel. */
+CSDR_API int csdr_q8_quantize(const void* x, const void* gate, int dtype, int rows, int n,
+                              int64_t x_stride, int64_t gate_stride, int8_t* codes, float* scales,
+                              void* hip_stream);
+/* out (rows x n, packed, of dtype) = scale * code. */
+CSDR_API int csdr_q8_dequantize(const int8_t* codes, const float* scales, int rows, int n, void* out,
+                                int dtype, void* hip_stream);
+/* RMSNorm (rms_norm, cortex_sdk.cpp:1208-1232) with the residual's addition in front and 8-bit rows behind:
+ * h = x, or x + residual rounded to residual_dtype and written to residual_out (rows x n, packed; it may
+ * be residual itself where that is packed) if residual is not NULL; the norm h / sqrt(mean(h^2) + eps) * w
+ * goes to codes and scales (both or neither), to y (rows x n, packed, of x's dtype; may be NULL), or to
+ * both. Strides in elements, 0 = n. Outputs must not overlap inputs or each other otherwise. */
+CSDR_API int csdr_add_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual,
+                               int residual_dtype, int64_t residual_stride, void* residual_out,
+                               const float* w, float eps, int rows, int n, void* y, int8_t* codes,
+                               float* scales, void* hip_stream);
+/* y (M x R of y_dtype, rows y_stride elements apart, 0 = R) = x (M rows of C values) . w^T (R rows of C
+ * values), both as codes and scales, + bias (R floats, may be NULL) + add (M x R of y_dtype, rows
+ * add_stride apart; may be NULL, or y itself with y's stride): linear_forward's layout
+ * (blas_kernels.cpp:264-293). The sums of products of codes are exact; they are scaled and added to in
+ * fp32 and rounded once to y_dtype. y must not overlap an input but add. */
+CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const int8_t* x,
+                            const float* x_scales, int M, int C, const float* bias, const void* add,
+                            int64_t add_stride, void* y, int y_dtype, int64_t y_stride,
+                            void* hip_stream);
+
+/* ======================================================================
+ * Rotary positions
+ * ==================================================================== */
+
+/* Which dims make a pair: (2 j, 2 j + 1), or (j, j + dims / 2). */
+#define CSDR_ROTARY_ADJACENT 0
+#define CSDR_ROTARY_HALVES 1
+/* Heads of q and of k (may be NULL) turned at their tokens' positions (apply_rope_inplace,
+ * cortex_sdk.cpp:1395-1423, in the forms that csdr_paged_append, which appends such keys with theta 0, has
+ * not): pair j of a head's first `dims` dims (even) by positions[token] * turns[j] whole turns (dims / 2
+ * numbers in device memory, frequency / 2 pi, so that any scaling for long contexts is the caller's; formed
+ * and reduced in fp64), times magnitude; the other dims as they are. positions: n_tokens ints (device); a
+ * token with a negative one is none, its rows are not written. Strides in elements from one token to the
+ * next, 0 = heads x head_dim; q_out may be q, with q's stride, and k_out k; outputs must not overlap
+ * inputs otherwise. head_dim at most 1024. */
+CSDR_API int csdr_rotary(const void* q, void* q_out, int Hq, int64_t q_stride, int64_t q_out_stride,
+                         const void* k, void* k_out, int Hk, int64_t k_stride, int64_t k_out_stride,
+                         int dtype, int n_tokens, int head_dim, int dims, int layout,
+                         const int32_t* positions, const double* turns, float magnitude,
+                         void* hip_stream);
+
+/* ======================================================================
  * Containers: the .sdr archive, HSDC codes-only streams, the HSDA shared-dictionary archive
  * (host parsing; loads go to the current device)
  * ==================================================================== */
