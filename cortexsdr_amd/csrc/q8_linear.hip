@@ -4,8 +4,10 @@
 // a sum is converted to fp32, by two products and the additions in fp32, and once to y's type.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "q8.hpp"
 
@@ -24,22 +26,57 @@ struct Args {
     void* y;
     long long y_stride, add_stride;
     int R, M, pitch;
+    bool wide;  // four outputs at a multiple of four may be moved at once
 };
+
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+    typedef float type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Four<_Float16> {
+    typedef _Float16 type __attribute__((ext_vector_type(4)));
+};
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// The scales and biases of four neighbouring rows of w (the last one's again where there are fewer).
+__device__ __forceinline__ f4 four_of(const float* p, int r, int R) {
+    f4 v;
+    if (r + 3 < R) __builtin_memcpy(&v, p + r, 16);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = p[min(r + i, R - 1)];
+    return v;
+}
 
 // Four neighbouring outputs of a token, as many of them as there are.
 template <typename T>
-__device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& sum) {
+__device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
+                                       const f4& bias) {
     if (m >= a.M || r >= a.R) return;
-    const float xs = a.x_scales[m];
-    const int n = min(4, a.R - r);
+    using V = typename Four<T>::type;
     T* y = static_cast<T*>(a.y) + m * a.y_stride + r;
     const T* add = static_cast<const T*>(a.add) + m * a.add_stride + r;
-    for (int i = 0; i < n; ++i) {
-        float v = (float)sum[i] * xs * a.w_scales[r + i];
-        if (a.bias) v += a.bias[r + i];
-        if (a.add) v += csdr::to_f32(add[i]);
-        y[i] = (T)v;
+    f4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)sum[i] * xs * ws[i] + bias[i];
+    if (a.wide && r + 3 < a.R) {
+        if (a.add) {
+            const V u = *reinterpret_cast<const V*>(add);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += (float)u[i];
+        }
+        V o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
+        *reinterpret_cast<V*>(y) = o;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (r + i < a.R) y[i] = (T)(a.add ? v[i] + (float)add[i] : v[i]);
 }
 
 // 16 rows of w times 16 MT tokens; the waves take steps of 64 columns in turn and add up through LDS.
@@ -76,14 +113,185 @@ __global__ __launch_bounds__(WAVES * 64) void rows16_kernel(Args a) {
         i4 sum = part[0][j][l];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) sum += part[k][j][l];
-        finish<T>(a, m0 + 16 * j + (l & 15), r0 + 4 * (l >> 4), sum);
+        const int m = m0 + 16 * j + (l & 15), r = r0 + 4 * (l >> 4);
+        finish<T>(a, m, r, sum, a.x_scales[min(m, a.M - 1)], four_of(a.w_scales, r, a.R),
+                  a.bias ? four_of(a.bias, r, a.R) : f4{});
     }
+}
+
+// ------------------------------------------------------------------ tiles through LDS
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// TR rows of w times TM tokens a workgroup, in WR x WM waves. A step is 128 columns; its rows lie in LDS 128
+// bytes apart, 16-byte chunk c of row i at c ^ (i % 8), so that the 16 rows of an operand's chunk fall on
+// different banks.
+template <int TR, int TM, int WR, int WM>
+struct Tile {
+    static constexpr int kWaves = WR * WM, kThreads = 64 * kWaves;
+    static constexpr int FR = TR / WR / 16, FM = TM / WM / 16;  // operands of a wave
+    static constexpr int kBytes = (TR + TM) * 128;              // a step's
+    static constexpr int kPieces = kBytes / 1024 / kWaves;      // 1 KB loads a wave
+    static constexpr int kLds = 2 * kBytes;
+};
+
+constexpr int kRsrc = 0x00027000;  // a raw buffer
+
+// This wave's loads into LDS have arrived and its reads are done; then every wave's.
+__device__ __forceinline__ void arrived() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// sum += w . x. Written out so that the sums stay where they are: from the builtin the compiler gives results
+// other registers than their operands, and with all 256 accumulator registers in use copies them about in every
+// step. The next product of the same sum is (FR FM - 1) products away; the last ones are builtins, so that the
+// compiler knows what to wait for before it reads a sum.
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass knows no such registers)
+__device__ __forceinline__ void product(i4& sum, const i4& w, const i4& x) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(sum) : "v"(w), "v"(x));
+}
+#endif
+
+template <typename T, int TR, int TM, int WR, int WM>
+__global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r, int tiles_m) {
+#ifdef __HIP_DEVICE_COMPILE__
+    using S = Tile<TR, TM, WR, WM>;
+    constexpr int FR = S::FR, FM = S::FM, NP = S::kPieces, NW = TR / (8 * S::kWaves);
+    extern __shared__ __attribute__((aligned(128))) int8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, eight columns of tokens by
+    // as many rows as it has, so that its L2 serves what they share.
+    int tr, tm;
+    {
+        const int n = tiles_r * tiles_m, b = blockIdx.x, per = n / 8, rest = n % 8;
+        const int xcd = b % 8;
+        const int t = xcd * per + min(xcd, rest) + b / 8;
+        const int group = t / (8 * tiles_r), width = min(8, tiles_m - 8 * group);
+        const int in = t - group * 8 * tiles_r;
+        tr = in / width;
+        tm = 8 * group + in % width;
+    }
+    const int r0 = tr * TR, m0 = tm * TM;
+
+    // the lane's part of the wave's loads: 8 rows of a piece (the last row again where there are fewer), its
+    // chunk as the row's key says
+    static_assert(TR % (8 * S::kWaves) == 0, "a piece is of one operand");
+    const auto wb = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (long long)r0 * a.pitch), 0, -1, kRsrc);
+    const auto xb = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (long long)m0 * a.pitch), 0, -1, kRsrc);
+    int off[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int row = (i * S::kWaves + wave) * 8 + (lane >> 3);
+        const int in = i < NW ? min(row, a.R - 1 - r0) : min(row - TR, a.M - 1 - m0);
+        off[i] = in * a.pitch + 16 * ((lane & 7) ^ (lane >> 3));
+    }
+    // piece i of a step, into buffer `buf`
+    auto fetch = [&](int i, int buf, int step) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            i < NW ? wb : xb, (LdsPtr)(lds + buf * S::kBytes + (i * S::kWaves + wave) * 1024), 16, off[i],
+            step * 128, 0, 0);
+    };
+    const int wr = wave / WM, wm = wave % WM;
+    const int at = (lane & 15) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
+    const int at_w = wr * FR * 2048 + at, at_x = TR * 128 + wm * FM * 2048 + at;
+    i4 wf[2][FR], xf[2][FM];
+    // operand f of half a step
+    auto read = [&](int f, int half, int buf) {
+        const int8_t* base = lds + buf * S::kBytes;
+        if (f < FM) xf[half][f] = *reinterpret_cast<const i4*>(base + (at_x ^ (64 * half)) + f * 2048);
+        else wf[half][f - FM] = *reinterpret_cast<const i4*>(base + (at_w ^ (64 * half)) + (f - FM) * 2048);
+    };
+    i4 acc[FR][FM] = {};
+    constexpr int NF = FR + FM, N = FR * FM;
+    // The products of half a step, with the reads of the next half's operands (NR of them) and loads (NL) spread
+    // over the first three quarters of them.
+    auto multiply = [&](int half, auto nr, int read_buf, auto nl, int load_buf, int load_step) {
+        constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value, MOST = NR > NL ? NR : NL;
+        constexpr int EACH = MOST > 0 ? (N * 3 / 4) / MOST : N;
+        static_assert(EACH > 0, "more reads than products");
+        asm volatile("s_nop 1");  // (registers written just before a product written out need two states)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            // (behind a product: the first one's wait for its operands is not one for these reads)
+            product(acc[k / FM][k % FM], wf[half][k / FM], xf[half][k % FM]);
+            if (k % EACH == 0) {
+                if (k / EACH < NL) fetch(k / EACH, load_buf, load_step);
+                if (k / EACH < NR) read(k / EACH, half ^ 1, read_buf);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // A step: the products of its first half while the second half's operands are read; then every wave is
+    // done with the step's buffer and the next step has arrived in the other one: the products of the second
+    // half while the step after next is fetched into the buffer and the next one's first operands are read.
+    using Reads = std::integral_constant<int, NF>;
+    using Loads = std::integral_constant<int, NP>;
+    using None = std::integral_constant<int, 0>;
+    auto step = [&](int s, auto loads) {
+        const int cur = s & 1;
+        multiply(0, Reads(), cur, None(), 0, 0);
+        arrived();
+        multiply(1, Reads(), cur ^ 1, loads, cur, s + 2);
+    };
+    const int steps = a.pitch / 128;
+    for (int i = 0; i < NP; ++i) fetch(i, 0, 0);
+    if (steps > 1)
+        for (int i = 0; i < NP; ++i) fetch(i, 1, 1);
+    arrived();
+#pragma unroll
+    for (int f = 0; f < NF; ++f) read(f, 0, 0);
+    for (int s = 0; s < steps - 2; ++s) step(s, Loads());
+    if (steps > 1) step(steps - 2, None());
+    multiply(0, Reads(), (steps - 1) & 1, None(), 0, 0);
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0);
+    float xs[FM];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) xs[j] = a.x_scales[min(m0 + (wm * FM + j) * 16 + (lane & 15), a.M - 1)];
+#pragma unroll
+    for (int i = 0; i < FR; ++i) {
+        const int r = r0 + (wr * FR + i) * 16 + 4 * (lane >> 4);
+        const f4 ws = four_of(a.w_scales, r, a.R), bias = a.bias ? four_of(a.bias, r, a.R) : f4{};
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+            finish<T>(a, m0 + (wm * FM + j) * 16 + (lane & 15), r, acc[i][j], xs[j], ws, bias);
+    }
+#endif
+}
+
+template <typename T, int TR, int TM, int WR, int WM>
+void launch_tiles(const Args& a, hipStream_t st) {
+    using S = Tile<TR, TM, WR, WM>;
+    auto kernel = tile_kernel<T, TR, TM, WR, WM>;
+    if constexpr (S::kLds > 65536) {  // beyond the default: allowed once per device
+        static std::atomic<uint64_t> allowed{0};
+        int dev = 0;
+        (void)hipGetDevice(&dev);
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds);
+            allowed.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    const int tiles_r = (a.R + TR - 1) / TR, tiles_m = (a.M + TM - 1) / TM;
+    kernel<<<(unsigned)(tiles_r * tiles_m), S::kThreads, S::kLds, st>>>(a, tiles_r, tiles_m);
 }
 
 template <typename T>
 void launch(const Args& a, hipStream_t st) {
     const unsigned rows = (unsigned)((a.R + 15) / 16);
     if (a.M <= 16) rows16_kernel<T, 1, 8><<<dim3(rows, 1), 512, 0, st>>>(a);
+    else if (a.M > 64) launch_tiles<T, 256, 256, 2, 2>(a, st);
     else rows16_kernel<T, 4, 8><<<dim3(rows, (a.M + 63) / 64), 512, 0, st>>>(a);
 }
 
@@ -123,6 +331,9 @@ CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const
     a.R = R;
     a.M = M;
     a.pitch = (int)q8_pitch(C);
+    const size_t four = y_dtype == CSDR_F32 ? 16 : 8;
+    a.wide = a.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(y) % four == 0 &&
+             (!add || (a.add_stride % 4 == 0 && reinterpret_cast<uintptr_t>(add) % four == 0));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if (y_dtype == CSDR_F32) launch<float>(a, st);
     else launch<_Float16>(a, st);
