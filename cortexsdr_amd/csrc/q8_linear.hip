@@ -51,32 +51,36 @@ __device__ __forceinline__ f4 four_of(const float* p, int r, int R) {
     return v;
 }
 
-// Four neighbouring outputs of a token, as many of them as there are.
+__device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
+    return (float)sum * xs * ws + bias;
+}
+
+// Four neighbouring outputs of a token at once (a.wide, r + 3 < R, m < M).
+template <typename T>
+__device__ __forceinline__ void finish_wide(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
+                                            const f4& bias, const typename Four<T>::type& add) {
+    typename Four<T>::type o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (float)add[i]);
+    *reinterpret_cast<typename Four<T>::type*>(static_cast<T*>(a.y) + m * a.y_stride + r) = o;
+}
+template <typename T>
+__device__ __forceinline__ typename Four<T>::type wide_added(const Args& a, int m, int r) {
+    using V = typename Four<T>::type;
+    return *reinterpret_cast<const V*>(static_cast<const T*>(a.add) + m * a.add_stride + r);
+}
+
+// One by one, as many of them as there are.
 template <typename T>
 __device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
                                        const f4& bias) {
-    if (m >= a.M || r >= a.R) return;
-    using V = typename Four<T>::type;
+    if (m >= a.M) return;
     T* y = static_cast<T*>(a.y) + m * a.y_stride + r;
     const T* add = static_cast<const T*>(a.add) + m * a.add_stride + r;
-    f4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)sum[i] * xs * ws[i] + bias[i];
-    if (a.wide && r + 3 < a.R) {
-        if (a.add) {
-            const V u = *reinterpret_cast<const V*>(add);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += (float)u[i];
-        }
-        V o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
-        *reinterpret_cast<V*>(y) = o;
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (r + i < a.R) y[i] = (T)(a.add ? v[i] + (float)add[i] : v[i]);
+        if (r + i < a.R)
+            y[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (a.add ? (float)add[i] : 0.0f));
 }
 
 // 16 rows of w times 16 MT tokens; the waves take steps of 64 columns in turn and add up through LDS.
@@ -114,8 +118,13 @@ __global__ __launch_bounds__(WAVES * 64) void rows16_kernel(Args a) {
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) sum += part[k][j][l];
         const int m = m0 + 16 * j + (l & 15), r = r0 + 4 * (l >> 4);
-        finish<T>(a, m, r, sum, a.x_scales[min(m, a.M - 1)], four_of(a.w_scales, r, a.R),
-                  a.bias ? four_of(a.bias, r, a.R) : f4{});
+        const int rc = min(r, a.R - 1), mc = min(m, a.M - 1);
+        const float xs = a.x_scales[mc];
+        const f4 ws = four_of(a.w_scales, rc, a.R), bias = a.bias ? four_of(a.bias, rc, a.R) : f4{};
+        if (!a.wide || r + 3 >= a.R) finish<T>(a, m, r, sum, xs, ws, bias);
+        else if (m < a.M)
+            finish_wide<T>(a, m, r, sum, xs, ws, bias,
+                           a.add ? wide_added<T>(a, m, r) : typename Four<T>::type{});
     }
 }
 
@@ -133,6 +142,9 @@ struct Tile {
     static constexpr int kBytes = (TR + TM) * 128;              // a step's
     static constexpr int kPieces = kBytes / 1024 / kWaves;      // 1 KB loads a wave
     static constexpr int kLds = 2 * kBytes;
+    // through how many parts of the LDS a wave's sums go
+    static constexpr int kPasses = TR * TM * 4 > kLds ? 2 : 1;
+    static_assert(TR * TM * 4 <= kLds * kPasses, "sums of a pass");
 };
 
 constexpr int kRsrc = 0x00027000;  // a raw buffer
@@ -196,6 +208,13 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
             i < NW ? wb : xb, (LdsPtr)(lds + buf * S::kBytes + (i * S::kWaves + wave) * 1024), 16, off[i],
             step * 128, 0, 0);
     };
+    const int steps = a.pitch / 128;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) fetch(i, 0, 0);
+    if (steps > 1) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) fetch(i, 1, 1);
+    }
     const int wr = wave / WM, wm = wave % WM;
     const int at = (lane & 15) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
     const int at_w = wr * FR * 2048 + at, at_x = TR * 128 + wm * FM * 2048 + at;
@@ -207,13 +226,17 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
         else wf[half][f - FM] = *reinterpret_cast<const i4*>(base + (at_w ^ (64 * half)) + (f - FM) * 2048);
     };
     i4 acc[FR][FM] = {};
+#pragma unroll
+    for (int i = 0; i < FR; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) asm volatile("" : "+a"(acc[i][j]));  // (zero while the first loads run)
     constexpr int NF = FR + FM, N = FR * FM;
     // The products of half a step, with the reads of the next half's operands (NR of them) and loads (NL) spread
     // over the first three quarters of them.
     auto multiply = [&](int half, auto nr, int read_buf, auto nl, int load_buf, int load_step) {
         constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value, MOST = NR > NL ? NR : NL;
-        constexpr int EACH = MOST > 0 ? (N * 3 / 4) / MOST : N;
-        static_assert(EACH > 0, "more reads than products");
+        constexpr int EACH = MOST == 0 ? N : N * 3 / 4 / MOST > 0 ? N * 3 / 4 / MOST : 1;
+        static_assert(MOST <= N, "more reads than products");
         asm volatile("s_nop 1");  // (registers written just before a product written out need two states)
 #pragma unroll
         for (int k = 0; k < N; ++k) {
@@ -239,10 +262,6 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
         arrived();
         multiply(1, Reads(), cur ^ 1, loads, cur, s + 2);
     };
-    const int steps = a.pitch / 128;
-    for (int i = 0; i < NP; ++i) fetch(i, 0, 0);
-    if (steps > 1)
-        for (int i = 0; i < NP; ++i) fetch(i, 1, 1);
     arrived();
 #pragma unroll
     for (int f = 0; f < NF; ++f) read(f, 0, 0);
@@ -254,16 +273,53 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
 #pragma unroll
         for (int j = 0; j < FM; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0);
-    float xs[FM];
+    // Each wave turns its sums through its part of the LDS, `TOKENS` tokens at a time (token-major, 16-byte chunk c
+    // of token m at c ^ (m % 8)): a lane then has neighbouring rows for whole lines of y, and a short loop writes
+    // them, where straight code over the registers was 40 KB of instructions that came from memory at each launch
+    // (14 us of a launch, 3 with the loop).
+    constexpr int CHUNKS = TR / WR / 4, PASSES = S::kPasses, TOKENS = TM / WM / PASSES;
+    constexpr int PER = 64 / CHUNKS;  // tokens at once
+    constexpr int BATCH = TOKENS / PER < 16 ? TOKENS / PER : 16;
+    using V = typename Four<T>::type;
+    i4* part = reinterpret_cast<i4*>(lds) + wave * (TOKENS * CHUNKS);
+    const int c = lane % CHUNKS, mine = lane / CHUNKS;
+    const int r = r0 + wr * (TR / WR) + 4 * c;
+    const f4 ws = four_of(a.w_scales, min(r, a.R - 1), a.R);
+    const f4 bias = a.bias ? four_of(a.bias, min(r, a.R - 1), a.R) : f4{};
+    const bool whole = a.wide && r + 3 < a.R;
+    arrived();  // every wave is done with the tiles
 #pragma unroll
-    for (int j = 0; j < FM; ++j) xs[j] = a.x_scales[min(m0 + (wm * FM + j) * 16 + (lane & 15), a.M - 1)];
+    for (int p = 0; p < PASSES; ++p) {
 #pragma unroll
-    for (int i = 0; i < FR; ++i) {
-        const int r = r0 + (wr * FR + i) * 16 + 4 * (lane >> 4);
-        const f4 ws = four_of(a.w_scales, r, a.R), bias = a.bias ? four_of(a.bias, r, a.R) : f4{};
+        for (int j = 0; j < TOKENS / 16; ++j)
 #pragma unroll
-        for (int j = 0; j < FM; ++j)
-            finish<T>(a, m0 + (wm * FM + j) * 16 + (lane & 15), r, acc[i][j], xs[j], ws, bias);
+            for (int i = 0; i < FR; ++i) {
+                const int m = 16 * j + (lane & 15);
+                part[m * CHUNKS + ((4 * i + (lane >> 4)) ^ (m & 7))] = acc[i][p * (TOKENS / 16) + j];
+            }
+        const int first = m0 + wm * (TM / WM) + p * TOKENS + mine;
+        auto sum_of = [&](int k) { return part[(k + mine) * CHUNKS + (c ^ ((k + mine) & 7))]; };
+        if (whole) {
+#pragma unroll 1
+            for (int k = 0; k < TOKENS; k += BATCH * PER) {
+                float xs[BATCH];
+                V add[BATCH] = {};
+#pragma unroll
+                for (int q = 0; q < BATCH; ++q) {
+                    const int m = min(first + k + q * PER, a.M - 1);
+                    xs[q] = a.x_scales[m];
+                    if (a.add) add[q] = wide_added<T>(a, m, r);
+                }
+#pragma unroll
+                for (int q = 0; q < BATCH; ++q)
+                    if (first + k + q * PER < a.M)
+                        finish_wide<T>(a, first + k + q * PER, r, sum_of(k + q * PER), xs[q], ws, bias, add[q]);
+            }
+        } else if (r < a.R) {
+#pragma unroll 1
+            for (int k = 0; k < TOKENS; k += PER)
+                finish<T>(a, first + k, r, sum_of(k), a.x_scales[min(first + k, a.M - 1)], ws, bias);
+        }
     }
 #endif
 }
@@ -291,7 +347,18 @@ template <typename T>
 void launch(const Args& a, hipStream_t st) {
     const unsigned rows = (unsigned)((a.R + 15) / 16);
     if (a.M <= 16) rows16_kernel<T, 1, 8><<<dim3(rows, 1), 512, 0, st>>>(a);
-    else if (a.M > 64) launch_tiles<T, 256, 256, 2, 2>(a, st);
+    else if (a.M > 64) {
+        const char* e = getenv("TILE");
+        const int t = e ? atoi(e) : 0;
+        if (t == 0) launch_tiles<T, 256, 256, 2, 2>(a, st);
+        else if (t == 1) launch_tiles<T, 256, 128, 2, 2>(a, st);
+        else if (t == 2) launch_tiles<T, 128, 128, 2, 2>(a, st);
+        else if (t == 3) launch_tiles<T, 64, 64, 2, 2>(a, st);
+        else if (t == 4) launch_tiles<T, 128, 64, 2, 2>(a, st);
+        else if (t == 5) launch_tiles<T, 64, 128, 2, 2>(a, st);
+        else if (t == 6) launch_tiles<T, 128, 256, 2, 2>(a, st);
+        else if (t == 7) rows16_kernel<T, 4, 8><<<dim3(rows, (a.M + 63) / 64), 512, 0, st>>>(a);
+    }
     else rows16_kernel<T, 4, 8><<<dim3(rows, (a.M + 63) / 64), 512, 0, st>>>(a);
 }
 
