@@ -4,6 +4,7 @@
 // a sum is converted to fp32, by two products and the additions in fp32, and once to y's type.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -83,76 +84,35 @@ __device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& su
             y[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (a.add ? (float)add[i] : 0.0f));
 }
 
-// 16 rows of w times 16 MT tokens; the waves take steps of 64 columns in turn and add up through LDS.
-// w and x come from memory straight into the operands: lane l holds row l % 16, columns 16 (l / 16) and
-// on of a step (both operands alike, so their order within a step does not matter).
-template <typename T, int MT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void rows16_kernel(Args a) {
-    __shared__ i4 part[WAVES][MT][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-    const long long at = 16 * (lane >> 4);
-    const int8_t* w = a.w + (long long)min(r0 + (lane & 15), a.R - 1) * a.pitch + at;
-    const int8_t* x[MT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-        x[j] = a.x + (long long)min(m0 + 16 * j + (lane & 15), a.M - 1) * a.pitch + at;
-    i4 acc[MT] = {};
-    const int steps = a.pitch / 64;
-#pragma unroll 4
-    for (int s = wave; s < steps; s += WAVES) {
-        const i4 wv = *reinterpret_cast<const i4*>(w + 64 * s);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            const i4 xv = *reinterpret_cast<const i4*>(x[j] + 64 * s);
-            acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xv, acc[j], 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) part[wave][j][lane] = acc[j];
-    __syncthreads();
-    // D: lane l holds rows 4 (l / 16) and on, column l % 16
-    for (int i = threadIdx.x; i < MT * 64; i += WAVES * 64) {
-        const int j = i >> 6, l = i & 63;
-        i4 sum = part[0][j][l];
-#pragma unroll
-        for (int k = 1; k < WAVES; ++k) sum += part[k][j][l];
-        const int m = m0 + 16 * j + (l & 15), r = r0 + 4 * (l >> 4);
-        const int rc = min(r, a.R - 1), mc = min(m, a.M - 1);
-        const float xs = a.x_scales[mc];
-        const f4 ws = four_of(a.w_scales, rc, a.R), bias = a.bias ? four_of(a.bias, rc, a.R) : f4{};
-        if (!a.wide || r + 3 >= a.R) finish<T>(a, m, r, sum, xs, ws, bias);
-        else if (m < a.M)
-            finish_wide<T>(a, m, r, sum, xs, ws, bias,
-                           a.add ? wide_added<T>(a, m, r) : typename Four<T>::type{});
-    }
-}
-
-// ------------------------------------------------------------------ tiles through LDS
-
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
 // TR rows of w times TM tokens a workgroup, in WR x WM waves. A step is 128 columns; its rows lie in LDS 128
 // bytes apart, 16-byte chunk c of row i at c ^ (i % 8), so that the 16 rows of an operand's chunk fall on
-// different banks.
-template <int TR, int TM, int WR, int WM>
+// different banks. KG groups of waves take a step each of a stage's KG and add up at the end; NBUF stages are
+// in LDS or on their way.
+template <int TR, int TM, int KG, int WR, int WM, int NBUF>
 struct Tile {
-    static constexpr int kWaves = WR * WM, kThreads = 64 * kWaves;
+    static constexpr int kWaves = KG * WR * WM, kThreads = 64 * kWaves;
     static constexpr int FR = TR / WR / 16, FM = TM / WM / 16;  // operands of a wave
-    static constexpr int kBytes = (TR + TM) * 128;              // a step's
+    static constexpr int kGroup = (TR + TM) * 128;              // a step's bytes
+    static constexpr int kBytes = KG * kGroup;                  // a stage's
     static constexpr int kPieces = kBytes / 1024 / kWaves;      // 1 KB loads a wave
-    static constexpr int kLds = 2 * kBytes;
-    // through how many parts of the LDS a wave's sums go
-    static constexpr int kPasses = TR * TM * 4 > kLds ? 2 : 1;
-    static_assert(TR * TM * 4 <= kLds * kPasses, "sums of a pass");
+    static_assert(kPieces * 1024 * kWaves == kBytes, "whole pieces");
+    static constexpr int kLds = NBUF * kBytes;
+    // through how many parts the sums go to the other threads
+    static constexpr int kPasses = KG * TR * TM * 4 > kLds ? 2 : 1;
+    static_assert(KG * TR * TM * 4 <= kLds * kPasses && kLds <= 160 * 1024, "LDS");
 };
 
 constexpr int kRsrc = 0x00027000;  // a raw buffer
 
 // This wave's loads into LDS have arrived and its reads are done; then every wave's.
+// (LATER: loads of steps that need not have.)
+template <int LATER>
 __device__ __forceinline__ void arrived() {
+    static_assert(LATER < 64, "the counter's width");
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -168,11 +128,11 @@ __device__ __forceinline__ void product(i4& sum, const i4& w, const i4& x) {
 }
 #endif
 
-template <typename T, int TR, int TM, int WR, int WM>
-__global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r, int tiles_m) {
+template <typename T, int TR, int TM, int KG, int WR, int WM, int NBUF>
+__global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int tiles_r, int tiles_m) {
 #ifdef __HIP_DEVICE_COMPILE__
-    using S = Tile<TR, TM, WR, WM>;
-    constexpr int FR = S::FR, FM = S::FM, NP = S::kPieces, NW = TR / (8 * S::kWaves);
+    using S = Tile<TR, TM, KG, WR, WM, NBUF>;
+    constexpr int FR = S::FR, FM = S::FM, NP = S::kPieces;
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -192,31 +152,35 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
 
     // the lane's part of the wave's loads: 8 rows of a piece (the last row again where there are fewer), its
     // chunk as the row's key says
-    static_assert(TR % (8 * S::kWaves) == 0, "a piece is of one operand");
-    const auto wb = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (long long)r0 * a.pitch), 0, -1, kRsrc);
-    const auto xb = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (long long)m0 * a.pitch), 0, -1, kRsrc);
+    const int steps = a.pitch / 128, stages = (steps + KG - 1) / KG;
+    constexpr int PW = TR / 8, PG = (TR + TM) / 8;  // pieces of w, and of a step
     int off[NP];
+    auto of_w = [&](int i) {  // which operand piece i is of: known when compiled where TR is whole pieces of all
+        if constexpr (KG == 1 && PW % S::kWaves == 0) return i < PW / S::kWaves;
+        else return (i * S::kWaves + wave) % PG < PW;
+    };
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int row = (i * S::kWaves + wave) * 8 + (lane >> 3);
-        const int in = i < NW ? min(row, a.R - 1 - r0) : min(row - TR, a.M - 1 - m0);
+        const int row = (i * S::kWaves + wave) % PG * 8 + (lane >> 3);
+        const int in = of_w(i) ? min(row, a.R - 1 - r0) : min(row - TR, a.M - 1 - m0);
         off[i] = in * a.pitch + 16 * ((lane & 7) ^ (lane >> 3));
     }
-    // piece i of a step, into buffer `buf`
-    auto fetch = [&](int i, int buf, int step) {
+    // piece i of a stage, into buffer `buf` (the last step again behind the end)
+    auto fetch = [&](int i, int buf, int stage) {
+        const int8_t* base = of_w(i) ? a.w + (long long)r0 * a.pitch : a.x + (long long)m0 * a.pitch;
+        const int p = i * S::kWaves + wave, step = KG == 1 ? stage : min(stage * KG + p / PG, steps - 1);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            i < NW ? wb : xb, (LdsPtr)(lds + buf * S::kBytes + (i * S::kWaves + wave) * 1024), 16, off[i],
-            step * 128, 0, 0);
+            __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, kRsrc), (LdsPtr)(lds + buf * S::kBytes + p * 1024),
+            16, off[i], step * 128, 0, 0);
     };
-    const int steps = a.pitch / 128;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) fetch(i, 0, 0);
-    if (steps > 1) {
+    for (int b = 0; b < NBUF; ++b)
+        if (b < stages) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) fetch(i, 1, 1);
-    }
-    const int wr = wave / WM, wm = wave % WM;
-    const int at = (lane & 15) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
+            for (int i = 0; i < NP; ++i) fetch(i, b, b);
+        }
+    const int group = wave / (WR * WM), wr = wave / WM % WR, wm = wave % WM;
+    const int at = group * S::kGroup + (lane & 15) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
     const int at_w = wr * FR * 2048 + at, at_x = TR * 128 + wm * FM * 2048 + at;
     i4 wf[2][FR], xf[2][FM];
     // operand f of half a step
@@ -225,109 +189,139 @@ __global__ __launch_bounds__(64 * WR * WM) void tile_kernel(Args a, int tiles_r,
         if (f < FM) xf[half][f] = *reinterpret_cast<const i4*>(base + (at_x ^ (64 * half)) + f * 2048);
         else wf[half][f - FM] = *reinterpret_cast<const i4*>(base + (at_w ^ (64 * half)) + (f - FM) * 2048);
     };
+    constexpr int NF = FR + FM, N = FR * FM;
+    constexpr bool OUT = N >= 4;  // products written out: three others at least between two of a sum
     i4 acc[FR][FM] = {};
 #pragma unroll
     for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < FM; ++j) asm volatile("" : "+a"(acc[i][j]));  // (zero while the first loads run)
-    constexpr int NF = FR + FM, N = FR * FM;
+        for (int j = 0; j < FM; ++j)
+            if constexpr (OUT) asm volatile("" : "+a"(acc[i][j]));  // (zero while the first loads run)
+
     // The products of half a step, with the reads of the next half's operands (NR of them) and loads (NL) spread
     // over the first three quarters of them.
     auto multiply = [&](int half, auto nr, int read_buf, auto nl, int load_buf, int load_step) {
         constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value, MOST = NR > NL ? NR : NL;
         constexpr int EACH = MOST == 0 ? N : N * 3 / 4 / MOST > 0 ? N * 3 / 4 / MOST : 1;
-        static_assert(MOST <= N, "more reads than products");
-        asm volatile("s_nop 1");  // (registers written just before a product written out need two states)
+        constexpr int GROUP = (MOST + N - 1) / N;  // of them behind a product
+        if constexpr (OUT) asm volatile("s_nop 1");  // (registers written just before need two states)
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             // (behind a product: the first one's wait for its operands is not one for these reads)
-            product(acc[k / FM][k % FM], wf[half][k / FM], xf[half][k % FM]);
+            i4& sum = acc[k / FM][k % FM];
+            if constexpr (OUT) product(sum, wf[half][k / FM], xf[half][k % FM]);
+            else sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[half][k / FM], xf[half][k % FM], sum, 0, 0, 0);
             if (k % EACH == 0) {
-                if (k / EACH < NL) fetch(k / EACH, load_buf, load_step);
-                if (k / EACH < NR) read(k / EACH, half ^ 1, read_buf);
+#pragma unroll
+                for (int i = k / EACH * GROUP; i < (k / EACH + 1) * GROUP; ++i) {
+                    if (i < NL) fetch(i, load_buf, load_step);
+                    if (i < NR) read(i, half ^ 1, read_buf);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     // A step: the products of its first half while the second half's operands are read; then every wave is
-    // done with the step's buffer and the next step has arrived in the other one: the products of the second
-    // half while the step after next is fetched into the buffer and the next one's first operands are read.
+    // done with the step's buffer and the next step has arrived in its own: the products of the second half
+    // while a later step is fetched into the buffer and the next one's first operands are read.
     using Reads = std::integral_constant<int, NF>;
     using Loads = std::integral_constant<int, NP>;
     using None = std::integral_constant<int, 0>;
+    int buf = 0;
     auto step = [&](int s, auto loads) {
-        const int cur = s & 1;
-        multiply(0, Reads(), cur, None(), 0, 0);
-        arrived();
-        multiply(1, Reads(), cur ^ 1, loads, cur, s + 2);
+        const int next = buf + 1 < NBUF ? buf + 1 : 0;
+        multiply(0, Reads(), buf, None(), 0, 0);
+        if constexpr (decltype(loads)::value > 0) arrived<(NBUF - 2) * NP>();
+        else arrived<0>();
+        multiply(1, Reads(), next, loads, buf, s + NBUF);
+        buf = next;
     };
-    arrived();
+    if (stages >= NBUF) arrived<(NBUF - 1) * NP>();
+    else arrived<0>();
 #pragma unroll
     for (int f = 0; f < NF; ++f) read(f, 0, 0);
-    for (int s = 0; s < steps - 2; ++s) step(s, Loads());
-    if (steps > 1) step(steps - 2, None());
-    multiply(0, Reads(), (steps - 1) & 1, None(), 0, 0);
+    int s = 0;
+    for (; s < stages - NBUF; ++s) step(s, Loads());
+#pragma unroll 1
+    for (; s < stages - 1; ++s) step(s, None());
+    if (KG == 1 || s * KG + group < steps) {
+        multiply(0, Reads(), buf, None(), 0, 0);
 #pragma unroll
-    for (int i = 0; i < FR; ++i)
+        for (int i = 0; i < FR; ++i)
 #pragma unroll
-        for (int j = 0; j < FM; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0);
-    // Each wave turns its sums through its part of the LDS, `TOKENS` tokens at a time (token-major, 16-byte chunk c
-    // of token m at c ^ (m % 8)): a lane then has neighbouring rows for whole lines of y, and a short loop writes
-    // them, where straight code over the registers was 40 KB of instructions that came from memory at each launch
-    // (14 us of a launch, 3 with the loop).
-    constexpr int CHUNKS = TR / WR / 4, PASSES = S::kPasses, TOKENS = TM / WM / PASSES;
-    constexpr int PER = 64 / CHUNKS;  // tokens at once
-    constexpr int BATCH = TOKENS / PER < 16 ? TOKENS / PER : 16;
+            for (int j = 0; j < FM; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0);
+    } else if constexpr (OUT) {  // the last products of these waves were written out: until their sums are there
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // The sums go through LDS (token-major, 16-byte chunk c of token m at c ^ (m % 8)): a thread then has
+    // neighbouring rows for whole lines of y, and a short loop writes them, where straight code over the registers
+    // was 40 KB of instructions that came from memory at each launch, and one read of `add` after another.
+    constexpr int CHUNKS = TR / 4, KEYS = CHUNKS < 8 ? CHUNKS : 8, PASSES = S::kPasses;
+    constexpr int TOKENS = TM / PASSES, MINE = TOKENS / WM;      // of a pass, and of those a wave's
+    constexpr int PER = S::kThreads / CHUNKS;                    // tokens at once
+    constexpr int ROUNDS = TOKENS > PER ? TOKENS / PER : 1, BATCH = ROUNDS < 8 ? ROUNDS : 8;
     using V = typename Four<T>::type;
-    i4* part = reinterpret_cast<i4*>(lds) + wave * (TOKENS * CHUNKS);
-    const int c = lane % CHUNKS, mine = lane / CHUNKS;
-    const int r = r0 + wr * (TR / WR) + 4 * c;
+    i4* part = reinterpret_cast<i4*>(lds);
+    const int c = threadIdx.x % CHUNKS, mine = threadIdx.x / CHUNKS;
+    const int r = r0 + 4 * c;
     const f4 ws = four_of(a.w_scales, min(r, a.R - 1), a.R);
     const f4 bias = a.bias ? four_of(a.bias, min(r, a.R - 1), a.R) : f4{};
     const bool whole = a.wide && r + 3 < a.R;
-    arrived();  // every wave is done with the tiles
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
+        arrived<0>();  // every wave is done with what lay there
 #pragma unroll
-        for (int j = 0; j < TOKENS / 16; ++j)
+        for (int j = 0; j < MINE / 16; ++j)
 #pragma unroll
             for (int i = 0; i < FR; ++i) {
-                const int m = 16 * j + (lane & 15);
-                part[m * CHUNKS + ((4 * i + (lane >> 4)) ^ (m & 7))] = acc[i][p * (TOKENS / 16) + j];
+                const int m = wm * MINE + 16 * j + (lane & 15), k = (wr * FR + i) * 4 + (lane >> 4);
+                part[(group * TOKENS + m) * CHUNKS + (k ^ (m & (KEYS - 1)))] = acc[i][p * (MINE / 16) + j];
             }
-        const int first = m0 + wm * (TM / WM) + p * TOKENS + mine;
-        auto sum_of = [&](int k) { return part[(k + mine) * CHUNKS + (c ^ ((k + mine) & 7))]; };
+        arrived<0>();
+        // token m of a pass: the wave of its columns has it there
+        auto token = [&](int m) { return m0 + m / MINE * (TM / WM) + p * MINE + m % MINE; };
+        auto sum_of = [&](int m) {
+            i4 sum = part[m * CHUNKS + (c ^ (m & (KEYS - 1)))];
+#pragma unroll
+            for (int g = 1; g < KG; ++g) sum += part[(g * TOKENS + m) * CHUNKS + (c ^ (m & (KEYS - 1)))];
+            return sum;
+        };
         if (whole) {
 #pragma unroll 1
-            for (int k = 0; k < TOKENS; k += BATCH * PER) {
+            for (int k = mine; k < TOKENS; k += BATCH * PER) {
                 float xs[BATCH];
                 V add[BATCH] = {};
 #pragma unroll
                 for (int q = 0; q < BATCH; ++q) {
-                    const int m = min(first + k + q * PER, a.M - 1);
+                    const int m = min(token(k + q * PER), a.M - 1);
                     xs[q] = a.x_scales[m];
                     if (a.add) add[q] = wide_added<T>(a, m, r);
                 }
 #pragma unroll
-                for (int q = 0; q < BATCH; ++q)
-                    if (first + k + q * PER < a.M)
-                        finish_wide<T>(a, first + k + q * PER, r, sum_of(k + q * PER), xs[q], ws, bias, add[q]);
+                for (int q = 0; q < BATCH; ++q) {
+                    const int m = token(k + q * PER);
+                    if (m < a.M) finish_wide<T>(a, m, r, sum_of(k + q * PER), xs[q], ws, bias, add[q]);
+                }
             }
         } else if (r < a.R) {
 #pragma unroll 1
-            for (int k = 0; k < TOKENS; k += PER)
-                finish<T>(a, first + k, r, sum_of(k), a.x_scales[min(first + k, a.M - 1)], ws, bias);
+            for (int k = mine; k < TOKENS; k += PER) {
+                const int m = token(k);
+                finish<T>(a, m, r, sum_of(k), a.x_scales[min(m, a.M - 1)], ws, bias);
+            }
         }
     }
 #endif
 }
 
-template <typename T, int TR, int TM, int WR, int WM>
-void launch_tiles(const Args& a, hipStream_t st) {
-    using S = Tile<TR, TM, WR, WM>;
-    auto kernel = tile_kernel<T, TR, TM, WR, WM>;
+template <typename T, int TR, int TM, int KG, int WR, int WM, int NBUF>
+int launch_tiles(const Args& a, hipStream_t st) {
+    using S = Tile<TR, TM, KG, WR, WM, NBUF>;
+    auto kernel = tile_kernel<T, TR, TM, KG, WR, WM, NBUF>;
     if constexpr (S::kLds > 65536) {  // beyond the default: allowed once per device
         static std::atomic<uint64_t> allowed{0};
         int dev = 0;
@@ -340,26 +334,56 @@ void launch_tiles(const Args& a, hipStream_t st) {
         }
     }
     const int tiles_r = (a.R + TR - 1) / TR, tiles_m = (a.M + TM - 1) / TM;
+    if ((long long)tiles_r * tiles_m >= (1LL << 32) / S::kThreads)
+        return set_error(CSDR_E_INVALID, "q8_linear: more workgroups than a launch may have");
     kernel<<<(unsigned)(tiles_r * tiles_m), S::kThreads, S::kLds, st>>>(a, tiles_r, tiles_m);
+    return CSDR_OK;
+}
+
+// What a tile costs, in us: `fixed` for a workgroup's start and end, a step of 128 columns `alone` for one workgroup on
+// a CU and `each` for every one of `held` (as many as a CU's LDS holds). Fitted to products of 1 to 4096 tokens with
+// 4096 or 11008 rows and 896 to 11008 columns, which they give within a tenth to a fifth; the rule has only to tell
+// tiles apart.
+struct Cost {
+    int tr, tm, held;
+    float fixed, alone, each;
+};
+constexpr Cost kCosts[] = {
+    {256, 256, 1, 11.0f, 1.35f, 1.35f}, {128, 128, 2, 5.0f, 0.53f, 0.445f}, {128, 64, 2, 3.0f, 0.33f, 0.30f},
+    {64, 64, 3, 3.0f, 0.235f, 0.197f},  {32, 64, 3, 3.0f, 0.165f, 0.122f},  {32, 32, 2, 2.4f, 0.122f, 0.10f},
+    {16, 16, 3, 2.3f, 0.088f, 0.073f},
+};
+constexpr int kCUs = 256;
+
+float cost_of(const Cost& c, const Args& a) {
+    const long long tiles = (long long)((a.R + c.tr - 1) / c.tr) * ((a.M + c.tm - 1) / c.tm);
+    const long long most = (tiles + kCUs - 1) / kCUs;  // of a CU
+    const int steps = a.pitch / 128, rest = (int)(most % c.held);
+    float us = (float)(most / c.held) * (c.fixed + steps * c.held * c.each);
+    if (rest) us += c.fixed + steps * std::max(c.alone, rest * c.each);
+    return us;
 }
 
 template <typename T>
-void launch(const Args& a, hipStream_t st) {
-    const unsigned rows = (unsigned)((a.R + 15) / 16);
-    if (a.M <= 16) rows16_kernel<T, 1, 8><<<dim3(rows, 1), 512, 0, st>>>(a);
-    else if (a.M > 64) {
-        const char* e = getenv("TILE");
-        const int t = e ? atoi(e) : 0;
-        if (t == 0) launch_tiles<T, 256, 256, 2, 2>(a, st);
-        else if (t == 1) launch_tiles<T, 256, 128, 2, 2>(a, st);
-        else if (t == 2) launch_tiles<T, 128, 128, 2, 2>(a, st);
-        else if (t == 3) launch_tiles<T, 64, 64, 2, 2>(a, st);
-        else if (t == 4) launch_tiles<T, 128, 64, 2, 2>(a, st);
-        else if (t == 5) launch_tiles<T, 64, 128, 2, 2>(a, st);
-        else if (t == 6) launch_tiles<T, 128, 256, 2, 2>(a, st);
-        else if (t == 7) rows16_kernel<T, 4, 8><<<dim3(rows, (a.M + 63) / 64), 512, 0, st>>>(a);
+int launch(const Args& a, hipStream_t st) {
+    int best = 0;
+    float least = INFINITY;
+    for (int i = 0; i < (int)(sizeof kCosts / sizeof *kCosts); ++i) {
+        const float us = cost_of(kCosts[i], a);
+        if (us < least) {
+            least = us;
+            best = i;
+        }
     }
-    else rows16_kernel<T, 4, 8><<<dim3(rows, (a.M + 63) / 64), 512, 0, st>>>(a);
+    switch (best) {
+        case 0: return launch_tiles<T, 256, 256, 1, 2, 4, 2>(a, st);
+        case 1: return launch_tiles<T, 128, 128, 1, 4, 2, 2>(a, st);
+        case 2: return launch_tiles<T, 128, 64, 1, 2, 2, 3>(a, st);
+        case 3: return launch_tiles<T, 64, 64, 1, 2, 2, 3>(a, st);
+        case 4: return launch_tiles<T, 32, 64, 1, 1, 4, 4>(a, st);
+        case 5: return launch_tiles<T, 32, 32, 2, 1, 2, 4>(a, st);
+        default: return launch_tiles<T, 16, 16, 4, 1, 1, 3>(a, st);
+    }
 }
 
 }  // namespace
@@ -402,8 +426,8 @@ CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const
     a.wide = a.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(y) % four == 0 &&
              (!add || (a.add_stride % 4 == 0 && reinterpret_cast<uintptr_t>(add) % four == 0));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    if (y_dtype == CSDR_F32) launch<float>(a, st);
-    else launch<_Float16>(a, st);
+    const int rc = y_dtype == CSDR_F32 ? launch<float>(a, st) : launch<_Float16>(a, st);
+    if (rc != CSDR_OK) return rc;
     CSDR_LAUNCH_CHECK("q8_linear");
     return CSDR_OK;
 }
