@@ -5,13 +5,13 @@
 // are those of exact arithmetic, so that a code does not depend on the order of a sum or on which kernel
 // made it. The norm's 1 / rms is in every value of a row and cancels in its codes: they come from
 // t = h w alone, a product of two fp32 numbers that fp64 holds exactly, and one pass over the row gives
-// both the sum of squares and top. fp64 runs at the fp32 rate here. 127 t / top is taken as a product
-// with the reciprocal (off by 1e-13), and divided only where that lies next to a border. A gated value
-// costs an exponential: those are computed in fp32 (off by less than 4e-7 of themselves), and in fp64
-// where the code lies next to a border or the value may be the row's largest.
+// both the sum of squares (fp64) and top. Values, their largest and their codes are formed in fp32, and
+// in fp64 only where that may not be enough: the values that may be the row's largest, the codes next to a
+// border between two (one of several thousand), rows so small that fp32 holds their values with few bits
+// or so large that it does not hold them.
 //
-// A row that holds a value which is not finite (or whose largest value passes fp32) has the scale NaN
-// and codes 0, so it reads as NaN; a row of zeros has the scale 0.
+// A row that holds a value which is not finite (or whose scale passes fp32) has the scale NaN and codes 0,
+// so it reads as NaN; a row of zeros has the scale 0.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -38,6 +38,22 @@ struct __attribute__((packed, aligned(sizeof(T)))) Vec {
     T v[kChunk];
 };
 
+// The chunk at `at` of a row of n values as it lies there, without a branch (another chunk of the row where it is not
+// whole), so that a thread's loads are on their way together; then its values, zeros behind the last.
+template <typename T>
+__device__ __forceinline__ Vec<T> raw_of(const T* row, int at, int n) {
+    return *reinterpret_cast<const Vec<T>*>(row + (at + kChunk <= n ? at : 0));
+}
+template <typename T>
+__device__ __forceinline__ void values_of(const Vec<T>& raw, const T* row, int at, int n, float* f) {
+    if (at + kChunk <= n) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) f[i] = csdr::to_f32(raw.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) f[i] = at + i < n ? csdr::to_f32(row[at + i]) : 0.0f;
+    }
+}
 template <typename T>
 __device__ __forceinline__ void load(const T* p, int left, float* f) {
     if (left >= kChunk) {
@@ -61,68 +77,133 @@ __device__ __forceinline__ void store(T* p, int left, const float* f) {
     }
 }
 
-// What a row's threads have to agree on.
-struct Row {
-    double sum, top;
-};
-
 __device__ __forceinline__ uint64_t bits_of(double v) { return __builtin_bit_cast(uint64_t, v); }
 __device__ __forceinline__ double of_bits(uint64_t v) { return __builtin_bit_cast(double, v); }
-// The larger magnitude; a NaN is larger than any number.
-__device__ __forceinline__ double larger(double a, double b) {
-    return of_bits(max(bits_of(a), bits_of(b)));
-}
 
-// Over the workgroup; `lds` has a Row per wave.
-__device__ __forceinline__ Row join(Row r, Row* lds) {
+// How far a value formed in fp32 is off at most, of itself: 8 roundings for a gated value (the exponential and the
+// reciprocal are off by a step), one for a norm's; and then its code, of 127 at most: with a quarter to spare.
+constexpr float kValueOff = 1.2e-6f, kCodeOff = 1e-4f;
+// Rows whose largest value is below kTiny are formed in fp64 throughout.
+constexpr float kTiny = 1e-25f;
+// Rows with a gate below it too: the sigmoid leaves the normal numbers of fp32.
+constexpr float kLow = -87.0f;
+
+// What a row's threads have to agree on, and what they pass it through.
+struct Joined {
+    double sum;
+    uint32_t most;  // bits of the largest magnitude in fp32; a NaN's are larger than any number's
+    bool low;
+};
+struct Shared {
+    double sum[kMaxThreads / 64];
+    uint32_t most[kMaxThreads / 64];
+    unsigned long long top;
+};
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const u2 b = __builtin_bit_cast(u2, v);
+    return __builtin_bit_cast(double, u2{dpp<CTRL>(b[0]), dpp<CTRL>(b[1])});
+}
+// lane ^ 1, lane ^ 2, mirrored within 8 and within 16 lanes, which then hold one value
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+
+template <bool SUM>
+__device__ __forceinline__ Joined join(Joined r, Shared& lds) {
+    r.most = max(r.most, dpp<kXor1>(r.most));
+    r.most = max(r.most, dpp<kXor2>(r.most));
+    r.most = max(r.most, dpp<kHalfMirror>(r.most));
+    r.most = max(r.most, dpp<kMirror>(r.most));
+    uint32_t most = 0;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        r.sum += __shfl_xor(r.sum, off, 64);
-        r.top = larger(r.top, __shfl_xor(r.top, off, 64));
+    for (int i = 0; i < 4; ++i) most = max(most, (uint32_t)__builtin_amdgcn_readlane((int)r.most, 16 * i));
+    if (SUM) {
+        r.sum += dpp<kXor1>(r.sum);
+        r.sum += dpp<kXor2>(r.sum);
+        r.sum += dpp<kHalfMirror>(r.sum);
+        r.sum += dpp<kMirror>(r.sum);
+        r.sum += __shfl_xor(r.sum, 16, 64);
+        r.sum += __shfl_xor(r.sum, 32, 64);
     }
+    r.low = __any(r.low);
+    if (threadIdx.x == 0) lds.top = 0;
     const int waves = blockDim.x >> 6;
-    if (waves == 1) return r;
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = r;
-    __syncthreads();
-    r = lds[0];
-    for (int i = 1; i < waves; ++i) {
-        r.sum += lds[i].sum;
-        r.top = larger(r.top, lds[i].top);
+    if ((threadIdx.x & 63) == 0) {
+        if (SUM) lds.sum[threadIdx.x >> 6] = r.sum;
+        lds.most[threadIdx.x >> 6] = most << 1 | (r.low ? 1u : 0u);  // (the sign's bit is free)
     }
+    __syncthreads();
+    r.sum = 0.0;
+    uint32_t both = 0, low = 0;
+    for (int i = 0; i < waves; ++i) {
+        if (SUM) r.sum += lds.sum[i];
+        both = max(both, lds.most[i]);
+        low |= lds.most[i] & 1u;
+    }
+    r.most = both >> 1;
+    r.low = low != 0;
     return r;
 }
 
-// Next to a border between two codes, as a distance of q from a half.
-__device__ __forceinline__ bool at_border(double q, double r) { return fabs(fabs(q - r) - 0.5) < 1e-9; }
-
 struct Scale {
     double inv, top;  // 127 / top (0 for rows without codes)
-    float value;
+    float inv32, value;
+    bool wide;        // codes in fp64 throughout
 };
 
-__device__ __forceinline__ Scale scale_of(double top, double factor) {
+__device__ __forceinline__ Scale scale_of(double top, double factor, bool wide) {
     Scale s;
     s.top = top;
     s.value = (float)(top * factor / 127.0);
     const bool fine = s.value < INFINITY;  // (not for a NaN)
     if (!fine) s.value = NAN;
     s.inv = fine && top > 0.0 ? 127.0 / top : 0.0;
+    s.inv32 = (float)s.inv;
+    s.wide = wide;
     return s;
 }
 
+// In exact arithmetic, but for 1e-13 of the product with the reciprocal: divided where that lies next to a border.
 __device__ __forceinline__ int code_of(double t, const Scale& s) {
     const double q = t * s.inv;
     double r = rint(q);
-    if (__builtin_expect(at_border(q, r), 0)) r = rint(127.0 * t / s.top);
+    if (__builtin_expect(fabs(fabs(q - r) - 0.5) < 1e-9, 0)) r = rint(127.0 * t / s.top);
     return (int)r;
 }
 
-__device__ __forceinline__ void store_codes(int8_t* p, const int* c) {
+// The codes of a chunk's values t, exact(i) being value i in fp64. 3 2^22 + q holds rint(q) in its low bits.
+template <typename Exact>
+__device__ __forceinline__ void put_codes(int8_t* p, const float* t, const Scale& s, Exact exact) {
     u2 v = {0, 0};
+    if (s.inv > 0.0) {
+        constexpr float kMagic = 12582912.0f;
+        uint32_t c[kChunk];
+        float d[kChunk], most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i / 4] |= (uint32_t)(c[i] & 255) << (8 * (i % 4));
+        for (int i = 0; i < kChunk; ++i) {
+            const float u = fmaf(t[i], s.inv32, kMagic);
+            d[i] = fabsf(fmaf(t[i], s.inv32, -(u - kMagic)));
+            c[i] = __float_as_uint(u);
+            most = fmaxf(most, d[i]);
+        }
+        if (__builtin_expect(most > 0.5f - kCodeOff || s.wide, 0)) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i)
+                if (d[i] > 0.5f - kCodeOff || s.wide) c[i] = (uint32_t)code_of(exact(i), s);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            v[i] = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u) |
+                   __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x04000c0cu);
+    }
     *reinterpret_cast<u2*>(p) = v;
 }
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // ------------------------------------------------------------------ norm
 
@@ -150,76 +231,112 @@ __device__ __forceinline__ void load_h(const NormArgs& a, long long row, int at,
 }
 
 // A row per workgroup. NV > 0: its values stay in registers, NV chunks a thread; 0: rows of any width,
-// read twice.
+// formed again for each step. What fp64 needs comes from memory again.
 template <typename TX, typename TR, bool RES, int NV>
 __global__ __launch_bounds__(kMaxThreads) void norm_kernel(NormArgs a) {
-    __shared__ Row lds[kMaxThreads / 64];
+    __shared__ Shared lds;
     const long long row = blockIdx.x;
     const int step = blockDim.x * kChunk, first = threadIdx.x * kChunk;
     constexpr int N = NV > 0 ? NV : 1;
-    float h[N][kChunk];
-    double sum = 0.0, top = 0.0;
+    float t[N][kChunk] = {};  // h w
+    Joined r = {0.0, 0, false};
     TR* out = RES ? static_cast<TR*>(a.residual_out) + row * a.n : nullptr;
 
-    auto take = [&](float* v, int at) {
-        float w[kChunk];
+    auto each = [&](int end, auto f) {
+        if (NV > 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (first + j * step < end) f(j, first + j * step);
+        } else {
+            for (int at = first; at < end; at += step) f(0, at);
+        }
+    };
+    // h as the stream holds it (where that is updated in place its old values are gone)
+    auto load_again = [&](int at, float* h, float* w) {
         load(a.w + at, a.n - at, w);
-        load_h<TX, TR, RES>(a, row, at, v);
-        if (RES) store(out + at, a.n - at, v);
+        if (RES) load(out + at, a.n - at, h);
+        else load_h<TX, TR, RES>(a, row, at, h);
+    };
+    auto again = [&](int at) {
+        if (NV > 0) return;
+        float h[kChunk], w[kChunk];
+        load_again(at, h, w);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) t[0][i] = h[i] * w[i];
+    };
+    auto exact = [&](int at) {  // (at < n)
+        const float h = RES ? csdr::to_f32(out[at])
+                            : csdr::to_f32(static_cast<const TX*>(a.x)[row * a.x_stride + at]);
+        return (double)h * (double)a.w[at];
+    };
+    const TX* px = static_cast<const TX*>(a.x) + row * a.x_stride;
+    const TR* pr = static_cast<const TR*>(a.residual) + row * a.residual_stride;
+    auto take = [&](int j, int at, const Vec<TX>& x, const Vec<TR>& res, const Vec<float>& wv) {
+        float h[kChunk], w[kChunk], u[kChunk];
+        values_of(wv, a.w, at, a.n, w);
+        values_of(x, px, at, a.n, h);
+        if (RES) {
+            values_of(res, pr, at, a.n, u);
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) h[i] = (float)(TR)(h[i] + u[i]);
+            store(out + at, a.n - at, h);
+        }
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
-            sum = fma((double)v[i], (double)v[i], sum);
-            top = larger(top, fabs((double)v[i] * (double)w[i]));
+            t[j][i] = h[i] * w[i];
+            r.sum = fma((double)h[i], (double)h[i], r.sum);
+            r.most = max(r.most, magnitude(t[j][i]));
         }
     };
-    if (NV > 0) {
+    Vec<TX> x[N];
+    Vec<TR> res[N];
+    Vec<float> wv[N];
+    auto fetch = [&](int j, int at) {
+        x[j] = raw_of(px, at, a.n);
+        if (RES) res[j] = raw_of(pr, at, a.n);
+        wv[j] = raw_of(a.w, at, a.n);
+    };
+    if (NV > 0 && a.n >= kChunk) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (first + j * step < a.n) take(h[j], first + j * step);
-    } else {
-        for (int at = first; at < a.n; at += step) take(h[0], at);
+        for (int j = 0; j < N; ++j) fetch(j, first + j * step);
     }
-    const Row r = join({sum, top}, lds);
+    each(a.n, [&](int j, int at) {
+        if (NV == 0) fetch(0, at);
+        take(j, at, x[j], res[j], wv[j]);
+    });
+    const uint32_t mine = r.most;
+    r = join<true>(r, lds);
+    const float top32 = __uint_as_float(r.most);
+    const bool wide = !(top32 >= kTiny) || top32 == INFINITY;
+    if (wide || __uint_as_float(mine) >= top32 * (1.0f - kValueOff)) {
+        each(a.n, [&](int j, int at) {
+            again(at);
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i)
+                if ((wide || fabsf(t[j][i]) >= top32 * (1.0f - kValueOff)) && at + i < a.n)
+                    atomicMax(&lds.top, (unsigned long long)bits_of(fabs(exact(at + i))));
+        });
+    }
+    __syncthreads();
     const double rms = 1.0 / sqrt(r.sum / a.n + (double)a.eps);
     // (a finite top beside a sum that is not: a weight of 0 under a value that is not finite)
-    const Scale s = scale_of(r.sum < INFINITY ? r.top : (double)NAN, rms);
+    const Scale s = scale_of(r.sum < INFINITY && top32 == top32 ? of_bits(lds.top) : (double)NAN, rms, wide);
     if (threadIdx.x == 0 && a.scales) a.scales[row] = s.value;
 
-    auto put = [&](const float* v, int at) {
-        float w[kChunk];
-        load(a.w + at, a.n - at, w);
-        if (a.codes) {
-            int c[kChunk];
+    if (a.codes)
+        each(a.pitch, [&](int j, int at) {
+            again(at);
+            put_codes(a.codes + row * a.pitch + at, t[j], s,
+                      [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
+        });
+    if (a.y)
+        each(a.n, [&](int, int at) {
+            float h[kChunk], w[kChunk];
+            load_again(at, h, w);
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) c[i] = code_of((double)v[i] * (double)w[i], s);
-            store_codes(a.codes + row * a.pitch + at, c);
-        }
-        if (a.y && at < a.n) {
-            float y[kChunk];
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) y[i] = (float)((double)v[i] * rms * (double)w[i]);
-            store(static_cast<TX*>(a.y) + row * a.n + at, a.n - at, y);
-        }
-    };
-    const int end = a.codes ? a.pitch : a.n;
-    if (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = first + j * step;
-            if (at >= a.n) {
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) h[j][i] = 0.0f;
-            }
-            if (at < end) put(h[j], at);
-        }
-    } else {
-        for (int at = first; at < end; at += step) {
-            // (where the stream is updated in place its old values are gone: the sums are read back)
-            if (RES) load(out + at, a.n - at, h[0]);
-            else load_h<TX, TR, RES>(a, row, at, h[0]);
-            put(h[0], at);
-        }
-    }
+            for (int i = 0; i < kChunk; ++i) h[i] = (float)((double)h[i] * rms * (double)w[i]);
+            store(static_cast<TX*>(a.y) + row * a.n + at, a.n - at, h);
+        });
 }
 
 // ------------------------------------------------------------------ rows as they are, or gated
@@ -232,118 +349,99 @@ struct RowsArgs {
     int n, pitch;
 };
 
-// How far a gated value computed in fp32 may be off, of itself, and its code, with both to spare.
-constexpr float kGatedOff = 2e-6f, kCodeOff = 2e-4f;
-// In fp64 throughout: rows whose largest value is below kTiny, whose smaller ones fp32 holds with few
-// bits or none; values whose gate is below kLow, where the exponential passes fp32.
-constexpr float kTiny = 1e-30f, kLow = -88.0f;
-
-__device__ __forceinline__ float gated(float g, float x) { return g / (1.0f + expf(-g)) * x; }
+// silu(g) x. exp(-g) = 2^p (1 + rest ln 2), p and the rest of its rounding from two parts of 1 / ln 2, so that a
+// large gate costs no bits; beyond kLow the gate is held where the exponential is still a number, and above 150 it is
+// nothing beside 1.
+__device__ __forceinline__ float gated(float g, float x) {
+    constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596299e-8f, kLn2 = 0.69314718f;
+    const float v = __builtin_amdgcn_fmed3f(-g, -150.0f, 88.0f), p = v * kHi;
+    const float rest = fmaf(v, kLo, fmaf(v, kHi, -p));
+    const float e2 = __builtin_amdgcn_exp2f(p), e = fmaf(e2, rest * kLn2, e2);
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * x;
+}
 __device__ __forceinline__ double gated(double g, double x) { return g / (1.0 + exp(-g)) * x; }
 
 template <typename T, bool GATE, int NV>
 __global__ __launch_bounds__(kMaxThreads) void rows_kernel(RowsArgs a) {
-    __shared__ Row lds[kMaxThreads / 64];
-    __shared__ unsigned long long exact_top;
+    __shared__ Shared lds;
     const long long row = blockIdx.x;
     const int step = blockDim.x * kChunk, first = threadIdx.x * kChunk;
     constexpr int N = NV > 0 ? NV : 1;
-    float x[N][kChunk], g[N][GATE ? kChunk : 1];
+    float t[N][kChunk] = {};
+    Joined r = {0.0, 0, false};
     const T* px = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* pg = static_cast<const T*>(a.gate) + row * a.gate_stride;
-    uint32_t most = 0;  // bits of the largest magnitude; a NaN's are larger than any number's
 
-    auto take = [&](float* v, float* u, int at) {
-        load(px + at, a.n - at, v);
-        if (GATE) load(pg + at, a.n - at, u);
-    };
-    auto value = [&](const float* v, const float* u, int i) { return GATE ? gated(u[i], v[i]) : v[i]; };
-    auto look = [&](const float* v, const float* u) {
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i)
-            most = max(most, __float_as_uint(value(v, u, i)) & 0x7FFFFFFFu);
-    };
-    if (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = first + j * step;
-            if (at < a.n) {
-                take(x[j], g[j], at);
-                look(x[j], g[j]);
-            }
-        }
-    } else {
-        for (int at = first; at < a.n; at += step) {
-            take(x[0], g[0], at);
-            look(x[0], g[0]);
-        }
-    }
-    if (GATE && threadIdx.x == 0) exact_top = 0;
-    const Row r = join({0.0, (double)__uint_as_float(most)}, lds);
-    const float top32 = (float)r.top;
-    double top = r.top;
-    const bool tiny = GATE && top32 < kTiny;
-    if (GATE) {
-        if (blockDim.x <= 64) __syncthreads();  // (else join has had one)
-        auto check = [&](const float* v, const float* u) {
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i)
-                if (fabsf(value(v, u, i)) >= top32 * (1.0f - kGatedOff) || u[i] < kLow || tiny)
-                    atomicMax(&exact_top, (unsigned long long)bits_of(fabs(
-                                              gated((double)u[i], (double)v[i]))));
-        };
+    auto each = [&](int end, auto f) {
         if (NV > 0) {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (first + j * step < a.n) check(x[j], g[j]);
+                if (first + j * step < end) f(j, first + j * step);
         } else {
-            for (int at = first; at < a.n; at += step) {
-                take(x[0], g[0], at);
-                check(x[0], g[0]);
+            for (int at = first; at < end; at += step) f(0, at);
+        }
+    };
+    Vec<T> x[N], gate[N];
+    auto fetch = [&](int j, int at) {
+        x[j] = raw_of(px, at, a.n);
+        if (GATE) gate[j] = raw_of(pg, at, a.n);
+    };
+    auto take = [&](int j, int at, bool look) {
+        float g[kChunk];
+        if (NV == 0) fetch(0, at);
+        values_of(x[j], px, at, a.n, t[j]);
+        if (GATE) {
+            values_of(gate[j], pg, at, a.n, g);
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+                // (in fp16 what the exponential loses is below kTiny / 127 of any row formed in fp32)
+                if (sizeof(T) == 4 && look) r.low |= g[i] < kLow;
+                t[j][i] = gated(g[i], t[j][i]);
             }
+        }
+    };
+    if (NV > 0 && a.n >= kChunk) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) fetch(j, first + j * step);
+    }
+    auto again = [&](int at) {
+        if (NV == 0) take(0, at, false);
+    };
+    auto exact = [&](int at) {  // (at < n)
+        const double x = (double)csdr::to_f32(px[at]);
+        return GATE ? gated((double)csdr::to_f32(pg[at]), x) : x;
+    };
+    each(a.n, [&](int j, int at) {
+        take(j, at, true);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) r.most = max(r.most, magnitude(t[j][i]));
+    });
+    const uint32_t mine = r.most;
+    r = join<false>(r, lds);
+    const float top32 = __uint_as_float(r.most);
+    double top = (double)top32;
+    bool wide = !(top32 >= kTiny);
+    if (GATE) {
+        wide = wide || r.low || top32 == INFINITY;
+        if (wide || __uint_as_float(mine) >= top32 * (1.0f - kValueOff)) {
+            each(a.n, [&](int j, int at) {
+                again(at);
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                    if ((wide || fabsf(t[j][i]) >= top32 * (1.0f - kValueOff)) && at + i < a.n)
+                        atomicMax(&lds.top, (unsigned long long)bits_of(fabs(exact(at + i))));
+            });
         }
         __syncthreads();
-        if (r.top < INFINITY) top = of_bits(exact_top);
+        if (top32 == top32) top = of_bits(lds.top);
     }
-    const Scale s = scale_of(top, 1.0);
+    const Scale s = scale_of(top, 1.0, wide);
     if (threadIdx.x == 0) a.scales[row] = s.value;
-    const float inv32 = (float)s.inv;
-
-    auto put = [&](const float* v, const float* u, int at) {
-        int c[kChunk];
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            if (GATE) {
-                const float q = value(v, u, i) * inv32, f = rintf(q);
-                c[i] = (int)f;
-                if (__builtin_expect(fabsf(fabsf(q - f) - 0.5f) < kCodeOff || u[i] < kLow || tiny, 0))
-                    c[i] = s.inv > 0.0 ? code_of(gated((double)u[i], (double)v[i]), s) : 0;
-            } else {
-                c[i] = code_of((double)v[i], s);
-            }
-            if (!(s.inv > 0.0)) c[i] = 0;
-        }
-        store_codes(a.codes + row * a.pitch + at, c);
-    };
-    if (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = first + j * step;
-            if (at >= a.n) {
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i) {
-                    x[j][i] = 0.0f;
-                    if (GATE) g[j][i] = 0.0f;
-                }
-            }
-            if (at < a.pitch) put(x[j], g[j], at);
-        }
-    } else {
-        for (int at = first; at < a.pitch; at += step) {
-            take(x[0], g[0], at);
-            put(x[0], g[0], at);
-        }
-    }
+    each(a.pitch, [&](int j, int at) {
+        again(at);
+        put_codes(a.codes + row * a.pitch + at, t[j], s,
+                  [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
+    });
 }
 
 // ------------------------------------------------------------------ back to values
@@ -369,18 +467,16 @@ __global__ __launch_bounds__(256) void values_kernel(const int8_t* codes, const 
     }
 }
 
-// Threads of a row and chunks a thread (0: more than four, which the registers do not hold).
+// Threads of a row and chunks a thread (0: more than the registers hold): one or two of them as long as 1024 threads
+// are enough. With a thread's loads on their way together that was best at every number of rows (4096 gated rows of
+// 11008 in fp16: 55 us with two, 59 with six; of 4864: 23 with two, 31 with one by 640 threads).
 struct Shape {
     int threads, nv;
 };
 Shape shape_of(int width) {
     const int chunks = (width + kChunk - 1) / kChunk;
-    Shape s;
-    s.threads = std::min(256, (chunks + 63) / 64 * 64);
-    if (chunks > 4 * 256) s.threads = std::min(kMaxThreads, (chunks / 4 + 63) / 64 * 64);
-    const int nv = (chunks + s.threads - 1) / s.threads;
-    s.nv = nv <= 1 ? 1 : nv == 2 ? 2 : nv <= 4 ? 4 : 0;
-    return s;
+    const int nv = chunks <= 512 ? 1 : chunks <= 2 * kMaxThreads ? 2 : chunks <= 4 * kMaxThreads ? 4 : 0;
+    return {nv ? ((chunks + nv - 1) / nv + 63) / 64 * 64 : kMaxThreads, nv};
 }
 
 template <typename TX, typename TR, bool RES>

@@ -32,14 +32,14 @@ def _pitch(n: int) -> int:
 
 def _rows(what: str, t, n=None) -> int:
     """The row stride of a (rows, n) tensor with a row's values side by side (0: one row)."""
-    if t.dim() != 2 or (n is not None and t.shape[1] != n) or \
-            (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, s = t.shape, t.stride()
+    if len(shape) != 2 or (n is not None and shape[1] != n) or (s[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what} must be (rows, {n or 'n'}) with a row's values side by side")
-    if t.shape[0] < 2:
+    if shape[0] < 2:
         return 0
-    if t.stride(0) < t.shape[1]:  # an expanded tensor, or rows that overlap
+    if s[0] < shape[1]:  # an expanded tensor, or rows that overlap
         raise ValueError(f"the rows of {what} overlap")
-    return t.stride(0)
+    return s[0]
 
 
 def _type(torch, dtype: str):
@@ -62,17 +62,11 @@ class Q8Rows:
         if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != _pitch(n) or \
                 not codes.is_contiguous():
             raise ValueError(f"codes must be a contiguous int8 tensor (rows, {_pitch(n)})")
-        if scales.dtype != torch.float32 or tuple(scales.shape) != (codes.shape[0],) or \
+        if scales.dtype != torch.float32 or scales.shape != (codes.shape[0],) or \
                 not scales.is_contiguous():
             raise ValueError("scales must be a contiguous float32 tensor, one per row")
         _on_device(torch, "codes and scales", codes, scales)
         self.codes, self.scales, self.n, self.rows = codes, scales, n, int(codes.shape[0])
-
-    @classmethod
-    def _new(cls, codes, scales, n, rows):
-        r = cls.__new__(cls)
-        r.codes, r.scales, r.n, r.rows = codes, scales, n, rows
-        return r
 
     @classmethod
     def pack(cls, codes, scales) -> "Q8Rows":
@@ -95,20 +89,29 @@ class Q8Rows:
             _out("out", out, dt, self.rows, self.n)
         dev = _on_device(torch, "tensors", self.codes, self.scales, out)
         if self.rows:
-            _check(_lib.load().csdr_q8_dequantize(
+            rc = _lib.load().csdr_q8_dequantize(
                 self.codes.data_ptr(), self.scales.data_ptr(), _int(self.rows), self.n, out.data_ptr(),
-                int(dtype == "f16"), _stream_of(torch, dev, stream)))
+                int(dtype == "f16"), _stream_of(torch, dev, stream))
+            if rc:
+                _check(rc)
         return out
 
 
 def _out(what: str, t, dt, rows, n) -> None:
-    if t.dtype != dt or tuple(t.shape) != (rows, n) or not t.is_contiguous():
+    if t.dtype != dt or t.shape != (rows, n) or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dt} tensor ({rows}, {n})")
 
 
 def _new_rows(torch, rows, n, device, stream) -> Q8Rows:
-    return Q8Rows._new(_empty(torch, (rows, _pitch(n)), torch.int8, device, stream),
-                       _empty(torch, (rows,), torch.float32, device, stream), n, rows)
+    r = Q8Rows.__new__(Q8Rows)
+    r.n, r.rows = n, rows
+    if stream is None:
+        r.codes = torch.empty((rows, _pitch(n)), dtype=torch.int8, device=device)
+        r.scales = torch.empty(rows, dtype=torch.float32, device=device)
+    else:
+        r.codes = _empty(torch, (rows, _pitch(n)), torch.int8, device, stream)
+        r.scales = _empty(torch, (rows,), torch.float32, device, stream)
+    return r
 
 
 def quantize(x, gate=None, stream=None) -> Q8Rows:
@@ -126,9 +129,11 @@ def quantize(x, gate=None, stream=None) -> Q8Rows:
     dev = _on_device(torch, "tensors", x, gate)
     r = _new_rows(torch, rows, n, x.device, stream)
     if rows:
-        _check(_lib.load().csdr_q8_quantize(
+        rc = _lib.load().csdr_q8_quantize(
             x.data_ptr(), gate.data_ptr() if gate is not None else None, dt, _int(rows), n, xs, gs,
-            r.codes.data_ptr(), r.scales.data_ptr(), _stream_of(torch, dev, stream)))
+            r.codes.data_ptr(), r.scales.data_ptr(), _stream_of(torch, dev, stream))
+        if rc:
+            _check(rc)
     return r
 
 
@@ -146,7 +151,7 @@ def rms_norm(x, w, eps: float = 1e-5, residual=None, residual_out=None, q8: bool
     torch = _torch()
     dt, xs = _dtype(x), _rows("x", x)
     rows, n = x.shape
-    if w.dtype != torch.float32 or tuple(w.shape) != (n,) or not w.is_contiguous():
+    if w.dtype != torch.float32 or w.shape != (n,) or not w.is_contiguous():
         raise ValueError("w must be a contiguous float32 tensor, one per column")
     if not (q8 or y):
         raise ValueError("ask for q8, y or both")
@@ -165,11 +170,13 @@ def rms_norm(x, w, eps: float = 1e-5, residual=None, residual_out=None, q8: bool
     r = _new_rows(torch, rows, n, x.device, stream) if q8 else None
     yt = _empty(torch, (rows, n), x.dtype, x.device, stream) if y else None
     if rows:
-        _check(_lib.load().csdr_add_rms_norm(
+        rc = _lib.load().csdr_add_rms_norm(
             x.data_ptr(), dt, xs, residual.data_ptr() if residual is not None else None, rdt, rs,
             residual_out.data_ptr() if residual is not None else None, w.data_ptr(), eps, _int(rows),
             _int(n), yt.data_ptr() if y else None, r.codes.data_ptr() if q8 else None,
-            r.scales.data_ptr() if q8 else None, _stream_of(torch, dev, stream)))
+            r.scales.data_ptr() if q8 else None, _stream_of(torch, dev, stream))
+        if rc:
+            _check(rc)
     return Normed(r, yt, residual_out)
 
 
@@ -181,7 +188,7 @@ def linear(w: Q8Rows, x: Q8Rows, bias=None, add=None, dtype: str = "f32", out=No
     dt = _type(torch, dtype)
     if w.n != n:
         raise ValueError(f"w has rows of {w.n} values, x of {n}")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (R,) or
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (R,) or
                              not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous float32 tensor, one per row of w")
     ads = 0
@@ -197,10 +204,12 @@ def linear(w: Q8Rows, x: Q8Rows, bias=None, add=None, dtype: str = "f32", out=No
             raise ValueError(f"out must be ({M}, {R}) of {dtype}")
     dev = _on_device(torch, "tensors", w.codes, w.scales, x.codes, x.scales, bias, add, out)
     if M and R:
-        _check(_lib.load().csdr_q8_linear(
+        rc = _lib.load().csdr_q8_linear(
             w.codes.data_ptr(), w.scales.data_ptr(), _int(R), x.codes.data_ptr(), x.scales.data_ptr(),
             _int(M), n,
             bias.data_ptr() if bias is not None else None,
             add.data_ptr() if add is not None else None, ads, out.data_ptr(), int(dtype == "f16"),
-            os, _stream_of(torch, dev, stream)))
+            os, _stream_of(torch, dev, stream))
+        if rc:
+            _check(rc)
     return out

@@ -70,24 +70,30 @@ class Rotary:
         self._layout = LAYOUTS[layout]
         self._turns = torch.tensor([f / (2 * math.pi) for f in freqs], dtype=torch.float64,
                                    device="cuda")
+        self._at = self._turns.data_ptr()
+        self._call = _lib.load().csdr_rotary
 
-    def _side(self, torch, what, x, out, n, stream):
-        """Heads and strides of x and of its output, which is made if there is none."""
-        hd = self.head_dim
-        strides = []
-        for name, t in ((what, x), (what + "_out", out)):
-            if t is None:
-                t = out = _empty(torch, tuple(x.shape), x.dtype, x.device, stream)
-            if t.dim() != 3 or t.shape[2] != hd or t.stride(2) != 1 or \
-                    (t.shape[1] > 1 and t.stride(1) != hd) or t.shape[1] < 1:
-                raise ValueError(f"{name} must be (tokens, heads, {hd}) with a token's values side "
-                                 "by side")
-            if t.shape[0] != n or t.dtype != x.dtype or t.shape[1] != x.shape[1]:
-                raise ValueError(f"{name}: other tokens, heads or type")
-            if n > 1 and t.stride(0) < t.shape[1] * hd:
-                raise ValueError(f"{name}: its tokens overlap")
-            strides.append(t.stride(0) if n > 1 else 0)
-        return out, x.shape[1], strides[0], strides[1]
+    def _stride(self, what: str, x, n: int) -> int:
+        """The token stride of (n, heads, head_dim) with a token's values side by side (0: one token)."""
+        shape, hd = x.shape, self.head_dim
+        if len(shape) == 3 and shape[0] == n and shape[2] == hd and shape[1] > 0:
+            s = x.stride()
+            if s[2] == 1 and (s[1] == hd or shape[1] == 1):
+                if n < 2:
+                    return 0
+                if s[0] >= shape[1] * hd:
+                    return s[0]
+                raise ValueError(f"{what}: its tokens overlap")
+        raise ValueError(f"{what} must be ({n}, heads, {hd}) with a token's values side by side")
+
+    def _out(self, torch, what, x, out, n, stream):
+        """Where x's heads go, and its token stride."""
+        if out is None:
+            return (x.new_empty(x.shape) if stream is None else
+                    _empty(torch, x.shape, x.dtype, x.device, stream)), 0
+        if out.dtype != x.dtype or out.shape != x.shape:
+            raise ValueError(f"{what}: other tokens, heads or type")
+        return out, self._stride(what, out, n)
 
     def apply(self, q, positions, k=None, q_out=None, k_out=None, stream=None):
         """q and k (tokens, heads, head_dim), float32 or float16 with tokens any stride apart, turned
@@ -95,23 +101,27 @@ class Rotary:
         (in place). A token with a negative position is none: its rows are not written."""
         torch = _torch()
         dt, n = _dtype(q), q.shape[0]
-        if positions.dtype != torch.int32 or tuple(positions.shape) != (n,) or \
+        if positions.dtype != torch.int32 or positions.shape != (n,) or \
                 not positions.is_contiguous():
             raise ValueError("positions must be a contiguous int32 tensor, one per token")
-        q_out, hq, qs, qos = self._side(torch, "q", q, q_out, n, stream)
+        qs = self._stride("q", q, n)
+        q_out, qos = self._out(torch, "q_out", q, q_out, n, stream)
         hk = ks = kos = 0
+        kp = kop = None
         if k is not None:
             if k.dtype != q.dtype:
                 raise ValueError("q and k must have the same type")
-            k_out, hk, ks, kos = self._side(torch, "k", k, k_out, n, stream)
+            ks, hk = self._stride("k", k, n), k.shape[1]
+            k_out, kos = self._out(torch, "k_out", k, k_out, n, stream)
+            kp, kop = k.data_ptr(), k_out.data_ptr()
         elif k_out is not None:
             raise ValueError("k_out without k")
         dev = _on_device(torch, "tensors", q, k, q_out, k_out, positions, self._turns)
         if n:
-            _check(_lib.load().csdr_rotary(
-                q.data_ptr(), q_out.data_ptr(), _int(hq), qs, qos,
-                k.data_ptr() if k is not None else None,
-                k_out.data_ptr() if k is not None else None, _int(hk), ks, kos, dt, _int(n), self.head_dim,
-                self.dims, self._layout, positions.data_ptr(), self._turns.data_ptr(),
-                self.magnitude, _stream_of(torch, dev, stream)))
+            rc = self._call(q.data_ptr(), q_out.data_ptr(), _int(q.shape[1]), qs, qos, kp, kop, _int(hk),
+                            ks, kos, dt, _int(n), self.head_dim, self.dims, self._layout,
+                            positions.data_ptr(), self._at, self.magnitude,
+                            _stream_of(torch, dev, stream))
+            if rc:
+                _check(rc)
         return q_out if k is None else (q_out, k_out)
