@@ -27,9 +27,12 @@ def silu_mul(gate, x):
     return g / (1 + np.exp(-g)) * x
 
 
-def linear(xc, xs, wc, ws, bias=None, add=None):
+def sums(xc, wc):
+    return xc.astype(np.float64) @ wc.astype(np.float64).T  # exact: below 2^53
+
+
+def linear(sums, xs, ws, bias=None, add=None):
     """The product and the sum of its terms' magnitudes, fp64."""
-    sums = xc.astype(np.float64) @ wc.astype(np.float64).T  # exact: below 2^53
     p = sums * xs.astype(np.float64)[:, None] * ws.astype(np.float64)
     mag = np.abs(p)
     if bias is not None:

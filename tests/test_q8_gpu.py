@@ -221,6 +221,9 @@ def test_norm_ranges(gpu):
         assert (np.abs(y[i] - want) <= np.abs(want) * U32 * 1.001 + 2.0 ** -150).all()
     zero = q8.rms_norm(dev(gpu, x[:1]), gpu.zeros(n, device="cuda"))
     assert zero.rows.scales.item() == 0 and not zero.rows.codes.any()
+    # without eps a row of zeros has no norm
+    none = q8.rms_norm(gpu.zeros(2, 100, device="cuda"), gpu.ones(100, device="cuda"), 0.0, y=True)
+    assert gpu.isnan(none.rows.scales).all() and not none.rows.codes.any() and gpu.isnan(none.y).all()
     nan = q8.rms_norm(dev(gpu, x[:1]), gpu.full((n,), float("nan"), device="cuda"))
     assert gpu.isnan(nan.rows.scales).all() and not nan.rows.codes.any()
 
@@ -239,7 +242,11 @@ def random_rows(torch, rows, n, seed, whole=False):
 
 
 def check_linear(y, xc, xs, wc, ws, bias=None, add=None):
-    p, mag = q8_ref.linear(xc, xs, wc, ws, bias, add)
+    check_sums(y, q8_ref.sums(xc, wc), xs, ws, bias, add)
+
+
+def check_sums(y, sums, xs, ws, bias=None, add=None):
+    p, mag = q8_ref.linear(sums, xs, ws, bias, add)
     y = y.cpu().numpy()
     half = y.dtype == np.float16
     # fp32: the sum's conversion, two scales, two additions; then one rounding to the type
@@ -248,10 +255,25 @@ def check_linear(y, xc, xs, wc, ws, bias=None, add=None):
     assert (np.abs(y - p)[~over] <= tol[~over]).all(), np.max((np.abs(y - p) - tol)[~over])
 
 
-PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 17, 130), (2, 1152, 896), (3, 5, 4096), (5, 33, 1000), (16, 896, 4864),
-            (17, 100, 777), (31, 257, 128), (33, 64, 300), (64, 1001, 999), (65, 129, 640), (100, 300, 1),
-            (127, 255, 513), (129, 257, 1024), (255, 511, 384), (256, 512, 896), (300, 1152, 896),
-            (333, 1001, 4999), (515, 700, 129), (1000, 130, 2000), (1030, 1290, 257)]
+# By the tile that the rule takes for them (rows x tokens); each with rests of rows and tokens, with fewer steps of
+# 128 columns than stages in flight and with more
+PRODUCTS = [
+    # 16 x 16, four waves sharing the columns
+    (1, 1, 1), (1, 16, 64), (1, 17, 130), (2, 1152, 896), (3, 5, 4096), (5, 33, 1000), (16, 896, 4864),
+    (17, 100, 777), (31, 257, 128), (33, 64, 300), (64, 1001, 999), (129, 257, 1024), (255, 511, 384),
+    # 32 x 32, two waves sharing the columns
+    (256, 512, 896), (300, 1152, 896), (515, 700, 129), (1000, 130, 2000), (64, 4096, 1100),
+    # 32 x 64
+    (333, 1001, 4999), (420, 1003, 3000),
+    # 64 x 64
+    (520, 4090, 100), (600, 1500, 1), (2, 33000, 257),
+    # 128 x 64
+    (1, 22001, 300), (1, 22016, 1), (260, 11001, 700), (900, 2100, 140), (1030, 1290, 257),
+    # 128 x 128
+    (1500, 3000, 130),
+    # 256 x 256
+    (3900, 4090, 1000), (3901, 3900, 385),
+]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -264,19 +286,20 @@ def test_linear(gpu, M, R, C, dtype):
     if dtype == "f16":  # keep within fp16
         ws = (ws / C).astype(np.float32)
         w = q8.Q8Rows.pack(dev(gpu, wc), dev(gpu, ws))
-    check_linear(q8.linear(w, x, dtype=dtype), xc, xs, wc, ws)
+    sums = q8_ref.sums(xc, wc)
+    check_sums(q8.linear(w, x, dtype=dtype), sums, xs, ws)
     r = np.random.default_rng(C)
     bias = r.standard_normal(R).astype(np.float32)
     add = r.standard_normal((M, R)).astype(NP[dtype])
-    check_linear(q8.linear(w, x, bias=dev(gpu, bias), dtype=dtype), xc, xs, wc, ws, bias)
-    check_linear(q8.linear(w, x, add=dev(gpu, add), dtype=dtype), xc, xs, wc, ws, None, add)
+    check_sums(q8.linear(w, x, bias=dev(gpu, bias), dtype=dtype), sums, xs, ws, bias)
+    check_sums(q8.linear(w, x, add=dev(gpu, add), dtype=dtype), sums, xs, ws, None, add)
     # into rows of a larger buffer at an odd offset, onto what they hold
     wide = gpu.full((M, R + 7), 5.0, dtype=getattr(gpu, "float32" if dtype == "f32" else "float16"),
                     device="cuda")
     out = wide[:, 3:3 + R]
     out.copy_(dev(gpu, add))
     y = q8.linear(w, x, bias=dev(gpu, bias), add=out, dtype=dtype, out=out)
-    check_linear(y, xc, xs, wc, ws, bias, add)
+    check_sums(y, sums, xs, ws, bias, add)
     assert (wide[:, :3] == 5).all() and (wide[:, 3 + R:] == 5).all()
 
 
@@ -349,6 +372,45 @@ def test_linear_far(gpu, rows):
         assert torch.equal(y[i], v[i] * v), i
     del y
     torch.cuda.empty_cache()
+
+
+def test_norm_past_fp32(gpu):
+    """Values whose products with the weights pass fp32, and some that leave its normal numbers."""
+    from cortexsdr_amd import q8
+
+    x = activations(4, 500, "f32", seed=21)
+    x[0] *= np.float32(1e37)
+    x[1] *= np.float32(1e-37)
+    x[2, 7] = 3e38
+    w = (1 + np.random.default_rng(3).random(500)).astype(np.float32) * np.float32(50)
+    w[::3] = np.float32(1e-30)
+    for n in (500, 499):
+        r = q8.rms_norm(dev(gpu, x[:, :n]), dev(gpu, w[:n]), 1e-5)
+        rms, t = norm_parts(x[:, :n], w[:n], 1e-5)
+        check_rows(r.rows, t, rms, extra=(n + 8) * 2.0 ** -52)
+
+
+def test_streams(gpu):
+    """Products and norms on two streams at once, each with its own outputs."""
+    from cortexsdr_amd import q8
+
+    torch = gpu
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    sets = []
+    for i in range(2):
+        xc, xs, x = random_rows(torch, 200 + i, 700, seed=i)
+        wc, ws, w = random_rows(torch, 900, 700, seed=i + 5)
+        sets.append((x, w, torch.randn(300, 4000 + i, device="cuda"), torch.ones(4000 + i, device="cuda")))
+    want = [(q8.linear(w, x), q8.rms_norm(v, n).rows.codes) for x, w, v, n in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate((a, b)):
+            x, w, v, n = sets[i]
+            got[i].append((q8.linear(w, x, stream=st), q8.rms_norm(v, n, stream=st).rows.codes))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i][0]) and torch.equal(c, want[i][1]) for y, c in got[i])
 
 
 def test_python_refusals(gpu):
