@@ -1,7 +1,20 @@
 // q8_linear.hip — products of 8-bit rows on the integer matrix cores (gfx950):
 //   y[m][r] = x_scales[m] * w_scales[r] * sum_c x[m][c] w[r][c] (+ bias[r]) (+ add[m][r])
-// The sums are exact (32-bit integers), so no order of summation shows in the result: it is rounded as
-// a sum is converted to fp32, by two products and the additions in fp32, and once to y's type.
+// The sums are exact (32-bit integers), so no order of summation shows in the result: it is rounded as a sum is
+// converted to fp32, by two products and the additions in fp32, and once to y's type.
+//
+// One kernel, seven tiles. Rows of codes come from memory straight into LDS (no register, no instruction of the
+// waves between), several stages ahead; a wave reads its operands for the next half step while the matrix cores
+// work on this one, with one barrier a stage. What bounds it, by the number of tokens (times of launches in a
+// graph):
+//   one to 16    the stream of the weights: 22016 x 4096 for one token 18 us, 5.0 TB/s; small ones the chain of a
+//                launch, first loads, barrier, sums (1152 x 896 2.7 us)
+//   up to some   what a CU takes from L2, 30 to 42 bytes a cycle: 64 tokens, 4096 x 11008, 12.8 us; there large tiles
+//   hundreds     take fewer bytes and leave CUs without work, so tiles are chosen by what they cost (kCosts)
+//   thousands    the matrix cores at the clock that they can be fed at: 4096 tokens, 4096 x 11008, 135 us, 2.74
+//                POPS, 65% of the cycles at 1.97 GHz (nothing but the products runs at 1.9 GHz, 3.9 POPS; taking the
+//                same rows for every tile, so that all loads hit L2, changes nothing, nor does the order of
+//                loads, reads and products, nor the waves' priority); 12 us of it start and end, 67 MB of y and `add`
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -119,9 +132,9 @@ __device__ __forceinline__ void arrived() {
 }
 
 // sum += w . x. Written out so that the sums stay where they are: from the builtin the compiler gives results
-// other registers than their operands, and with all 256 accumulator registers in use copies them about in every
-// step. The next product of the same sum is (FR FM - 1) products away; the last ones are builtins, so that the
-// compiler knows what to wait for before it reads a sum.
+// other registers than their operands, and copies them about in every step of the larger tiles. The next
+// product of the same sum is three others away at least, longer than one takes; the last ones are builtins, so
+// that the compiler knows what to wait for before it reads a sum.
 #ifdef __HIP_DEVICE_COMPILE__  // (the host's pass knows no such registers)
 __device__ __forceinline__ void product(i4& sum, const i4& w, const i4& x) {
     asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(sum) : "v"(w), "v"(x));
@@ -136,8 +149,8 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
     extern __shared__ __attribute__((aligned(128))) int8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, eight columns of tokens by
-    // as many rows as it has, so that its L2 serves what they share.
+    // Workgroups go to the eight XCDs in turn: each XCD takes a run of tiles, eight tiles of tokens by
+    // as many of rows as it has, so that its L2 serves what they share.
     int tr, tm;
     {
         const int n = tiles_r * tiles_m, b = blockIdx.x, per = n / 8, rest = n % 8;
@@ -198,8 +211,8 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
         for (int j = 0; j < FM; ++j)
             if constexpr (OUT) asm volatile("" : "+a"(acc[i][j]));  // (zero while the first loads run)
 
-    // The products of half a step, with the reads of the next half's operands (NR of them) and loads (NL) spread
-    // over the first three quarters of them.
+    // The products of half a step, with the reads of the next half's operands (NR of them) and loads (NL)
+    // spread over the first three quarters of them.
     auto multiply = [&](int half, auto nr, int read_buf, auto nl, int load_buf, int load_step) {
         constexpr int NR = decltype(nr)::value, NL = decltype(nl)::value, MOST = NR > NL ? NR : NL;
         constexpr int EACH = MOST == 0 ? N : N * 3 / 4 / MOST > 0 ? N * 3 / 4 / MOST : 1;
@@ -258,8 +271,9 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
         __builtin_amdgcn_sched_barrier(0);
     }
     // The sums go through LDS (token-major, 16-byte chunk c of token m at c ^ (m % 8)): a thread then has
-    // neighbouring rows for whole lines of y, and a short loop writes them, where straight code over the registers
-    // was 40 KB of instructions that came from memory at each launch, and one read of `add` after another.
+    // neighbouring rows for whole lines of y, and a short loop writes them, eight tokens' reads of `add`
+    // together. (Straight code over the registers was 30 KB of instructions, read for every tile, with one read
+    // of `add` after another: 163 us where this takes 137, for 4096 tokens onto a residual.)
     constexpr int CHUNKS = TR / 4, KEYS = CHUNKS < 8 ? CHUNKS : 8, PASSES = S::kPasses;
     constexpr int TOKENS = TM / PASSES, MINE = TOKENS / WM;      // of a pass, and of those a wave's
     constexpr int PER = S::kThreads / CHUNKS;                    // tokens at once
@@ -340,10 +354,13 @@ int launch_tiles(const Args& a, hipStream_t st) {
     return CSDR_OK;
 }
 
-// What a tile costs, in us: `fixed` for a workgroup's start and end, a step of 128 columns `alone` for one workgroup on
-// a CU and `each` for every one of `held` (as many as a CU's LDS holds). Fitted to products of 1 to 4096 tokens with
-// 4096 or 11008 rows and 896 to 11008 columns, which they give within a tenth to a fifth; the rule has only to tell
-// tiles apart.
+// What a tile costs, in us: `fixed` for a workgroup's start and end, a step of 128 columns `alone` for one
+// workgroup on a CU and `each` for every one of `held` (as many as a CU's LDS holds). Fitted to products of 1
+// to 4096 tokens with 1152 to 11008 rows and 896 to 11008 columns, which they give within a tenth to a fifth;
+// the rule has only to tell tiles apart. Both sides of its borders, measured for 4096 x 4096: 64 tokens 6.3 us
+// in tiles of 32 x 32, 8.1 of 32 x 64; 128 tokens 8.1 of 32 x 32, 8.2 of 32 x 64, 10.6 of 64 x 64; 512 tokens
+// 13.8 of 128 x 64, 15 of 64 x 64, 22.7 of 128 x 128; 2048 tokens 34 of 128 x 128, 42 of 128 x 64, 46 of 256 x
+// 256; 4096 tokens 58 of 256 x 256, 66 of 128 x 128.
 struct Cost {
     int tr, tm, held;
     float fixed, alone, each;

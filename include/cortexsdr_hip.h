@@ -692,8 +692,9 @@ CSDR_API int csdr_q8_dequantize(const int8_t* codes, const float* scales, int ro
 /* RMSNorm (rms_norm, cortex_sdk.cpp:1208-1232) with the residual's addition in front and 8-bit rows behind:
  * h = x, or x + residual rounded to residual_dtype and written to residual_out (rows x n, packed; it may
  * be residual itself where that is packed) if residual is not NULL; the norm h / sqrt(mean(h^2) + eps) * w
- * goes to codes and scales (both or neither), to y (rows x n, packed, of x's dtype; may be NULL), or to
- * both. Strides in elements, 0 = n. Outputs must not overlap inputs or each other otherwise. */
+ * (statistics in fp64; without eps a row of zeros is NaN) goes to codes and scales (both or neither), to
+ * y (rows x n, packed, of x's dtype; may be NULL), or to both. Strides in elements, 0 = n. Outputs must
+ * not overlap inputs or each other otherwise. */
 CSDR_API int csdr_add_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual,
                                int residual_dtype, int64_t residual_stride, void* residual_out,
                                const float* w, float eps, int rows, int n, void* y, int8_t* codes,
