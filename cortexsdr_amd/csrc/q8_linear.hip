@@ -393,7 +393,7 @@ int launch(const Args& a, hipStream_t st) {
         }
     }
     switch (best) {
-        case 0: return launch_tiles<T, 256, 256, 1, 2, 4, 2>(a, st);
+        case 0: return launch_tiles<T, 256, 256, 1, 4, 2, 2>(a, st);
         case 1: return launch_tiles<T, 128, 128, 1, 4, 2, 2>(a, st);
         case 2: return launch_tiles<T, 128, 64, 1, 2, 2, 3>(a, st);
         case 3: return launch_tiles<T, 64, 64, 1, 2, 2, 3>(a, st);
