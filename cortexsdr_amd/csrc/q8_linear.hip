@@ -40,23 +40,17 @@ struct Args {
     void* y;
     long long y_stride, add_stride;
     int R, M, pitch;
-    bool wide;  // four outputs at a multiple of four may be moved at once
 };
 
+// Four neighbouring values at any alignment of their type.
 template <typename T>
-struct Four;
-template <>
-struct Four<float> {
-    typedef float type __attribute__((ext_vector_type(4)));
-};
-template <>
-struct Four<_Float16> {
-    typedef _Float16 type __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T v[4];
 };
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 // The scales and biases of four neighbouring rows of w (the last one's again where there are fewer).
-__device__ __forceinline__ f4 four_of(const float* p, int r, int R) {
+[[maybe_unused]] __device__ __forceinline__ f4 four_of(const float* p, int r, int R) {
     f4 v;
     if (r + 3 < R) __builtin_memcpy(&v, p + r, 16);
     else
@@ -65,23 +59,18 @@ __device__ __forceinline__ f4 four_of(const float* p, int r, int R) {
     return v;
 }
 
-__device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
+[[maybe_unused]] __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
     return (float)sum * xs * ws + bias;
 }
 
-// Four neighbouring outputs of a token at once (a.wide, r + 3 < R, m < M).
+// Four neighbouring outputs of a token at once (r + 3 < R, m < M).
 template <typename T>
-__device__ __forceinline__ void finish_wide(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
-                                            const f4& bias, const typename Four<T>::type& add) {
-    typename Four<T>::type o;
+__device__ __forceinline__ void finish_four(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
+                                            const f4& bias, const Four<T>& add) {
+    Four<T> o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (float)add[i]);
-    *reinterpret_cast<typename Four<T>::type*>(static_cast<T*>(a.y) + m * a.y_stride + r) = o;
-}
-template <typename T>
-__device__ __forceinline__ typename Four<T>::type wide_added(const Args& a, int m, int r) {
-    using V = typename Four<T>::type;
-    return *reinterpret_cast<const V*>(static_cast<const T*>(a.add) + m * a.add_stride + r);
+    for (int i = 0; i < 4; ++i) o.v[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (float)add.v[i]);
+    *reinterpret_cast<Four<T>*>(static_cast<T*>(a.y) + m * a.y_stride + r) = o;
 }
 
 // One by one, as many of them as there are.
@@ -117,7 +106,7 @@ struct Tile {
     static_assert(KG * TR * TM * 4 <= kLds * kPasses && kLds <= 160 * 1024, "LDS");
 };
 
-constexpr int kRsrc = 0x00027000;  // a raw buffer
+[[maybe_unused]] constexpr int kRsrc = 0x00027000;  // a raw buffer
 
 // This wave's loads into LDS have arrived and its reads are done; then every wave's.
 // (LATER: loads of steps that need not have.)
@@ -278,13 +267,12 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
     constexpr int TOKENS = TM / PASSES, MINE = TOKENS / WM;      // of a pass, and of those a wave's
     constexpr int PER = S::kThreads / CHUNKS;                    // tokens at once
     constexpr int ROUNDS = TOKENS > PER ? TOKENS / PER : 1, BATCH = ROUNDS < 8 ? ROUNDS : 8;
-    using V = typename Four<T>::type;
     i4* part = reinterpret_cast<i4*>(lds);
     const int c = threadIdx.x % CHUNKS, mine = threadIdx.x / CHUNKS;
     const int r = r0 + 4 * c;
     const f4 ws = four_of(a.w_scales, min(r, a.R - 1), a.R);
     const f4 bias = a.bias ? four_of(a.bias, min(r, a.R - 1), a.R) : f4{};
-    const bool whole = a.wide && r + 3 < a.R;
+    const bool whole = r + 3 < a.R;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         arrived<0>();  // every wave is done with what lay there
@@ -308,18 +296,23 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
 #pragma unroll 1
             for (int k = mine; k < TOKENS; k += BATCH * PER) {
                 float xs[BATCH];
-                V add[BATCH] = {};
+                Four<T> add[BATCH] = {};
+                int m[BATCH];
 #pragma unroll
                 for (int q = 0; q < BATCH; ++q) {
-                    const int m = min(token(k + q * PER), a.M - 1);
-                    xs[q] = a.x_scales[m];
-                    if (a.add) add[q] = wide_added<T>(a, m, r);
+                    m[q] = token(k + q * PER);
+                    xs[q] = a.x_scales[min(m[q], a.M - 1)];
+                }
+                if (a.add) {
+#pragma unroll
+                    for (int q = 0; q < BATCH; ++q)
+                        add[q] = *reinterpret_cast<const Four<T>*>(
+                            static_cast<const T*>(a.add) + min(m[q], a.M - 1) * a.add_stride + r);
                 }
 #pragma unroll
-                for (int q = 0; q < BATCH; ++q) {
-                    const int m = token(k + q * PER);
-                    if (m < a.M) finish_wide<T>(a, m, r, sum_of(k + q * PER), xs[q], ws, bias, add[q]);
-                }
+                for (int q = 0; q < BATCH; ++q)
+                    if (m[q] < a.M)
+                        finish_four<T>(a, m[q], r, sum_of(k + q * PER), xs[q], ws, bias, add[q]);
             }
         } else if (r < a.R) {
 #pragma unroll 1
@@ -439,9 +432,6 @@ CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const
     a.R = R;
     a.M = M;
     a.pitch = (int)q8_pitch(C);
-    const size_t four = y_dtype == CSDR_F32 ? 16 : 8;
-    a.wide = a.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(y) % four == 0 &&
-             (!add || (a.add_stride % 4 == 0 && reinterpret_cast<uintptr_t>(add) % four == 0));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     const int rc = y_dtype == CSDR_F32 ? launch<float>(a, st) : launch<_Float16>(a, st);
     if (rc != CSDR_OK) return rc;

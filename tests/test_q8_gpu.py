@@ -94,6 +94,25 @@ def test_quantize_ranges(gpu, scale):
     check_rows(q8.quantize(dev(gpu, x), gate=dev(gpu, g)), q8_ref.silu_mul(g, x))
 
 
+@pytest.mark.parametrize("n", [40, 5000, 33000])
+def test_quantize_gated_past_fp32(gpu, n):
+    """Gated values past fp32 whose scale is not, and ones whose sigmoid leaves its normal numbers."""
+    from cortexsdr_amd import q8
+
+    g, x = activations(3, n, "f32", seed=n), activations(3, n, "f32", seed=n + 1)
+    x[0] *= np.float32(1e36)
+    x[0, 3], g[0, 3] = 3e38, 9.0
+    x[1] = 1e-3
+    x[1, ::7], g[1, ::7] = 1e37, -88.5
+    g[2, 1], x[2, 1] = -120.0, 3e38
+    r = q8.quantize(dev(gpu, x), gate=dev(gpu, g))
+    check_rows(r, q8_ref.silu_mul(g, x))
+    # and the scale past fp32 too
+    x[0, 3], g[0, 3] = 3e38, 3e38
+    r = q8.quantize(dev(gpu, x[:1]), gate=dev(gpu, g[:1]))
+    assert gpu.isnan(r.scales).all() and not r.codes.any()
+
+
 @pytest.mark.parametrize("n", [40, 700, 5000, 40000])
 @pytest.mark.parametrize("gate", [False, True])
 def test_quantize_not_finite(gpu, n, gate):
