@@ -6,7 +6,7 @@
 // The angle is held in turns in fp64 (an fp32 angle is off by 4e-3 rad at position 65536), its whole turns
 // dropped before the fp32 sine and cosine of what is left, at most half a turn. They are computed once per
 // token and pair and shared by the heads of a workgroup through LDS. A thread takes 8 pairs, 32 or 64 bytes in
-// and out. Bound by memory: 8192 tokens of 32 + 32 heads of 128 in fp16 take 56 us, 4.8 TB/s; a step's tokens
+// and out. Bound by memory: 8192 tokens of 32 + 32 heads of 128 in fp16 take 45 us, 5.9 TB/s; a step's tokens
 // one round trip (64 of 32 + 8 heads 3.3 us).
 #include <hip/hip_runtime.h>
 
@@ -40,96 +40,109 @@ struct Args {
     Side q, k;
     const int32_t* positions;
     const double* turns;  // frequencies / 2 pi, of pair j
-    int n_tokens, hd, dims, groups;
+    int n_tokens, hd, dims, groups, tokens;  // workgroups of a token, or tokens of a workgroup
     float magnitude;
 };
 
-// A workgroup per token and group of heads. WIDE: 8 pairs a thread; else one.
+// A workgroup per token and group of heads, or several tokens of few heads. WIDE: 8 pairs a thread; else one. A
+// thread's first items are on their way while the sines and cosines are formed (8192 tokens of 64 heads 57 -> 45 us).
 template <typename T, bool HALVES, bool WIDE>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(Args a) {
     __shared__ float2 cs[kMaxDim / 2];
-    const int token = blockIdx.x / a.groups, group = blockIdx.x % a.groups;
-    const int pos = a.positions[token];
-    if (pos < 0) return;  // no token
-    const int half = a.dims / 2;
-    for (int j = threadIdx.x; j < half; j += kThreads) {
-        const double u = (double)pos * a.turns[j];
-        const float f = (float)(u - rint(u));
+    const int first = (int)(blockIdx.x / a.groups) * a.tokens, group = blockIdx.x % a.groups;
+    const int half = a.dims / 2, tokens = min(a.tokens, a.n_tokens - first);
+    // items of a head: its pairs, then its other dims (the last one alone where they are odd)
+    constexpr int P = WIDE ? kUnit : 1, O = 2 * P, AHEAD = 2;
+    const int turned = half / P, items = turned + (a.hd - a.dims) / O + (WIDE ? 0 : (a.hd - a.dims) % O);
+    const int each = (a.q.heads + a.k.heads) * items, all = tokens * each, step = a.groups * kThreads;
+
+    // what item i is: where its two pieces lie, and which sines are its pairs' (-1: none, as they are)
+    struct Item {
+        const T* in;
+        T* out;
+        int second, pair;
+        bool one, none;
+    };
+    auto item_of = [&](int i) {
+        const int local = tokens > 1 ? i / each : 0, head = (i - local * each) / items, item = i % items;
+        const int token = first + local;
+        const bool is_k = head >= a.q.heads;
+        const Side& s = is_k ? a.k : a.q;
+        const long long h = (long long)(is_k ? head - a.q.heads : head) * a.hd;
+        const bool pairs = item < turned;
+        const int at = pairs ? (HALVES ? item * P : item * O) : a.dims + (item - turned) * O;
+        Item t;
+        t.in = static_cast<const T*>(s.in) + token * s.in_stride + h + at;
+        t.out = static_cast<T*>(s.out) + token * s.out_stride + h + at;
+        t.second = HALVES && pairs ? half : P;
+        t.pair = pairs ? local * half + item * P : -1;
+        t.none = a.positions[token] < 0;  // no token
+        t.one = !WIDE && at + 1 == a.hd;
+        return t;
+    };
+    using V = Vec<T, P>;
+    auto load = [&](const Item& t, V& u, V& v) {
+        u = *reinterpret_cast<const V*>(t.in);
+        v = *reinterpret_cast<const V*>(t.in + (t.one ? 0 : t.second));
+    };
+    auto put = [&](const Item& t, const V& u, const V& v) {
+        if (t.none) return;
+        V p = u, w = v;
+        if (t.pair >= 0) {
+            float x[O];  // (u, v) of the pairs, one after the other
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                x[HALVES ? 2 * e : e] = csdr::to_f32(u.v[e]);
+                x[HALVES ? 2 * e + 1 : P + e] = csdr::to_f32(v.v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                const float2 c = cs[t.pair + e];
+                const float y = x[2 * e] * c.x - x[2 * e + 1] * c.y;
+                x[2 * e + 1] = x[2 * e] * c.y + x[2 * e + 1] * c.x;
+                x[2 * e] = y;
+            }
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                p.v[e] = (T)x[HALVES ? 2 * e : e];
+                w.v[e] = (T)x[HALVES ? 2 * e + 1 : P + e];
+            }
+        }
+        *reinterpret_cast<V*>(t.out) = p;
+        if (!t.one) *reinterpret_cast<V*>(t.out + t.second) = w;
+    };
+
+    const int mine = group * kThreads + threadIdx.x;
+    Item t[AHEAD];
+    V u[AHEAD], v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (i * step < all) {
+            t[i] = item_of(min(mine + i * step, all - 1));
+            load(t[i], u[i], v[i]);
+        }
+    for (int j = threadIdx.x; j < tokens * half; j += kThreads) {
+        const int local = tokens > 1 ? j / half : 0;
+        const double r = (double)a.positions[first + local] * a.turns[j - local * half];
+        const float f = (float)(r - rint(r));
         float s, c;
         sincospif(2.0f * f, &s, &c);
         cs[j] = make_float2(c * a.magnitude, s * a.magnitude);
     }
     __syncthreads();
-    // items of a head: its pairs, then its other dims
-    constexpr int P = WIDE ? kUnit : 1, O = 2 * P;
-    const int turned = half / P, items = turned + (a.hd - a.dims) / O + (WIDE ? 0 : (a.hd - a.dims) % O);
-    const int heads = a.q.heads + a.k.heads;
-    for (int i = group * kThreads + threadIdx.x; i < heads * items; i += a.groups * kThreads) {
-        const int head = i / items, item = i % items;
-        const bool is_k = head >= a.q.heads;
-        const Side& s = is_k ? a.k : a.q;
-        const int h = is_k ? head - a.q.heads : head;
-        const T* in = static_cast<const T*>(s.in) + token * s.in_stride + (long long)h * a.hd;
-        T* out = static_cast<T*>(s.out) + token * s.out_stride + (long long)h * a.hd;
-        if (item >= turned) {  // as they are
-            const int at = a.dims + (item - turned) * O;
-            if (in != out) {
-                if (at + O <= a.hd)
-                    *reinterpret_cast<Vec<T, O>*>(out + at) = *reinterpret_cast<const Vec<T, O>*>(in + at);
-                else
-                    out[at] = in[at];
-            }
-            continue;
-        }
-        const int j = item * P;
-        float u[P], v[P];
-        if (HALVES) {
-            const Vec<T, P> x0 = *reinterpret_cast<const Vec<T, P>*>(in + j);
-            const Vec<T, P> x1 = *reinterpret_cast<const Vec<T, P>*>(in + half + j);
 #pragma unroll
-            for (int e = 0; e < P; ++e) {
-                u[e] = csdr::to_f32(x0.v[e]);
-                v[e] = csdr::to_f32(x1.v[e]);
-            }
-        } else {
-            const Vec<T, O> x = *reinterpret_cast<const Vec<T, O>*>(in + 2 * j);
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                u[e] = csdr::to_f32(x.v[2 * e]);
-                v[e] = csdr::to_f32(x.v[2 * e + 1]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < P; ++e) {
-            const float2 t = cs[j + e];
-            const float p = u[e] * t.x - v[e] * t.y;
-            v[e] = u[e] * t.y + v[e] * t.x;
-            u[e] = p;
-        }
-        if (HALVES) {
-            Vec<T, P> y0, y1;
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                y0.v[e] = (T)u[e];
-                y1.v[e] = (T)v[e];
-            }
-            *reinterpret_cast<Vec<T, P>*>(out + j) = y0;
-            *reinterpret_cast<Vec<T, P>*>(out + half + j) = y1;
-        } else {
-            Vec<T, O> y;
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-                y.v[2 * e] = (T)u[e];
-                y.v[2 * e + 1] = (T)v[e];
-            }
-            *reinterpret_cast<Vec<T, O>*>(out + 2 * j) = y;
-        }
+    for (int i = 0; i < AHEAD; ++i)
+        if (mine + i * step < all) put(t[i], u[i], v[i]);
+    for (int i = mine + AHEAD * step; i < all; i += step) {
+        t[0] = item_of(i);
+        load(t[0], u[0], v[0]);
+        put(t[0], u[0], v[0]);
     }
 }
 
 template <typename T>
 void launch(const Args& a, bool halves, bool wide, hipStream_t st) {
-    const unsigned grid = (unsigned)a.n_tokens * (unsigned)a.groups;
+    const unsigned grid = (unsigned)((a.n_tokens + a.tokens - 1) / a.tokens) * (unsigned)a.groups;
     if (halves) {
         if (wide) rotary_kernel<T, true, true><<<grid, kThreads, 0, st>>>(a);
         else rotary_kernel<T, true, false><<<grid, kThreads, 0, st>>>(a);
@@ -177,10 +190,12 @@ CSDR_API int csdr_rotary(const void* q, void* q_out, int Hq, int64_t q_stride, i
     a.dims = dims;
     a.magnitude = magnitude;
     const bool wide = dims % (2 * kUnit) == 0 && head_dim % (2 * kUnit) == 0;
-    // few tokens: their heads over more workgroups
+    // few tokens: their heads over more workgroups; many of few heads: several to a workgroup
     const long long items = (nq + nk) / (wide ? 2 * kUnit : 2);
-    a.groups = (int)std::min<long long>((items + kThreads - 1) / kThreads,
-                                        std::max(1, 1024 / n_tokens));
+    a.groups = (int)std::min<long long>((items + kThreads - 1) / kThreads, std::max(1, 1024 / n_tokens));
+    a.tokens = 1;
+    if (a.groups == 1 && n_tokens > 1024)
+        a.tokens = (int)std::max<long long>(1, std::min<long long>(kThreads / items, kMaxDim / dims));
     if ((long long)n_tokens * a.groups >= (1LL << 24))
         return set_error(CSDR_E_INVALID, "rotary: more than 2^24 - 1 tokens");
     hipStream_t st = static_cast<hipStream_t>(hip_stream);

@@ -37,6 +37,8 @@ CASES = [
     (1, 14, 2, 64, 64), (1, 1, 0, 2, 2), (3, 4, 2, 64, 32), (5, 32, 8, 128, 128), (2, 3, 1, 96, 96),
     (7, 5, 3, 80, 20), (4, 2, 2, 33, 6), (3, 2, 1, 47, 46), (600, 32, 32, 128, 32), (1100, 14, 2, 64, 64),
     (2, 3, 2, 1024, 1024), (3, 1, 1, 256, 16), (5, 2, 2, 72, 48), (5, 2, 2, 64, 60),
+    # several tokens to a workgroup, the last one's fewer
+    (1025, 3, 1, 64, 64), (3001, 1, 0, 64, 32), (2050, 2, 1, 33, 6), (1031, 1, 1, 16, 16), (5000, 1, 0, 2, 2),
 ]
 
 
@@ -66,6 +68,23 @@ def test_rotary(gpu, n, hq, hk, hd, dims, layout, dtype):
     rot.apply(q, p, k=k, q_out=q, k_out=k)
     assert torch.equal(q, qo) and torch.equal(k, ko)
     assert torch.equal(d[:, hq + hk:].cpu(), torch.from_numpy(x[:, hq + hk:]))
+
+
+@pytest.mark.parametrize("layout", ["adjacent", "halves"])
+def test_padding_among_many(gpu, layout):
+    """Rows without a token between others of one workgroup."""
+    from cortexsdr_amd.rotary import Rotary, frequencies
+
+    torch = gpu
+    r = np.random.default_rng(8)
+    x = r.standard_normal((1500, 2, 64)).astype(np.float32)
+    pos = r.integers(-3, 5000, 1500).astype(np.int32)
+    pos[r.random(1500) < 0.3] = -1
+    out = torch.full((1500, 2, 64), 9.0, device="cuda")
+    Rotary(64, layout=layout).apply(torch.from_numpy(x).cuda(), torch.from_numpy(pos).cuda(), q_out=out)
+    none = torch.from_numpy(pos < 0).cuda()
+    assert (out[none] == 9).all()
+    check(out[~none], x[pos >= 0], pos[pos >= 0], frequencies(64, 1e6), layout)
 
 
 @pytest.mark.parametrize("hd,dims", [(64, 64), (70, 50)])
