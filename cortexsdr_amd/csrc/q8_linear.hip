@@ -417,6 +417,7 @@ CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const
         return set_error(CSDR_E_INVALID, "q8_linear: a row stride is below R");
     if (add == y && M > 1 && (add_stride ? add_stride : R) != (y_stride ? y_stride : R))
         return set_error(CSDR_E_INVALID, "q8_linear: in place add and y must have the same stride");
+    if (y == w || y == x) return set_error(CSDR_E_INVALID, "q8_linear: y is an input");
     if (reinterpret_cast<uintptr_t>(w) % 16 || reinterpret_cast<uintptr_t>(x) % 16)
         return set_error(CSDR_E_INVALID, "q8_linear: codes must be 16-byte aligned");
     Args a{};

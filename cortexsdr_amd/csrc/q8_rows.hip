@@ -548,6 +548,7 @@ CSDR_API int csdr_q8_quantize(const void* x, const void* gate, int dtype, int ro
         return set_error(CSDR_E_INVALID, "q8_quantize: a row stride is below n");
     if (!aligned(codes, 16))
         return set_error(CSDR_E_INVALID, "q8_quantize: codes must be 16-byte aligned");
+    if (codes == x || codes == gate) return set_error(CSDR_E_INVALID, "q8_quantize: codes are an input");
     RowsArgs a{x, gate, codes, scales, x_stride ? x_stride : n, gate_stride ? gate_stride : n, n,
                (int)q8_pitch(n)};
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
@@ -571,6 +572,7 @@ CSDR_API int csdr_q8_dequantize(const int8_t* codes, const float* scales, int ro
     if (int rc = check_rows("q8_dequantize", rows, n)) return rc;
     if (!aligned(codes, 16))
         return set_error(CSDR_E_INVALID, "q8_dequantize: codes must be 16-byte aligned");
+    if (out == codes) return set_error(CSDR_E_INVALID, "q8_dequantize: out is codes");
     const int per_row = (n + 16 * 256 - 1) / (16 * 256);
     const long long blocks = (long long)rows * per_row;
     if (blocks >= (1LL << 24))
@@ -606,6 +608,8 @@ CSDR_API int csdr_add_rms_norm(const void* x, int dtype, int64_t x_stride, const
     if (residual && residual_out == residual && rows > 1 && residual_stride != 0 &&
         residual_stride != n)
         return set_error(CSDR_E_INVALID, "add_rms_norm: a stream updated in place must be packed");
+    if ((residual && residual_out == x) || (y && (y == x || y == residual || y == residual_out)))
+        return set_error(CSDR_E_INVALID, "add_rms_norm: an output is an input or another output");
     NormArgs a{};
     a.x = x;
     a.residual = residual;

@@ -183,6 +183,8 @@ CSDR_API int csdr_rotary(const void* q, void* q_out, int Hq, int64_t q_stride, i
     if (n_tokens > 1 && ((q == q_out && a.q.in_stride != a.q.out_stride) ||
                          (k && k == k_out && a.k.in_stride != a.k.out_stride)))
         return set_error(CSDR_E_INVALID, "rotary: in place both strides must be the same");
+    if (k && (q_out == k || k_out == q || q_out == k_out))
+        return set_error(CSDR_E_INVALID, "rotary: an output is the other's input or output");
     a.positions = positions;
     a.turns = turns;
     a.n_tokens = n_tokens;

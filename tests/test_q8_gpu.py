@@ -432,6 +432,33 @@ def test_streams(gpu):
         assert all(torch.equal(y, want[i][0]) and torch.equal(c, want[i][1]) for y, c in got[i])
 
 
+def test_rows_far(gpu):
+    """Offsets past 2^32 bytes: in the values, the codes, the stream and the way back."""
+    from cortexsdr_amd import q8
+
+    torch = gpu
+    n, rows = 131071, 33000
+    x = torch.zeros((rows, n), dtype=torch.float16, device="cuda")
+    last = activations(2, n, "f16", seed=1)
+    x[rows - 2:] = dev(torch, last)
+    r = q8.quantize(x)
+    assert not r.scales[:rows - 2].any() and not r.codes[rows - 3].any()
+    check_rows(q8.Q8Rows(r.codes[rows - 2:], r.scales[rows - 2:], n), last)
+    v = r.values("f16")
+    assert torch.equal(v[rows - 1], (r.scales[rows - 1] * r.codes[rows - 1, :n].float()).half())
+    assert not v[rows - 3].any()
+    del v
+    w = torch.ones(n, device="cuda")
+    normed = q8.rms_norm(x, w, residual=x, residual_out=None)
+    assert torch.equal(normed.residual[rows - 2:], x[rows - 2:] + x[rows - 2:])
+    h = (last.astype(np.float32) * 2).astype(np.float16)
+    rms, t = norm_parts(h, np.ones(n, np.float32), 1e-5)
+    check_rows(q8.Q8Rows(normed.rows.codes[rows - 2:], normed.rows.scales[rows - 2:], n), t, rms,
+               extra=(n + 8) * 2.0 ** -52)
+    del x, r, normed
+    torch.cuda.empty_cache()
+
+
 def test_python_refusals(gpu):
     from cortexsdr_amd import q8
 

@@ -9,7 +9,7 @@ from cortexsdr_amd.rotary import frequencies
 
 INVALID, UNSUPPORTED = -1, -6
 P = 4096  # aligned addresses that no refused call reads
-OUT = 2 * P
+OUT, OTHER, K, KO = 2 * P, 3 * P, 4 * P, 5 * P
 
 
 def refused(rc, status):
@@ -32,6 +32,7 @@ QUANTIZE = dict(x=P, gate=None, dtype=0, rows=2, n=100, xs=0, gs=0, codes=OUT, s
     (dict(rows=-1), INVALID), (dict(rows=1 << 22), INVALID), (dict(n=0), INVALID),
     (dict(n=-5), INVALID), (dict(n=131072), UNSUPPORTED), (dict(xs=99), INVALID),
     (dict(xs=-100), INVALID), (dict(gate=P, gs=99), INVALID), (dict(codes=OUT + 8), INVALID),
+    (dict(codes=P), INVALID), (dict(gate=OUT), INVALID),
 ])
 def test_quantize(over, status):
     a = {**QUANTIZE, **over}
@@ -43,7 +44,7 @@ def test_quantize(over, status):
     (dict(codes=None), INVALID), (dict(scales=None), INVALID), (dict(out=None), INVALID),
     (dict(dtype=2), INVALID), (dict(rows=0), INVALID), (dict(rows=1 << 22), INVALID),
     (dict(n=0), INVALID), (dict(n=131072), UNSUPPORTED), (dict(codes=P + 4), INVALID),
-    (dict(rows=(1 << 22) - 1, n=131071), INVALID),  # more workgroups than a launch may have
+    (dict(out=P), INVALID), (dict(rows=(1 << 22) - 1, n=131071), INVALID),  # more workgroups than a launch may have
 ])
 def test_dequantize(over, status):
     a = {**dict(codes=P, scales=P, rows=2, n=100, out=OUT, dtype=0), **over}
@@ -51,8 +52,8 @@ def test_dequantize(over, status):
                                            a["dtype"], None), status)
 
 
-NORM = dict(x=P, dtype=0, xs=0, res=P, rdt=0, rs=0, rout=OUT, w=P, eps=1e-5, rows=2, n=100, y=None,
-            codes=OUT, scales=P)
+NORM = dict(x=P, dtype=0, xs=0, res=K, rdt=0, rs=0, rout=OUT, w=P, eps=1e-5, rows=2, n=100, y=None,
+            codes=OTHER, scales=KO)
 
 
 @pytest.mark.parametrize("over,status", [
@@ -62,7 +63,8 @@ NORM = dict(x=P, dtype=0, xs=0, res=P, rdt=0, rs=0, rout=OUT, w=P, eps=1e-5, row
     (dict(rows=0), INVALID), (dict(rows=1 << 22), INVALID), (dict(n=0), INVALID),
     (dict(n=131072), UNSUPPORTED), (dict(eps=-1.0), INVALID), (dict(eps=math.nan), INVALID),
     (dict(eps=math.inf), INVALID), (dict(xs=99), INVALID), (dict(rs=99), INVALID),
-    (dict(codes=OUT + 8), INVALID), (dict(rout=P, rs=128), INVALID),
+    (dict(codes=OUT + 8), INVALID), (dict(rout=K, rs=128), INVALID), (dict(rout=P), INVALID),
+    (dict(y=P), INVALID), (dict(y=K), INVALID), (dict(y=OUT), INVALID),
 ])
 def test_norm(over, status):
     a = {**NORM, **over}
@@ -81,6 +83,7 @@ LINEAR = dict(w=P, ws=P, R=8, x=P, xs=P, M=4, C=100, bias=None, add=None, ads=0,
     (dict(dt=2), INVALID), (dict(ys=7), INVALID), (dict(add=P, ads=7), INVALID), (dict(w=P + 8), INVALID),
     (dict(x=P + 4), INVALID), (dict(M=1 << 22), INVALID), (dict(R=2 ** 31 - 1), INVALID),
     (dict(add=OUT, ads=16), INVALID),  # y in place with another stride
+    (dict(y=P), INVALID),
 ])
 def test_linear(over, status):
     a = {**LINEAR, **over}
@@ -89,7 +92,7 @@ def test_linear(over, status):
             status)
 
 
-ROTARY = dict(q=P, qo=OUT, Hq=4, qs=0, qos=0, k=P, ko=OUT, Hk=2, ks=0, kos=0, dt=0, n=3, hd=64, dims=64,
+ROTARY = dict(q=P, qo=OUT, Hq=4, qs=0, qos=0, k=K, ko=KO, Hk=2, ks=0, kos=0, dt=0, n=3, hd=64, dims=64,
               layout=0, pos=P, turns=P, mag=1.0)
 
 
@@ -102,7 +105,8 @@ ROTARY = dict(q=P, qo=OUT, Hq=4, qs=0, qos=0, k=P, ko=OUT, Hk=2, ks=0, kos=0, dt
     (dict(dims=0), UNSUPPORTED), (dict(dims=63), UNSUPPORTED), (dict(dims=66), UNSUPPORTED),
     (dict(mag=math.nan), INVALID), (dict(mag=math.inf), INVALID), (dict(qs=255), INVALID),
     (dict(qos=255), INVALID), (dict(ks=127), INVALID), (dict(kos=-128), INVALID),
-    (dict(qo=P, qs=512), INVALID), (dict(ko=P, kos=512), INVALID), (dict(n=1 << 24), INVALID),
+    (dict(qo=P, qs=512), INVALID), (dict(ko=K, kos=512), INVALID), (dict(n=1 << 24), INVALID),
+    (dict(qo=K), INVALID), (dict(ko=P), INVALID), (dict(ko=OUT), INVALID),
 ])
 def test_rotary(over, status):
     a = {**ROTARY, **over}

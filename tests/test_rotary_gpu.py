@@ -108,6 +108,24 @@ def test_no_tokens_and_padding(gpu, hd, dims):
     assert rot.apply(e, torch.empty(0, dtype=torch.int32, device="cuda")).shape == (0, 3, hd)
 
 
+def test_far(gpu):
+    """Tokens more than 2^32 bytes apart."""
+    from cortexsdr_amd.rotary import Rotary, frequencies
+
+    torch = gpu
+    buf = torch.empty((1 << 32) + 64, dtype=torch.float16, device="cuda")
+    x = buf.as_strided((3, 1, 64), (1 << 31, 64, 1))
+    h = np.random.default_rng(4).standard_normal((3, 1, 64)).astype(np.float16)
+    x.copy_(torch.from_numpy(h).cuda())
+    pos = np.array([3, 70000, 131071], np.int32)
+    p, rot = torch.from_numpy(pos).cuda(), Rotary(64, layout="halves")
+    check(rot.apply(x, p), h, pos, frequencies(64, 1e6), "halves")
+    rot.apply(x, p, q_out=x)
+    check(x, h, pos, frequencies(64, 1e6), "halves")
+    del buf, x
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("kv", ["f16", "q4"])
 def test_like_the_caches_own(gpu, kv, dtype):
