@@ -11,7 +11,7 @@
 //
 // A workgroup takes a row, and its values stay in registers between the pass that finds their largest and the
 // one that writes codes. Bound by memory: the norm of 4096 rows of 4096 in fp16 with its residual takes 22 us,
-// 5.3 TB/s; the gated rows of 4096 x 11008 in fp16 55 us, 4.1 TB/s (an exponential and a reciprocal a value, 30
+// 5.3 TB/s; the gated rows of 4096 x 11008 in fp16 49 us, 4.6 TB/s (an exponential and a reciprocal a value, 30
 // instructions in all, beside the loads); 22016 x 4096 fp32 weights 75 us, 6.0 TB/s; the way back to fp16 of
 // 4096 x 11008 22 us. Few rows are one round trip and two barriers (one row 3 us).
 //
@@ -33,6 +33,7 @@ using csdr::set_error;
 
 constexpr int kChunk = 8;  // consecutive values of a thread: one 8-byte store of codes
 constexpr int kMaxThreads = 1024;
+constexpr int kCUs = 256;
 constexpr int kMaxRows = (1 << 22) - 1;  // fewer than 2^32 threads a launch
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
@@ -489,32 +490,36 @@ __global__ __launch_bounds__(256) void values_kernel(const int8_t* codes, const 
     }
 }
 
-// Threads of a row and chunks a thread (0: more than the registers hold): one or two of them as long as 1024
-// threads are enough. With a thread's loads on their way together that was best at every number of rows (4096
-// gated rows of 11008 in fp16: 55 us with two, 59 with six; of 4864: 23 with two, 31 with one by 640 threads).
+// Threads of a row and chunks a thread (0: more than the registers hold). Many rows take up to 512 threads, so that more
+// of them are on a CU, one's loads beside another's codes (gated fp16 rows of 11008, 4096 of them: 47 to 50 us with
+// three chunks a thread, 54 to 57 with two; of 14336, 3000: 53 with four, 59 with two); few take as many as there may
+// be (64 gated rows of 14336: 6.8 us with two chunks, 7.8 with four).
 struct Shape {
     int threads, nv;
 };
-Shape shape_of(int width) {
-    const int chunks = (width + kChunk - 1) / kChunk;
-    const int nv = chunks <= 512 ? 1 : chunks <= 2 * kMaxThreads ? 2 : chunks <= 4 * kMaxThreads ? 4 : 0;
-    return {nv ? ((chunks + nv - 1) / nv + 63) / 64 * 64 : kMaxThreads, nv};
+Shape shape_of(int width, int rows) {
+    const int chunks = (width + kChunk - 1) / kChunk, want = rows < 2 * kCUs ? kMaxThreads : 512;
+    if (chunks > 4 * kMaxThreads) return {kMaxThreads, 0};
+    const int nv = std::min((chunks + want - 1) / want, 4);
+    return {((chunks + nv - 1) / nv + 63) / 64 * 64, nv};
 }
 
 template <typename TX, typename TR, bool RES>
 void launch_norm(const NormArgs& a, int rows, hipStream_t st) {
-    const Shape s = shape_of(a.codes ? a.pitch : a.n);
+    const Shape s = shape_of(a.codes ? a.pitch : a.n, rows);
     if (s.nv == 1) norm_kernel<TX, TR, RES, 1><<<rows, s.threads, 0, st>>>(a);
     else if (s.nv == 2) norm_kernel<TX, TR, RES, 2><<<rows, s.threads, 0, st>>>(a);
+    else if (s.nv == 3) norm_kernel<TX, TR, RES, 3><<<rows, s.threads, 0, st>>>(a);
     else if (s.nv == 4) norm_kernel<TX, TR, RES, 4><<<rows, s.threads, 0, st>>>(a);
     else norm_kernel<TX, TR, RES, 0><<<rows, s.threads, 0, st>>>(a);
 }
 
 template <typename T, bool GATE>
 void launch_rows(const RowsArgs& a, int rows, hipStream_t st) {
-    const Shape s = shape_of(a.pitch);
+    const Shape s = shape_of(a.pitch, rows);
     if (s.nv == 1) rows_kernel<T, GATE, 1><<<rows, s.threads, 0, st>>>(a);
     else if (s.nv == 2) rows_kernel<T, GATE, 2><<<rows, s.threads, 0, st>>>(a);
+    else if (s.nv == 3) rows_kernel<T, GATE, 3><<<rows, s.threads, 0, st>>>(a);
     else if (s.nv == 4) rows_kernel<T, GATE, 4><<<rows, s.threads, 0, st>>>(a);
     else rows_kernel<T, GATE, 0><<<rows, s.threads, 0, st>>>(a);
 }

@@ -36,7 +36,8 @@ def check_rows(rows, t, factor=1.0, extra=0.0):
 
 
 SHAPES = [(1, 1), (3, 2), (1, 896), (5, 100), (2, 127), (2, 128), (2, 129), (7, 1001), (3, 2049), (2, 4096),
-          (2, 5003), (64, 8192), (1, 11008), (3, 33000), (2, 131071)]
+          (2, 5003), (64, 8192), (1, 11008), (2, 20001), (3, 33000), (2, 131071)]
+MANY = [(515, 700), (513, 5003), (520, 9001), (512, 13001), (514, 17000)]  # up to 512 threads a row
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -193,6 +194,32 @@ def test_norm(gpu, rows, n, x_type, res_type):
     assert a.y is None and b.rows is None
     assert gpu.equal(a.rows.codes, r.rows.codes) and gpu.equal(a.rows.scales, r.rows.scales)
     assert gpu.equal(b.y, r.y)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,n", MANY)
+def test_many(gpu, rows, n, dtype):
+    """Many rows of each kind, some of them against the formulas, the others against calls of few rows."""
+    from cortexsdr_amd import q8
+
+    torch = gpu
+    both = activations(rows, 2 * n, dtype, seed=n)
+    d, w = dev(torch, both), dev(torch, np.linspace(0.5, 2, n).astype(np.float32))
+    x, g = d[:, n:], d[:, :n]
+    pick = [0, 1, rows // 2, rows - 1]
+    h = (both[pick, n:].astype(np.float32) + both[pick, :n].astype(np.float32)).astype(NP[dtype])
+    rms, t = norm_parts(h, w.cpu().numpy(), 1e-5)
+    kinds = [(lambda a, b: q8.quantize(a), both[pick, n:], 1.0, 0.0),
+             (lambda a, b: q8.quantize(a, gate=b), q8_ref.silu_mul(both[pick, :n], both[pick, n:]), 1.0, 0.0),
+             (lambda a, b: q8.rms_norm(a, w, residual=b).rows, t, rms, (n + 8) * 2.0 ** -52)]
+    for f, v, factor, extra in kinds:
+        r = f(x, g)
+        check_rows(q8.Q8Rows(r.codes[pick], r.scales[pick], n), v, factor, extra)
+        for first in range(0, rows, 100):
+            few = f(x[first:first + 100], g[first:first + 100])
+            assert torch.equal(few.codes, r.codes[first:first + 100])
+            # (a norm's sum of squares in another order)
+            assert ((few.scales - r.scales[first:first + 100]).abs() <= 2 * U32 * few.scales).all()
 
 
 @pytest.mark.parametrize("n", [100, 4096, 40000])
