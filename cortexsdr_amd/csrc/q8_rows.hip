@@ -2,7 +2,8 @@
 // residual's addition, from values as they are, or from silu(gate) * x; and back to values (gfx950).
 //
 // A row v: top = max |v|, code = rint(127 v / top) (ties to even), scale = top / 127 in fp32. The codes are
-// those of exact arithmetic, so that a code does not depend on the order of a sum or on which kernel made it.
+// those of exact arithmetic (of a gated value as fp64 holds it), so that a code does not depend on the order
+// of a sum or on which kernel made it.
 // The norm's 1 / rms is in every value of a row and cancels in its codes: they come from t = h w alone, a
 // product of two fp32 numbers that fp64 holds exactly, and one pass over the row gives both the sum of squares
 // (fp64) and top. Values, their largest and their codes are formed in fp32, and in fp64 only where that may not

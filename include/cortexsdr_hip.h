@@ -672,8 +672,8 @@ CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
  * A layer in 8 bits: rows of codes with a scale each, and their products
  * ==================================================================== */
 
-/* A row of n values v as 8-bit codes: code = round(127 v / max|v|), ties to even, in exact arithmetic,
- * scale = max|v| / 127 (fp32), a value being scale * code. A row of zeros has the scale 0; one that
+/* A row of n values v as 8-bit codes: code = round(127 v / max|v|), ties to even, in exact arithmetic
+ * (of a gated value as fp64 holds it), scale = max|v| / 127 (fp32), a value being scale * code. A row of zeros has the scale 0; one that
  * holds a value which is not finite, or whose scale passes fp32, the scale NaN and codes 0. Rows of codes
  * lie csdr_q8_pitch(n) bytes apart (n up to a whole number of 128; 0 for an n outside 1..131071), zeros
  * behind the last value, 16-byte aligned, with `rows` scales (device memory throughout). At most
