@@ -374,14 +374,16 @@ struct RowsArgs {
 };
 
 // silu(g) x. exp(-g) = 2^p (1 + rest ln 2), p and the rest of its rounding from two parts of 1 / ln 2, so that
-// a large gate costs no bits; beyond kLow the gate is held where the exponential is still a number, and above
-// 150 it is nothing beside 1.
+// a large gate costs no bits; beyond kLow the gate is held where the sigmoid is a normal number, and above 150 the
+// exponential is nothing beside 1. The sigmoid comes last: a subnormal gate has all its bits in g x (gate times sigmoid
+// would round to a few), where g x is itself subnormal the value is far below kTiny / 127, and where g x passes fp32 the
+// value is infinite here, so that its row is formed in fp64.
 __device__ __forceinline__ float gated(float g, float x) {
     constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596299e-8f, kLn2 = 0.69314718f;
-    const float v = __builtin_amdgcn_fmed3f(-g, -150.0f, 88.0f), p = v * kHi;
+    const float v = __builtin_amdgcn_fmed3f(-g, -150.0f, -kLow), p = v * kHi;
     const float rest = fmaf(v, kLo, fmaf(v, kHi, -p));
     const float e2 = __builtin_amdgcn_exp2f(p), e = fmaf(e2, rest * kLn2, e2);
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * x;
+    return g * x * __builtin_amdgcn_rcpf(1.0f + e);
 }
 __device__ __forceinline__ double gated(double g, double x) { return g / (1.0 + exp(-g)) * x; }
 
