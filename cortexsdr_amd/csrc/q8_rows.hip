@@ -2,8 +2,8 @@
 // residual's addition, from values as they are, or from silu(gate) * x; and back to values (gfx950).
 //
 // A row v: top = max |v|, code = rint(127 v / top) (ties to even), scale = top / 127 in fp32. The codes are
-// those of exact arithmetic (of a gated value as fp64 holds it), so that a code does not depend on the order
-// of a sum or on which kernel made it.
+// those of exact arithmetic (of a gated value as fp64 forms it, but within 2^-42 of a border), so that a code does
+// not depend on the order of a sum or on which kernel made it.
 // The norm's 1 / rms is in every value of a row and cancels in its codes: they come from t = h w alone, a
 // product of two fp32 numbers that fp64 holds exactly, and one pass over the row gives both the sum of squares
 // (fp64) and top. Values, their largest and their codes are formed in fp32, and in fp64 only where that may not
@@ -189,17 +189,30 @@ __device__ __forceinline__ Scale scale_of(double top, double factor, bool wide) 
     return s;
 }
 
-// In exact arithmetic, but for 1e-13 of the product with the reciprocal: divided where that lies next to a
-// border.
+// The nearest code of t, in exact arithmetic but for 1e-13 of the product with the reciprocal. Next to a border (k + 1/2
+// of a code) of |t|, EXACT (for t and top of 48 bits, products of two fp32 numbers): 254 |t| against (2 k + 1) top, the
+// second as a product and what it is rounded by, and their difference, a multiple of top's last place, too small to be
+// rounded; ties to even. Otherwise the quotient as fp64 rounds it: a gated value has fp64's roundings in itself, and
+// values of one gate that tie in the formula are to tie here.
+template <bool EXACT>
 __device__ __forceinline__ int code_of(double t, const Scale& s) {
     const double q = t * s.inv;
     double r = rint(q);
-    if (__builtin_expect(fabs(fabs(q - r) - 0.5) < 1e-9, 0)) r = rint(127.0 * t / s.top);
+    if (__builtin_expect(fabs(fabs(q - r) - 0.5) < 1e-9, 0)) {
+        if (EXACT) {
+            const double k = floor(fabs(q)), odd = 2.0 * k + 1.0, border = odd * s.top;
+            const double over = fma(254.0, fabs(t), -border), rounded = fma(odd, s.top, -border);
+            const bool up = over > rounded || (over == rounded && ((int)k & 1));
+            r = copysign(up ? k + 1.0 : k, t);
+        } else {
+            r = rint(127.0 * t / s.top);
+        }
+    }
     return (int)r;
 }
 
 // The codes of a chunk's values t, exact(i) being value i in fp64. 3 2^22 + q holds rint(q) in its low bits.
-template <typename Exact>
+template <bool EXACT, typename Exact>
 __device__ __forceinline__ void put_codes(int8_t* p, const float* t, const Scale& s, Exact exact) {
     u2 v = {0, 0};
     if (s.inv > 0.0) {
@@ -216,7 +229,7 @@ __device__ __forceinline__ void put_codes(int8_t* p, const float* t, const Scale
         if (__builtin_expect(most > 0.5f - kCodeOff || s.wide, 0)) {
 #pragma unroll
             for (int i = 0; i < kChunk; ++i)
-                if (d[i] > 0.5f - kCodeOff || s.wide) c[i] = (uint32_t)code_of(exact(i), s);
+                if (d[i] > 0.5f - kCodeOff || s.wide) c[i] = (uint32_t)code_of<EXACT>(exact(i), s);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -350,8 +363,8 @@ __global__ __launch_bounds__(kMaxThreads) void norm_kernel(NormArgs a) {
     if (a.codes)
         each(a.pitch, [&](int j, int at) {
             again(at);
-            put_codes(a.codes + row * a.pitch + at, t[j], s,
-                      [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
+            put_codes<true>(a.codes + row * a.pitch + at, t[j], s,
+                            [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
         });
     if (a.y)
         each(a.n, [&](int, int at) {
@@ -465,8 +478,8 @@ __global__ __launch_bounds__(kMaxThreads) void rows_kernel(RowsArgs a) {
     if (threadIdx.x == 0) a.scales[row] = s.value;
     each(a.pitch, [&](int j, int at) {
         again(at);
-        put_codes(a.codes + row * a.pitch + at, t[j], s,
-                  [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
+        put_codes<!GATE>(a.codes + row * a.pitch + at, t[j], s,
+                         [&](int i) { return at + i < a.n ? exact(at + i) : 0.0; });
     });
 }
 

@@ -673,10 +673,11 @@ CSDR_API int csdr_token_logprobs(const void* logits, int dtype, int rows, int n,
  * ==================================================================== */
 
 /* A row of n values v as 8-bit codes: code = round(127 v / max|v|), ties to even, in exact arithmetic
- * (of a gated value as fp64 holds it), scale = max|v| / 127 (fp32), a value being scale * code. A row of zeros has the scale 0; one that
- * holds a value which is not finite, or whose scale passes fp32, the scale NaN and codes 0. Rows of codes
- * lie csdr_q8_pitch(n) bytes apart (n up to a whole number of 128; 0 for an n outside 1..131071), zeros
- * behind the last value, 16-byte aligned, with `rows` scales (device memory throughout). At most
+ * (a gated value is formed in fp64: its code is the nearest but where it lies within 2^-42 of a border
+ * between two), scale = max|v| / 127 (fp32), a value being scale * code. A row of zeros has the scale 0;
+ * one that holds a value which is not finite, or whose scale passes fp32, the scale NaN and codes 0. Rows
+ * of codes lie csdr_q8_pitch(n) bytes apart (n up to a whole number of 128; 0 for an n outside 1..131071),
+ * zeros behind the last value, 16-byte aligned, with `rows` scales (device memory throughout). At most
  * 2^22 - 1 rows. */
 CSDR_API size_t csdr_q8_pitch(int n);
 /* The rows of x, or of silu(gate) * x (silu_mul, cortex_sdk.cpp:1245-1256) if gate is not NULL: `rows`
