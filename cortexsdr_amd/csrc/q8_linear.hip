@@ -59,11 +59,15 @@ typedef float f4 __attribute__((ext_vector_type(4)));
     return v;
 }
 
+// A sum times both scales. With a channel's scale below kLarge first the product passes fp32 in no sum (at most 2^31)
+// and, as a whole number of the scale's last place, loses nothing below the normal numbers; from there on the token's
+// scale goes first, and where that product passes fp32 the result does.
+constexpr float kLarge = 0x1p96f;
 [[maybe_unused]] __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
-    return (float)sum * xs * ws + bias;
+    return (float)sum * ws * xs + bias;
 }
 
-// Four neighbouring outputs of a token at once (r + 3 < R, m < M).
+// Four neighbouring outputs of a token at once (r + 3 < R, m < M, no large scale among theirs).
 template <typename T>
 __device__ __forceinline__ void finish_four(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
                                             const f4& bias, const Four<T>& add) {
@@ -73,7 +77,7 @@ __device__ __forceinline__ void finish_four(const Args& a, int m, int r, const i
     *reinterpret_cast<Four<T>*>(static_cast<T*>(a.y) + m * a.y_stride + r) = o;
 }
 
-// One by one, as many of them as there are.
+// One by one, as many of them as there are, with any scales.
 template <typename T>
 __device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& sum, float xs, const f4& ws,
                                        const f4& bias) {
@@ -82,8 +86,10 @@ __device__ __forceinline__ void finish(const Args& a, int m, int r, const i4& su
     const T* add = static_cast<const T*>(a.add) + m * a.add_stride + r;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (r + i < a.R)
-            y[i] = (T)(scaled(sum[i], xs, ws[i], bias[i]) + (a.add ? (float)add[i] : 0.0f));
+        if (r + i < a.R) {
+            const bool large = fabsf(ws[i]) >= kLarge;
+            y[i] = (T)(scaled(sum[i], large ? ws[i] : xs, large ? xs : ws[i], bias[i]) + (a.add ? (float)add[i] : 0.0f));
+        }
 }
 
 typedef __attribute__((address_space(3))) void* LdsPtr;
@@ -272,7 +278,8 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
     const int r = r0 + 4 * c;
     const f4 ws = four_of(a.w_scales, min(r, a.R - 1), a.R);
     const f4 bias = a.bias ? four_of(a.bias, min(r, a.R - 1), a.R) : f4{};
-    const bool whole = r + 3 < a.R;
+    const float most = fmaxf(fmaxf(fabsf(ws[0]), fabsf(ws[1])), fmaxf(fabsf(ws[2]), fabsf(ws[3])));
+    const bool whole = r + 3 < a.R && !(most >= kLarge);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         arrived<0>();  // every wave is done with what lay there
