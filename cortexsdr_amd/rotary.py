@@ -50,7 +50,9 @@ def frequencies(dims: int, theta: float = 1e6, scaling: str = "none", factor: fl
 class Rotary:
     """The rotation of heads of head_dim: of their first `dims` dims (0: all), as "adjacent" pairs
     (2 j, 2 j + 1) or "halves" (j, j + dims / 2). The frequencies are those of frequencies(), or
-    given: dims / 2 numbers, radians per position. Sine and cosine are multiplied by magnitude."""
+    given: dims / 2 numbers, radians per position. Sine and cosine are multiplied by magnitude. It may
+    be dropped while its calls are queued, on any stream; a captured one needs it until its graph's
+    last replay."""
 
     def __init__(self, head_dim: int, theta: float = 1e6, dims: int = 0, layout: str = "adjacent",
                  scaling: str = "none", factor: float = 1.0, original: int = 0, low: float = 1.0,
@@ -71,6 +73,8 @@ class Rotary:
         self._turns = torch.tensor([f / (2 * math.pi) for f in freqs], dtype=torch.float64,
                                    device="cuda")
         self._at = self._turns.data_ptr()
+        # the streams that the table's memory waits for before it is given to another tensor
+        self._streams = {_stream_of(torch, self._turns.get_device(), None)}
         self._call = _lib.load().csdr_rotary
 
     def _stride(self, what: str, x, n: int) -> int:
@@ -118,10 +122,13 @@ class Rotary:
             raise ValueError("k_out without k")
         dev = _on_device(torch, "tensors", q, k, q_out, k_out, positions, self._turns)
         if n:
+            on = _stream_of(torch, dev, stream)
+            if on not in self._streams:
+                self._turns.record_stream(torch.cuda.current_stream() if stream is None else stream)
+                self._streams.add(on)
             rc = self._call(q.data_ptr(), q_out.data_ptr(), _int(q.shape[1]), qs, qos, kp, kop, _int(hk),
                             ks, kos, dt, _int(n), self.head_dim, self.dims, self._layout,
-                            positions.data_ptr(), self._at, self.magnitude,
-                            _stream_of(torch, dev, stream))
+                            positions.data_ptr(), self._at, self.magnitude, on)
             if rc:
                 _check(rc)
         return q_out if k is None else (q_out, k_out)
