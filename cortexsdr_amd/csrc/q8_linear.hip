@@ -199,6 +199,8 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
     };
     constexpr int NF = FR + FM, N = FR * FM;
     constexpr bool OUT = N >= 4;  // products written out: three others at least between two of a sum
+    // (a group without a last step would end on products written out, with nothing to wait for their sums)
+    static_assert(KG == 1 || !OUT, "waves that share the columns end on builtin products");
     i4 acc[FR][FM] = {};
 #pragma unroll
     for (int i = 0; i < FR; ++i)
@@ -260,10 +262,6 @@ __global__ __launch_bounds__(64 * KG * WR * WM) void tile_kernel(Args a, int til
 #pragma unroll
             for (int j = 0; j < FM; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[1][i], xf[1][j], acc[i][j], 0, 0, 0);
-    } else if constexpr (OUT) {  // the last products of these waves were written out: until their sums are there
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
     }
     // The sums go through LDS (token-major, 16-byte chunk c of token m at c ^ (m % 8)): a thread then has
     // neighbouring rows for whole lines of y, and a short loop writes them, eight tokens' reads of `add`
