@@ -629,7 +629,8 @@ CSDR_API int csdr_add_rms_norm(const void* x, int dtype, int64_t x_stride, const
     if (residual && residual_out == residual && rows > 1 && residual_stride != 0 &&
         residual_stride != n)
         return set_error(CSDR_E_INVALID, "add_rms_norm: a stream updated in place must be packed");
-    if ((residual && residual_out == x) || (y && (y == x || y == residual || y == residual_out)))
+    if ((residual && residual_out == x) || (y && (y == x || y == residual || y == residual_out)) ||
+        (codes && (codes == x || codes == residual || codes == residual_out || codes == y)))
         return set_error(CSDR_E_INVALID, "add_rms_norm: an output is an input or another output");
     NormArgs a{};
     a.x = x;
