@@ -7,14 +7,18 @@
 // waves between), several stages ahead; a wave reads its operands for the next half step while the matrix cores
 // work on this one, with one barrier a stage. What bounds it, by the number of tokens (times of launches in a
 // graph):
-//   one to 16    the stream of the weights: 22016 x 4096 for one token 18 us, 5.0 TB/s; small ones the chain of a
-//                launch, first loads, barrier, sums (1152 x 896 2.7 us)
-//   up to some   what a CU takes from L2, 30 to 42 bytes a cycle: 64 tokens, 4096 x 11008, 12.8 us; there large tiles
-//   hundreds     take fewer bytes and leave CUs without work, so tiles are chosen by what they cost (kCosts)
+//   one to 16    the stream of the weights: 22016 x 4096 for one token 18 us with them in the Infinity Cache, 23 us (3.9
+//                TB/s) where 720 MB of them are read in turn; small ones the chain of a launch, first loads,
+//                barrier, sums (1152 x 896 2.9 us)
+//   up to some   reads of L2: 12 to 14 TB/s over a launch with its start and end, three quarters of them hits or more,
+//   hundreds     the matrix cores busy in a tenth to a quarter of the time: 64 tokens, 4096 x 11008, 14 us (18 with
+//                500 MB of weights in turn); there large tiles take fewer bytes and leave CUs without work, so tiles
+//                are chosen by what they cost (kCosts)
 //   thousands    the matrix cores at the clock that they can be fed at: 4096 tokens, 4096 x 11008, 135 us, 2.74
-//                POPS, 65% of the cycles at 1.97 GHz (nothing but the products runs at 1.9 GHz, 3.9 POPS; taking the
-//                same rows for every tile, so that all loads hit L2, changes nothing, nor does the order of
-//                loads, reads and products, nor the waves' priority); 12 us of it start and end, 67 MB of y and `add`
+//                POPS, busy in 68% of the cycles counted around a launch (nothing but the products runs at 1.9
+//                GHz, 3.9 POPS; taking the same rows for every tile, so that all loads hit L2, changes nothing, nor
+//                does the order of loads, reads and products, nor the waves' priority); 12 us of it start and end,
+//                67 MB of y and `add`
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -354,9 +358,10 @@ int launch_tiles(const Args& a, hipStream_t st) {
 
 // What a tile costs, in us: `fixed` for a workgroup's start and end, a step of 128 columns `alone` for one
 // workgroup on a CU and `each` for every one of `held` (as many as a CU's LDS holds). Fitted to products of 1
-// to 4096 tokens with 1152 to 11008 rows and 896 to 11008 columns, which they give within a tenth to a fifth;
-// the rule has only to tell tiles apart. Both sides of its borders, measured for 4096 x 4096: 64 tokens 6.3 us
-// in tiles of 32 x 32, 8.1 of 32 x 64; 128 tokens 8.1 of 32 x 32, 8.2 of 32 x 64, 10.6 of 64 x 64; 512 tokens
+// to 4096 tokens with 1152 to 11008 rows and 896 to 11008 columns whose codes lie in the Infinity Cache, which they
+// give within a tenth to a fifth; the rule has only to tell tiles apart. Codes from memory have no term in it (one
+// token, 22016 x 4096: 13.6 us here, 18 to 23 measured). Both sides of its borders, measured for 4096 x 4096: 64 tokens
+// 6.3 us in tiles of 32 x 32, 8.1 of 32 x 64; 128 tokens 8.1 of 32 x 32, 8.2 of 32 x 64, 10.6 of 64 x 64; 512 tokens
 // 13.8 of 128 x 64, 15 of 64 x 64, 22.7 of 128 x 128; 2048 tokens 34 of 128 x 128, 42 of 128 x 64, 46 of 256 x
 // 256; 4096 tokens 58 of 256 x 256, 66 of 128 x 128.
 struct Cost {

@@ -687,11 +687,11 @@ CSDR_API size_t csdr_q8_pitch(int n);
 CSDR_API int csdr_q8_quantize(const void* x, const void* gate, int dtype, int rows, int n,
                               int64_t x_stride, int64_t gate_stride, int8_t* codes, float* scales,
                               void* hip_stream);
-/* out (rows x n, packed, of dtype) = scale * code. */
+/* out (rows x n, packed, of dtype) = scale * code. rows times n up to a whole number of 4096 below 2^36. */
 CSDR_API int csdr_q8_dequantize(const int8_t* codes, const float* scales, int rows, int n, void* out,
                                 int dtype, void* hip_stream);
 /* RMSNorm (rms_norm, cortex_sdk.cpp:1208-1232) with the residual's addition in front and 8-bit rows behind:
- * h = x, or x + residual rounded to residual_dtype and written to residual_out (rows x n, packed; it may
+ * h = x, or x + residual in fp32, rounded to residual_dtype and written to residual_out (rows x n, packed; it may
  * be residual itself where that is packed) if residual is not NULL; the norm h / sqrt(mean(h^2) + eps) * w
  * (statistics in fp64; without eps a row of zeros is NaN) goes to codes and scales (both or neither), to
  * y (rows x n, packed, of x's dtype; may be NULL), or to both. Strides in elements, 0 = n. Outputs must
@@ -724,7 +724,7 @@ CSDR_API int csdr_q8_linear(const int8_t* w, const float* w_scales, int R, const
  * and reduced in fp64), times magnitude; the other dims as they are. positions: n_tokens ints (device); a
  * token with a negative one is none, its rows are not written. Strides in elements from one token to the
  * next, 0 = heads x head_dim; q_out may be q, with q's stride, and k_out k; outputs must not overlap
- * inputs otherwise. head_dim at most 1024. */
+ * inputs otherwise. head_dim at most 1024, 65535 heads of each, 2^24 - 1 tokens. */
 CSDR_API int csdr_rotary(const void* q, void* q_out, int Hq, int64_t q_stride, int64_t q_out_stride,
                          const void* k, void* k_out, int Hk, int64_t k_stride, int64_t k_out_stride,
                          int dtype, int n_tokens, int head_dim, int dims, int layout,
