@@ -11,8 +11,8 @@
 //                TB/s) where 720 MB of them are read in turn; small ones the chain of a launch, first loads,
 //                barrier, sums (1152 x 896 2.9 us)
 //   up to some   reads of L2: 12 to 14 TB/s over a launch with its start and end, three quarters of them hits or more,
-//   hundreds     the matrix cores busy in a tenth to a quarter of the time: 64 tokens, 4096 x 11008, 14 us (18 with
-//                500 MB of weights in turn); there large tiles take fewer bytes and leave CUs without work, so tiles
+//   hundreds     the matrix cores busy in a tenth to a quarter of the time: 64 tokens, 4096 x 11008, 13 us (18 with
+//                540 MB of weights in turn); there large tiles take fewer bytes and leave CUs without work, so tiles
 //                are chosen by what they cost (kCosts)
 //   thousands    the matrix cores at the clock that they can be fed at: 4096 tokens, 4096 x 11008, 135 us, 2.74
 //                POPS, busy in 68% of the cycles counted around a launch (nothing but the products runs at 1.9
