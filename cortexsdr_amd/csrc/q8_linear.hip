@@ -10,7 +10,7 @@
 //   one to 16    the stream of the weights: 22016 x 4096 for one token 18 us with them in the Infinity Cache, 23 us (3.9
 //                TB/s) where 720 MB of them are read in turn; small ones the chain of a launch, first loads,
 //                barrier, sums (1152 x 896 2.9 us)
-//   up to some   reads of L2: 12 to 14 TB/s over a launch with its start and end, three quarters of them hits or more,
+//   up to some   reads of L2: 12 to 14 TB/s over a launch with its start and end, seven tenths of them hits or more,
 //   hundreds     the matrix cores busy in a tenth to a quarter of the time: 64 tokens, 4096 x 11008, 13 us (18 with
 //                540 MB of weights in turn); there large tiles take fewer bytes and leave CUs without work, so tiles
 //                are chosen by what they cost (kCosts)
